@@ -24,6 +24,7 @@ extern "C" {
 #endif
 
 typedef struct pg_linear pg_linear; /* bf16 weights [experts][N][K] on the device */
+typedef struct pg_linear4 pg_linear4; /* weights of 4 bits with a scale per group of K, [experts][N][K] */
 typedef struct pg_route pg_route;   /* which token goes to which expert, rebuilt in every step */
 
 typedef enum pg_dtype { PG_F32 = 0, PG_BF16 = 1 } pg_dtype;
@@ -58,6 +59,25 @@ PG_API int32_t pg_linear_run_ld(pg_ctx *ctx, pg_linear *lin, const void *d_a, in
  * (its token) of a, else row r; y has one row per row of the route. */
 PG_API int32_t pg_linear_run_routed(pg_ctx *ctx, pg_linear *lin, pg_route *route, const void *d_a, int32_t dtype, int32_t by_token, int32_t act,
                                     float limit, void *d_y, int32_t y_dtype, int64_t ldy);
+
+/* ---- products with weights of 4 bits: W[n][k] = scale[n][k / group] * (q[n][k] - 8), q 0 .. 15, groups of 32, 64 or 128 ----
+ * Activations are bf16 (PG_BF16); K is a multiple of 64 and of the group.  A handle holds a copy of the weights in a layout of its own; making
+ * one waits until it is made, and cannot be recorded.
+ * From quants [experts][n][k / 2], two a byte with the first in the low half, and bf16 scales [experts][n][k / group]: */
+PG_API int32_t pg_linear4_pack(pg_ctx *ctx, const void *d_q, const void *d_scales_bf16, int64_t n, int64_t k, int64_t group, int64_t experts, pg_linear4 **out);
+/* From bf16 weights [experts][n][k]: scale = bf16(v / -8), v the group's value of largest magnitude (the first of equals), q = clamp(rint(w / scale) + 8, 0, 15).
+ * A group with a value that is not finite has the scale not-a-number. */
+PG_API int32_t pg_linear4_quantize(pg_ctx *ctx, const void *d_w_bf16, int64_t n, int64_t k, int64_t group, int64_t experts, pg_linear4 **out);
+PG_API int32_t pg_linear4_free(pg_ctx *ctx, pg_linear4 *lin);
+PG_API int64_t pg_linear4_bytes(const pg_linear4 *lin);
+/* the weights' values, f32 [experts][n][k] */
+PG_API int32_t pg_linear4_read(pg_ctx *ctx, const pg_linear4 *lin, float *d_w);
+/* as pg_linear_run_ld; sums are of the bf16 activations with the weights' values, in f32 */
+PG_API int32_t pg_linear4_run(pg_ctx *ctx, const pg_linear4 *lin, const void *d_a, int64_t lda, int32_t dtype, int64_t m, int32_t act, float limit, void *d_y,
+                              int32_t y_dtype, int64_t ldy);
+/* as pg_linear_run_routed */
+PG_API int32_t pg_linear4_run_routed(pg_ctx *ctx, const pg_linear4 *lin, const pg_route *route, const void *d_a, int32_t dtype, int32_t by_token, int32_t act, float limit,
+                                     void *d_y, int32_t y_dtype, int64_t ldy);
 
 /* ---- mixture of experts: softmax scores, corrected choice, groups, identity experts ---- */
 PG_API int32_t pg_route_create(pg_ctx *ctx, int64_t max_tokens, int64_t experts, int64_t identity, int64_t top, pg_route **out);

@@ -184,6 +184,13 @@ LM_SIGNATURES = {
     "pg_linear_run": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _f, _vp, _i32, _i64]),
     "pg_linear_run_ld": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _f, _vp, _i32, _i64]),
     "pg_linear_run_routed": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _f, _vp, _i32, _i64]),
+    "pg_linear4_pack": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, C.POINTER(_vp)]),
+    "pg_linear4_quantize": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, C.POINTER(_vp)]),
+    "pg_linear4_free": (_i32, [_vp, _vp]),
+    "pg_linear4_bytes": (_i64, [_vp]),
+    "pg_linear4_read": (_i32, [_vp, _vp, _vp]),
+    "pg_linear4_run": (_i32, [_vp, _vp, _vp, _i64, _i32, _i64, _i32, _f, _vp, _i32, _i64]),
+    "pg_linear4_run_routed": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _f, _vp, _i32, _i64]),
     "pg_route_create": (_i32, [_vp, _i64, _i64, _i64, _i64, C.POINTER(_vp)]),
     "pg_route_free": (_i32, [_vp, _vp]),
     "pg_route_max_rows": (_i64, [_vp]),

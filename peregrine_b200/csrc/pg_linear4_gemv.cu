@@ -1,0 +1,361 @@
+// Decode-size product y = act(a W^T) with weights of 4 bits (csrc/pg_linear4.cu), at most 16 rows, one pass over the weights.
+//
+//   * The weights are the M side of mma.sync m16n8k16 (16 rows x 16 k), activation rows its 8 columns; up to 16 rows of a take two column
+//     tiles on the same unpacked quants.  Quants become f16 integers (exact), sums of a group are scaled in f32.
+//   * The activations are bf16 and enter as f16: a warp divides each row of its part of K by a power of two of its own (four_range) and
+//     multiplies the sums back, so nothing is rounded that could be seen in an f32 sum.
+//   * One persistent CTA of 16 warps per SM.  `kw` warps share a tile of 16 weight rows, each with one part of K of at most 256 elements, whose
+//     activations it keeps in registers; a fill of its ring is two bulk copies, quants (up to 2 KB) and scales.  The parts meet in shared memory
+//     in a fixed order; the warps of a tile take turns in adding.
+//   * K beyond 16 x 256 (SPLIT): sp CTAs take the same tiles, their sums go to slabs, the last one in (a ticket) adds in a fixed order.
+//   * ROUTED: rows come in blocks of 16 that share an expert.
+//
+// Every mbarrier wait is bounded; a warp that gave up goes on through the remaining barriers without computing.
+#include <algorithm>
+
+#include "pg_async.cuh"
+#include "pg_four.cuh"
+
+namespace {
+
+constexpr int V4_WARPS = 16, V4_THREADS = V4_WARPS * 32;
+constexpr int V4_SLOTS = 5;
+constexpr int V4_KW_MAX = 256;
+constexpr int V4_Q = V4_KW_MAX / 64 * 512, V4_SLOT = V4_Q + V4_KW_MAX / 32 * 32;   // quants, then scales of groups of 32 at worst
+constexpr int V4_RING = V4_WARPS * V4_SLOTS * V4_SLOT;
+
+// shared memory: ring | partial sums [2][16 warps][32 lanes][4 NT] | barriers
+// slabs (SPLIT): [sp][items][32 lanes][4 NT]
+template <int ACT, int NT, bool ROUTED, bool SPLIT, typename TY>
+__global__ void __launch_bounds__(V4_THREADS, 1)
+    linear4_gemv_kernel(const bf16 *__restrict__ a, int64_t lda, int M, const uint4 *__restrict__ wq, const __half *__restrict__ ws, const float *__restrict__ wrow, int N,
+                        int K, int group, int tiles, int kw, int KW, int KH, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, int sp, float *slabs,
+                        unsigned int *tickets, int32_t *status, unsigned long long limit_ns)
+{
+    constexpr int CELL = 4 * NT;                          // floats per lane
+    extern __shared__ __align__(128) unsigned char smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
+    const int my_part = SPLIT ? (int)blockIdx.x % sp : 0;
+    const int groups = V4_WARPS / kw, slot_idx = warp / kw, kpart = warp - slot_idx * kw;
+    float *part = reinterpret_cast<float *>(smem + V4_RING);
+    unsigned char *tail = reinterpret_cast<unsigned char *>(part + 2 * V4_WARPS * 32 * CELL);
+    const uint32_t my_bar = pg_smem(tail) + (uint32_t)warp * (V4_SLOTS * 8);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + V4_WARPS * V4_SLOTS * 8);
+    const uint32_t ring = pg_smem(smem) + (uint32_t)warp * (V4_SLOTS * V4_SLOT);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < V4_WARPS * V4_SLOTS; i++) pg_mbar_init(pg_smem(tail) + 8 * i, 1);
+        *abort_flag = 0;
+        pg_mbar_fence();
+    }
+    __syncthreads();
+
+    const int ka0 = my_part * KH, k0 = ka0 + kpart * KW;
+    const int klen = max(0, min(KW, min(K, ka0 + KH) - k0));   // a multiple of 64 and of the group; 0 only in a short last range
+    const int64_t unit = SPLIT ? blockIdx.x / sp : blockIdx.x, units = SPLIT ? gridDim.x / sp : gridDim.x;
+    if (ROUTED) asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int nblk = ROUTED ? __ldcg(rt.blocks) : 1;
+    const int64_t items = (int64_t)nblk * tiles, per = (items + units * groups - 1) / (units * groups);
+    // a route's items in stretches, so that a block's activations are brought in once; else turn by turn
+    const int64_t first = ROUTED ? (unit * groups + slot_idx) * per : unit * groups + slot_idx, step = ROUTED ? 1 : units * groups;
+    const int mine = first >= items ? 0 : ROUTED ? (int)min(per, items - first) : (int)((items - first + step - 1) / step);
+    const int total = klen > 0 ? mine : 0;
+    const uint32_t q_bytes = (uint32_t)klen * 8u, s_bytes = (uint32_t)(klen / group) * 32u;
+
+    // row of the weights' layout: tile of an expert
+    auto base_of = [&](int64_t it) -> int64_t {
+        if (!ROUTED) return it;
+        const int blk = (int)(it / tiles);
+        return (int64_t)__ldcg(rt.block_expert + blk) * tiles + (it - (int64_t)blk * tiles);
+    };
+    auto issue = [&](int f) {
+        if (lane == 0) {
+            const uint32_t bar = my_bar + (uint32_t)(f % V4_SLOTS) * 8, at = ring + (uint32_t)(f % V4_SLOTS) * V4_SLOT;
+            const int64_t base = base_of(first + f * step);
+            pg_mbar_expect(bar, q_bytes + s_bytes);
+            pg_bulk_load(at, wq + (base * (K / 64) + k0 / 64) * 32, q_bytes, bar);
+            pg_bulk_load(at + V4_Q, ws + (base * (K / group) + k0 / group) * 16, s_bytes, bar);
+        }
+    };
+    for (int f = 0; f < V4_SLOTS; f++)
+        if (f < total) issue(f);
+    if (!ROUTED) asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // activations of the warp's part of K: word 4 c + i of column r (and r + 8): the pairs of columns 32 c + 8 t + 2 i
+    uint32_t x[NT][V4_KW_MAX / 8];
+    float back[NT][2];                                    // what the sums of columns 2 t and 2 t + 1 are multiplied by
+    int have = -1;
+    auto bring = [&](int blk) {
+        have = blk;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            int64_t at = r + 8 * j;
+            bool in = at < M;
+            if (ROUTED) {
+                const int p = __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + r + 8 * j);
+                in = p >= 0;
+                at = rt.by_token ? p / rt.top : blk * PG_ROUTE_SMALL + r + 8 * j;
+            }
+            const bf16 *src = a + at * lda + k0 + t * 8;
+            uint4 v[V4_KW_MAX / 32];
+            float top = 0.0f;
+#pragma unroll
+            for (int c = 0; c < V4_KW_MAX / 32; c++) v[c] = in && c * 32 < klen ? __ldcg(reinterpret_cast<const uint4 *>(src + c * 32)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int c = 0; c < V4_KW_MAX / 32; c++) {
+                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = fmaxf(top, fmaxf(fabsf(pg_bf16_lo(w[i])), fabsf(pg_bf16_hi(w[i]))));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            float down, up;
+            four_range(top, down, up);
+#pragma unroll
+            for (int c = 0; c < V4_KW_MAX / 32; c++) {
+                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[j][4 * c + i] = four_pack_f16(pg_bf16_lo(w[i]) * down, pg_bf16_hi(w[i]) * down);
+            }
+            back[j][0] = __shfl_sync(0xffffffffu, up, 8 * t);          // (lane 4 c has column c)
+            back[j][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+        }
+    };
+
+    // outputs of a tile; lane: weight rows r and r + 8, rows 2 t and 2 t + 1 of the activations
+    auto finish = [&](const float (&acc)[NT][4], int blk, int tile) {
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int m = (ROUTED ? blk * PG_ROUTE_SMALL : 0) + 8 * j + 2 * t + i;
+                if (ROUTED ? (__ldcg(rt.row_pair + m) < 0) : (m >= M)) continue;
+                const float v0 = acc[j][i], v1 = acc[j][2 + i];
+                if (ACT != PG_ACT_NONE) {
+                    pg_put(y + m * ldy + tile * 8 + r, pg_glu<ACT>(v0, v1, limit));
+                } else {
+                    const int n = tile * 16 + r;
+                    if (n < N) pg_put(y + m * ldy + n, v0);
+                    if (n + 8 < N) pg_put(y + m * ldy + n + 8, v1);
+                }
+            }
+    };
+
+    bool ok = true, second = NT == 2;
+    if (!ROUTED && mine > 0 && klen > 0) bring(0);
+    for (int j = 0; j < mine; j++) {
+        float acc[NT][4] = {};
+        const int64_t it = first + j * step;
+        const int blk = ROUTED ? (int)(it / tiles) : 0, tile = (int)(it - (int64_t)blk * tiles);
+        const int turn = (j + slot_idx) % kw;             // the warp that adds the parts up
+        if (klen > 0) {
+            const float *fac = wrow + base_of(it) * 16 + r;
+            const float f0 = __ldg(fac), f1 = __ldg(fac + 8) * 0.0625f;   // (sums of rows r + 8 are 16 times too large)
+            if (ROUTED && blk != have) {
+                bring(blk);
+                second = NT == 2 && __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + 8) >= 0;   // (a block's rows are filled from the first on)
+            }
+            ok = ok && pg_mbar_wait(my_bar + (uint32_t)(j % V4_SLOTS) * 8, (uint32_t)(j / V4_SLOTS) & 1u, abort_flag, status, limit_ns);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) {
+                const uint32_t at = ring + (uint32_t)(j % V4_SLOTS) * V4_SLOT + (uint32_t)lane * 16, sc = ring + (uint32_t)(j % V4_SLOTS) * V4_SLOT + V4_Q + (uint32_t)r * 2;
+                float sum[NT][4] = {};
+                uint32_t s_at = sc;
+#pragma unroll
+                for (int b = 0; b < V4_KW_MAX / 64; b++) {
+                    if (b * 64 >= klen) break;
+                    const uint4 q4 = pg_lds128(at + b * 512);
+                    const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int u = 2 * h; u < 2 * h + 2; u++) {
+                            const uint32_t w = q[u], w8 = w >> 8;
+                            const uint32_t a0 = four_f16_lo(w), a1 = four_f16_hi(w), a2 = four_f16_lo(w8), a3 = four_f16_hi(w8);
+                            four_mma_f16(sum[0], a0, a1, a2, a3, x[0][8 * b + 2 * u], x[0][8 * b + 2 * u + 1]);
+                            if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][8 * b + 2 * u], x[NT - 1][8 * b + 2 * u + 1]);
+                        }
+                        // (uniform: the group ends behind this half of the block)
+                        if ((2 * b + h + 1) * 32 % group == 0) {
+                            unsigned short u0, u1;
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u0) : "r"(s_at));
+                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u1) : "r"(s_at + 16));
+                            s_at += 32;
+                            const float s0 = __half2float(__ushort_as_half(u0)), s1 = __half2float(__ushort_as_half(u1));
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                acc[n][0] = fmaf(s0, sum[n][0], acc[n][0]), acc[n][1] = fmaf(s0, sum[n][1], acc[n][1]);
+                                acc[n][2] = fmaf(s1, sum[n][2], acc[n][2]), acc[n][3] = fmaf(s1, sum[n][3], acc[n][3]);
+                                sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.0f;
+                            }
+                        }
+                    }
+                }
+                __syncwarp();                             // every lane has read the slot
+                if (j + V4_SLOTS < total) issue(j + V4_SLOTS);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {            // (the row's factor first: what is multiplied is never far beyond the result)
+                    acc[n][0] = acc[n][0] * f0 * back[n][0], acc[n][1] = acc[n][1] * f0 * back[n][1];
+                    acc[n][2] = acc[n][2] * f1 * back[n][0], acc[n][3] = acc[n][3] * f1 * back[n][1];
+                }
+            }
+        }
+        if (kw > 1) {
+            float *cells = part + ((size_t)((j & 1) * V4_WARPS + slot_idx * kw) * 32 + lane) * CELL;
+            if (kpart != turn) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) reinterpret_cast<float4 *>(cells + (size_t)kpart * 32 * CELL)[n] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + slot_idx), "r"(kw * 32) : "memory");
+            if (kpart == turn) {
+                float all[NT][4] = {};
+#pragma unroll 4
+                for (int p = 0; p < kw; p++) {            // in the order of K, its own where its turn is
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float4 v = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+                        if (p != turn) v = reinterpret_cast<const float4 *>(cells + (size_t)p * 32 * CELL)[n];
+                        all[n][0] += v.x, all[n][1] += v.y, all[n][2] += v.z, all[n][3] += v.w;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[n][i] = all[n][i];
+            }
+        }
+        if (kpart == turn) {
+            if (SPLIT) {
+                float4 *dst = reinterpret_cast<float4 *>(slabs + (((int64_t)my_part * items + it) * 32 + lane) * CELL);
+#pragma unroll
+                for (int n = 0; n < NT; n++) dst[n] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+            } else if (ok) {
+                finish(acc, blk, tile);
+            }
+        }
+    }
+    if (SPLIT) {
+        __shared__ int last_in;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            __threadfence();
+            last_in = atomicAdd(tickets + unit, 1u) == (unsigned)(sp - 1);
+            if (last_in) tickets[unit] = 0;
+        }
+        __syncthreads();
+        if (last_in) {
+            __threadfence();
+            // the unit's items, a warp each
+            const int64_t count = ROUTED ? max((int64_t)0, min(groups * per, items - unit * groups * per)) : 0;
+            for (int64_t i = warp;; i += V4_WARPS) {
+                int64_t it;
+                if (ROUTED) {
+                    if (i >= count) break;
+                    it = unit * groups * per + i;
+                } else {
+                    it = unit * groups + i % groups + i / groups * (units * groups);
+                    if (unit * groups + i / groups * (units * groups) >= items) break;
+                    if (it >= items) continue;
+                }
+                const int blk = ROUTED ? (int)(it / tiles) : 0;
+                float acc[NT][4] = {};
+#pragma unroll 4
+                for (int p = 0; p < sp; p++) {
+                    const float4 *src = reinterpret_cast<const float4 *>(slabs + (((int64_t)p * items + it) * 32 + lane) * CELL);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float4 v = __ldcg(src + n);
+                        acc[n][0] += v.x, acc[n][1] += v.y, acc[n][2] += v.z, acc[n][3] += v.w;
+                    }
+                }
+                finish(acc, blk, (int)(it - (int64_t)blk * tiles));
+            }
+        }
+    }
+    if (!ok) {
+        // copies that are still in flight get a bounded time to land before the shared memory goes
+        const unsigned long long t0 = pg_globaltimer_ns();
+        while (pg_globaltimer_ns() - t0 < 2000000ull) {
+        }
+    }
+}
+
+// parts of K that CTAs share, and how long a CTA's and a warp's part is
+struct Parts {
+    int sp, KH, kw, KW;
+};
+Parts parts_of(const pg_linear4 *lin, int64_t items, int sms)
+{
+    const int K = (int)lin->k, unit = (int)std::max<int64_t>(64, lin->group);
+    Parts p;
+    p.sp = (K + V4_WARPS * V4_KW_MAX - 1) / (V4_WARPS * V4_KW_MAX);
+    p.KH = p.sp > 1 ? (int)pg_up((K + p.sp - 1) / p.sp, unit) : K;
+    const int64_t units = std::max(1, sms / p.sp);
+    // as few parts as registers allow, more while every (tile, part) still finds a warp of its own
+    p.kw = 1;
+    while (p.kw < V4_WARPS && pg_up((p.KH + p.kw - 1) / p.kw, unit) > V4_KW_MAX) p.kw *= 2;
+    while (p.kw < V4_WARPS && p.KH / (p.kw * 2) >= unit && items * (p.kw * 2) <= units * V4_WARPS) p.kw *= 2;
+    p.KW = (int)pg_up((p.KH + p.kw - 1) / p.kw, unit);
+    return p;
+}
+
+template <int ACT, int NT, bool ROUTED, bool SPLIT, typename TY>
+int32_t launch(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int M, const Parts &p, int grid, float limit, TY *y, int64_t ldy, const PgRouted &rt)
+{
+    auto kern = linear4_gemv_kernel<ACT, NT, ROUTED, SPLIT, TY>;
+    constexpr int smem = V4_RING + 2 * V4_WARPS * 32 * 4 * NT * 4 + V4_WARPS * V4_SLOTS * 8 + 16;
+    static_assert(smem <= 226 * 1024, "shared memory of the streaming form");
+    static std::atomic<uint64_t> set{0};
+    PG_CUDA(pg_max_smem_once(kern, smem, ctx->device, set));
+    unsigned int *tickets = reinterpret_cast<unsigned int *>(ctx->splitk);
+    float *slabs = SPLIT ? reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES) : nullptr;
+    return launch_pdl(ctx, kern, dim3((unsigned)grid), dim3(V4_THREADS), (size_t)smem, a, lda, M, lin->q, lin->s, lin->row, (int)lin->n, (int)lin->k, (int)lin->group,
+                      (int)lin->tiles, p.kw, p.KW, p.KH, limit, y, ldy, rt, p.sp, slabs, tickets, ctx->d_status, ctx->wait_limit_ns);
+}
+
+// slabs of a call
+size_t slab_bytes(int sp, int64_t items, int nt) { return sp > 1 ? PG_LM_TICKET_BYTES + (size_t)sp * (size_t)items * 32 * 4 * nt * sizeof(float) : 0; }
+
+}  // namespace
+
+size_t pgk_linear4_gemv_workspace(const pg_linear4 *lin)
+{
+    const int sp = (int)((lin->k + V4_WARPS * V4_KW_MAX - 1) / (V4_WARPS * V4_KW_MAX));
+    // (a route's blocks: as many as a route of 16 tokens can have would be 16 times the experts' rows; the experts' own number is the most)
+    return slab_bytes(sp, lin->tiles * lin->experts, 2);
+}
+
+int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int64_t m, int act, float limit, void *y, int y_dtype, int64_t ldy,
+                         const PgRouted *routed, int64_t max_blocks)
+{
+    const int64_t items = lin->tiles * (routed ? max_blocks : 1);
+    const Parts p = parts_of(lin, items, ctx->sm_count);
+    const int nt = m > 8 || routed ? 2 : 1;
+    PG_REQUIRE(p.KW <= V4_KW_MAX && p.sp <= 16, "linear4: K too long");
+    if (p.sp > 1) {
+        const int32_t rc = pg_splitk_reserve(ctx, slab_bytes(p.sp, items, nt));
+        if (rc != PG_OK) return rc;
+    }
+    const int groups = V4_WARPS / p.kw;
+    const int grid = (int)std::min<int64_t>(ctx->sm_count / p.sp, (items + groups - 1) / groups) * p.sp;
+    static const PgRouted no_route = {};
+    const PgRouted &rt = routed ? *routed : no_route;
+#define PG_V4(ACT, NT, RT, TY)                                                                                                                   \
+    do {                                                                                                                                         \
+        if (p.sp > 1) return launch<ACT, NT, RT, true, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                          \
+        return launch<ACT, NT, RT, false, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                                       \
+    } while (0)
+#define PG_V4_ACT(ACT, TY)                  \
+    do {                                    \
+        if (routed) PG_V4(ACT, 2, true, TY); \
+        if (nt == 2) PG_V4(ACT, 2, false, TY); \
+        PG_V4(ACT, 1, false, TY);           \
+    } while (0)
+    if (act == PG_ACT_GELU_TANH_GLU) PG_V4_ACT(PG_ACT_GELU_TANH_GLU, bf16);
+    if (act == PG_ACT_CLAMPED_SWISH_GLU) PG_V4_ACT(PG_ACT_CLAMPED_SWISH_GLU, bf16);
+    if (y_dtype == PG_BF16) PG_V4_ACT(PG_ACT_NONE, bf16);
+    PG_V4_ACT(PG_ACT_NONE, float);
+#undef PG_V4
+#undef PG_V4_ACT
+}

@@ -88,27 +88,30 @@ def expect(what: str, W, shapes: dict) -> None:
             raise ValueError(f"{what}: {name} is {list(W[name].shape)}, the configuration says {list(shape)}")
 
 
+def stacked(d: Device, w, gated: bool, multiple: int = 64):
+    """bf16 [experts, N, K] of a matrix, of one per expert, or of a pair (gate, up), K padded with zero columns to `multiple`; and the columns of
+    the product's output.  Gated: rows alternate eight gates, eight ups; F is padded to 8 with zero rows."""
+    t = d.torch
+    if gated:
+        gate, upw = (x if x.dim() == 3 else x[None] for x in w)
+        E, F, K = gate.shape
+        both = t.zeros(E, up(F, 8), 2, up(K, multiple), dtype=t.bfloat16, device=d.dev)
+        both[:, :F, 0, :K], both[:, :F, 1, :K] = gate, upw
+        return both.view(E, -1, 8, 2, both.shape[-1]).transpose(2, 3).reshape(E, 2 * up(F, 8), -1).contiguous(), up(F, 8)
+    w = w if w.dim() == 3 else w[None]
+    K = w.shape[2]
+    if K % multiple:
+        w = t.nn.functional.pad(w, (0, up(K, multiple) - K))
+    return w.contiguous(), w.shape[1]
+
+
 class Linear:
     """w: bf16 [N, K] or [experts, N, K] on the device; K is padded to 64 with zero columns.  `gated`: w is the pair
     (gate, up), whose rows are laid out in alternating blocks of eight; F is then padded to 8 with zero rows."""
 
     def __init__(self, d: Device, w, gated: bool = False):
-        t = d.torch
         self.d = d
-        if gated:
-            gate, upw = (x if x.dim() == 3 else x[None] for x in w)
-            E, F, K = gate.shape
-            both = t.zeros(E, up(F, 8), 2, up(K, 64), dtype=t.bfloat16, device=d.dev)
-            both[:, :F, 0, :K], both[:, :F, 1, :K] = gate, upw
-            w = both.view(E, -1, 8, 2, both.shape[-1]).transpose(2, 3).reshape(E, 2 * up(F, 8), -1).contiguous()
-            self.cols = up(F, 8)
-        else:
-            w = w if w.dim() == 3 else w[None]
-            E, N, K = w.shape
-            if K % 64:
-                w = t.nn.functional.pad(w, (0, up(K, 64) - K))
-            w = w.contiguous()
-            self.cols = N
+        w, self.cols = stacked(d, w, gated)
         self.w = w
         self.experts, self.n, self.k = w.shape
         h = C.c_void_p()
@@ -138,6 +141,72 @@ class Linear:
 
     def bytes(self) -> int:
         return self.w.numel() * 2
+
+
+class Linear4:
+    """The same with the weights held in 4 bits and a scale per `group` elements of K (csrc/pg_linear4.cu), for bf16 activations.  The matrix is
+    rounded when it is laid out; `from_quants` takes quants and scales that are there already, rows in the order of the product."""
+
+    GROUP = 64
+
+    def __init__(self, d: Device, w, gated: bool = False, group: int = GROUP):
+        w, cols = stacked(d, w, gated)
+        if w.shape[2] % group:
+            raise ValueError(f"weights in 4 bits: K = {w.shape[2]} is no multiple of the groups of {group}")
+        h = C.c_void_p()
+        d.torch.cuda.current_stream(d.dev).synchronize()     # torch laid the matrix out on a stream of its own
+        d.check(d.lib.pg_linear4_quantize(d.gpu.handle, w.data_ptr(), w.shape[1], w.shape[2], group, w.shape[0], C.byref(h)))
+        self._set(d, h, w.shape, cols, group)
+
+    @classmethod
+    def from_quants(cls, d: Device, q, scales) -> "Linear4":
+        """q: uint8 [N, K / 2] or [experts, N, K / 2], two quants a byte, the first in the low half; scales: bf16 [.., N, K / group]."""
+        t = d.torch
+        q, scales = (x if x.dim() == 3 else x[None] for x in (q, scales))
+        if q.dtype != t.uint8 or scales.dtype != t.bfloat16 or q.device != d.dev or scales.device != d.dev:
+            raise ValueError("weights in 4 bits: quants are uint8 and scales bfloat16, on the device")
+        E, N, K = q.shape[0], q.shape[1], 2 * q.shape[2]
+        if scales.shape[:2] != q.shape[:2] or not scales.shape[2] or K % scales.shape[2]:
+            raise ValueError(f"weights in 4 bits: scales {list(scales.shape)} for quants {list(q.shape)}")
+        q, scales = q.contiguous(), scales.contiguous()
+        t.cuda.current_stream(d.dev).synchronize()
+        h = C.c_void_p()
+        d.check(d.lib.pg_linear4_pack(d.gpu.handle, q.data_ptr(), scales.data_ptr(), N, K, K // scales.shape[2], E, C.byref(h)))
+        self = cls.__new__(cls)
+        self._set(d, h, (E, N, K), N, K // scales.shape[2])
+        return self
+
+    def _set(self, d: Device, handle, shape, cols: int, group: int) -> None:
+        self.d, self.handle, self.cols, self.group = d, handle, cols, group
+        self.experts, self.n, self.k = (int(x) for x in shape)
+        self._bytes = int(d.lib.pg_linear4_bytes(handle))
+
+    def run(self, a, rows: int, y, act: int = _lib.ACT_NONE, limit: float = 0.0) -> None:
+        d = self.d
+        d.check(d.lib.pg_linear4_run(d.gpu.handle, self.handle, a.data_ptr(), a.stride(0) if rows > 1 else self.k, d.code, rows, act, limit, y.data_ptr(),
+                                     _lib.F32 if y.dtype == d.torch.float32 else _lib.BF16, y.stride(0)))
+
+    def run_routed(self, route, a, by_token: bool, y, act: int = _lib.ACT_NONE, limit: float = 0.0) -> None:
+        """Rows of a are K elements apart."""
+        d = self.d
+        d.check(d.lib.pg_linear4_run_routed(d.gpu.handle, self.handle, route, a.data_ptr(), d.code, int(by_token), act, limit, y.data_ptr(),
+                                            _lib.F32 if y.dtype == d.torch.float32 else _lib.BF16, y.stride(0)))
+
+    def values(self):
+        """The weights as the product takes them: f32 [experts, N, K]."""
+        t = self.d.torch
+        out = t.empty(self.experts, self.n, self.k, dtype=t.float32, device=self.d.dev)
+        self.d.check(self.d.lib.pg_linear4_read(self.d.gpu.handle, self.handle, out.data_ptr()))
+        self.d.gpu.sync()
+        return out
+
+    def free(self) -> None:
+        if self.handle is not None:
+            self.d.lib.pg_linear4_free(self.d.gpu.handle, self.handle)
+            self.handle = None
+
+    def bytes(self) -> int:
+        return self._bytes
 
 
 def stack_rows(d: Device, parts, multiple: int = 4):
