@@ -11,10 +11,9 @@
 
 struct pg_linear4 {
     void *mem = nullptr;
-    const uint4 *q = nullptr;     // [experts][tiles][K / 64][32 lanes] 16 bytes: 16 rows x 64 k as mma.sync and the unpacking threads read them
-    const __half *s = nullptr;    // [experts][tiles][K / group][16]: scale / 2^row
-    const float *row = nullptr;   // [experts][tiles * 16]: 2^row
-    int64_t n = 0, k = 0, experts = 1, group = 0, tiles = 0, bytes = 0;
+    const unsigned char *w = nullptr;   // [experts][tiles][K / 64][record]: 16 rows x 64 k, quants and scales (csrc/pg_linear4.cu)
+    const float *row = nullptr;         // [experts][tiles * 16]: 2^row
+    int64_t n = 0, k = 0, experts = 1, group = 0, tiles = 0, record = 0, bytes = 0;
     int device = 0;
 };
 

@@ -1,13 +1,16 @@
 // Products with weights of 4 bits and a scale per group of K (include/peregrine_b200_lm.h): the handle, the layout of the weights, and
 // the choice of kernel.
 //
-// W[n][k] = s[n][k / group] (q[n][k] - 8).  16 rows x 64 k are 512 bytes: a lane (r = lane / 4, t = lane % 4) of a warp has 16, four words.  Word
-// 2 c + h holds rows r and r + 8, columns 32 c + 8 t + 4 h + {0, 1, 2, 3}: bits 0-3 row r, columns 0 (low half) and 1 (high half); bits 4-7
-// row r + 8, the same; bits 8-11 and 12-15 the two rows' columns 2 and 3.  That is an A operand of mma.sync m16n8k16 once the quants are f16
-// numbers, and a row's four lanes are 64 bytes next to each other.
+// W[n][k] = s[n][k / group] (q[n][k] - 8).  A record is 16 rows x 64 k: 512 bytes of quants, then one or (groups of 32) two times 16 scales.
+//
+// Quants: lane (r = lane / 4, t = lane % 4) of a warp has 16 bytes, at 16 (4 r + (t ^ (r / 2 & 3))): in this order neither a warp that reads all of
+// them nor threads that each read the 64 bytes of a row meet a bank twice.  Of its four words, word 2 c + h holds rows r and r + 8, columns
+// 32 c + 8 t + 4 h + {0, 1, 2, 3}: bits 0-3 row r, columns 0 (low half) and 1 (high half); bits 4-7 row r + 8, the same; bits 8-11 and 12-15 the two
+// rows' columns 2 and 3.  That is an A operand of mma.sync m16n8k16 once the quants are f16 numbers.  Scales: rows r and r + 8 side by side; where a
+// group is 128 long its two records both have them, so that a record is all that a block of 64 k needs.
 //
 // Scales are kept as f16 divided by a power of two per row, which brings the row's largest to [2^11, 2^12): scale * (q - 8) is then at most 8 + 3
-// significant bits, so an f16 number, exactly, as long as the row's scales are within 2^25 of each other (below, the smaller ones lose bits
+// significant bits, so an f16 number, exactly, as long as the row's scales are within 2^21 of each other (below, the smaller ones lose bits
 // that are under 2^-36 of the largest).
 #include <algorithm>
 #include <new>
@@ -20,7 +23,7 @@ namespace {
 // else from bf16 weights [n][k].
 template <bool QUANTS>
 __global__ void __launch_bounds__(128)
-    linear4_pack_kernel(const void *__restrict__ src, const bf16 *__restrict__ scales, int n, int k, int group, uint4 *__restrict__ q, __half *__restrict__ s,
+    linear4_pack_kernel(const void *__restrict__ src, const bf16 *__restrict__ scales, int n, int k, int group, int record, unsigned char *__restrict__ out,
                         float *__restrict__ row)
 {
     extern __shared__ float sm[];                      // scales [k / group][16] | largest of each row [16]
@@ -62,9 +65,12 @@ __global__ void __launch_bounds__(128)
     __syncthreads();
     if (threadIdx.x < 16) top[threadIdx.x] = down;
     __syncthreads();
-    __half *so = s + (e * tiles + tile) * (int64_t)groups * 16;
-    for (int i = threadIdx.x; i < 16 * groups; i += 128) so[i] = __float2half_rn(sm[i] * top[i & 15]);
-    uint4 *qo = q + (e * tiles + tile) * (int64_t)(k / 64) * 32;
+    unsigned char *dst = out + (e * tiles + tile) * (int64_t)(k / 64) * record;
+    const int per = (record - 512) / 32;               // scales of a row in a record
+    for (int i = threadIdx.x; i < k / 64 * per * 16; i += 128) {
+        const int b = i / (per * 16), c = i / 16 % per, x = i % 16, r = (x >> 1) + 8 * (x & 1);
+        reinterpret_cast<__half *>(dst + (int64_t)b * record + 512)[c * 16 + x] = __float2half_rn(sm[(b * 64 + c * 32) / group * 16 + r] * top[r]);
+    }
     for (int i = threadIdx.x; i < k / 64 * 32; i += 128) {
         const int b = i >> 5, lane = i & 31, r = lane >> 2, t = lane & 3;
         uint32_t w[4];
@@ -86,24 +92,25 @@ __global__ void __launch_bounds__(128)
                 w[j] |= v << ((c & 1) * 16 + (c >> 1) * 8 + (x & 1) * 4);
             }
         }
-        qo[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(dst + (int64_t)b * record + 16 * (4 * r + (t ^ (r >> 1 & 3)))) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
 // values as f32 [experts][n][k]
-__global__ void __launch_bounds__(256) linear4_read_kernel(const uint4 *__restrict__ q, const __half *__restrict__ s, const float *__restrict__ row, int n, int k, int group,
-                                                           int tiles, int64_t total, float *__restrict__ out)
+__global__ void __launch_bounds__(256) linear4_read_kernel(const unsigned char *__restrict__ w, const float *__restrict__ row, int n, int k, int record, int tiles,
+                                                           int64_t total, float *__restrict__ out)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
     const int col = (int)(i % k);
     const int64_t at = i / k, e = at / n;
-    const int rr = (int)(at - e * n), tile = rr / 16, r = rr % 16;
+    const int rr = (int)(at - e * n), tile = rr / 16, x = rr % 16, r = x % 8, hi = x / 8;
     const int64_t base = e * tiles + tile;
-    const int b = col / 64, c = col % 64, t = c % 32 / 8, j = 2 * (c / 32) + c % 8 / 4, x = c % 4;
-    const uint32_t w = reinterpret_cast<const uint32_t *>(q + (base * (k / 64) + b) * 32 + (r % 8) * 4 + t)[j];
-    const uint32_t v = w >> ((x & 1) * 16 + (x >> 1) * 8 + (r / 8) * 4) & 15u;
-    out[i] = __half2float(s[(base * (k / group) + col / group) * 16 + r]) * row[base * 16 + r] * (float)((int)v - 8);
+    const int b = col / 64, c = col % 64, t = c % 32 / 8, j = 2 * (c / 32) + c % 8 / 4, y = c % 4;
+    const unsigned char *rec = w + (base * (k / 64) + b) * record;
+    const uint32_t v = *reinterpret_cast<const uint32_t *>(rec + 16 * (4 * r + (t ^ (r >> 1 & 3))) + 4 * j) >> ((y & 1) * 16 + (y >> 1) * 8 + hi * 4) & 15u;
+    const __half s = reinterpret_cast<const __half *>(rec + 512)[(record > 544 ? c / 32 * 16 : 0) + 2 * r + hi];
+    out[i] = __half2float(s) * row[base * 16 + x] * (float)((int)v - 8);
 }
 
 int32_t create(pg_ctx *ctx, const void *src, const void *scales, int64_t n, int64_t k, int64_t group, int64_t experts, pg_linear4 **out)
@@ -118,11 +125,12 @@ int32_t create(pg_ctx *ctx, const void *src, const void *scales, int64_t n, int6
     pg_linear4 *l = new (std::nothrow) pg_linear4();
     if (!l) PG_FAIL(PG_ERR_NOMEM, "out of host memory");
     l->n = n, l->k = k, l->group = group, l->experts = experts, l->tiles = (n + 15) / 16, l->device = ctx->device;
-    const size_t qb = (size_t)experts * l->tiles * (k / 64) * 512, sb = (size_t)experts * l->tiles * (k / group) * 32, rb = (size_t)experts * l->tiles * 64;
-    l->bytes = (int64_t)(qb + sb + rb);
+    l->record = group == 32 ? 576 : 544;
+    const size_t wb = (size_t)experts * l->tiles * (k / 64) * l->record, rb = (size_t)experts * l->tiles * 64;
+    l->bytes = (int64_t)(wb + rb);
     int32_t rc = pg_splitk_reserve(ctx, std::max(pgk_linear4_gemv_workspace(l), pgk_linear4_tc_workspace(ctx)));
     if (rc == PG_OK) {
-        const cudaError_t e = cudaMalloc(&l->mem, qb + (size_t)pg_up(sb, 128) + rb);
+        const cudaError_t e = cudaMalloc(&l->mem, (size_t)pg_up(wb, 128) + rb);
         if (e != cudaSuccess) {
             cudaGetLastError();
             pg_set_error("linear4: %s", cudaGetErrorString(e));
@@ -134,14 +142,14 @@ int32_t create(pg_ctx *ctx, const void *src, const void *scales, int64_t n, int6
         return rc;
     }
     unsigned char *p = (unsigned char *)l->mem;
-    l->q = (const uint4 *)p;
-    l->s = (const __half *)(p + qb);
-    l->row = (const float *)(p + qb + pg_up(sb, 128));
+    l->w = p;
+    l->row = (const float *)(p + pg_up(wb, 128));
     const size_t smem = (size_t)(k / group * 16 + 16) * sizeof(float);
     const dim3 grid((unsigned)l->tiles, (unsigned)experts);
     auto go = [&](auto kern, std::atomic<uint64_t> &set) -> int32_t {
         PG_CUDA(pg_max_smem_once(kern, 160 * 1024, ctx->device, set));
-        return launch_whole(ctx, kern, grid, dim3(128), smem, src, (const bf16 *)scales, (int)n, (int)k, (int)group, (uint4 *)l->q, (__half *)l->s, (float *)l->row);
+        return launch_whole(ctx, kern, grid, dim3(128), smem, src, (const bf16 *)scales, (int)n, (int)k, (int)group, (int)l->record,
+                            (unsigned char *)l->w, (float *)l->row);
     };
     static std::atomic<uint64_t> set_q{0}, set_w{0};
     rc = scales ? go(linear4_pack_kernel<true>, set_q) : go(linear4_pack_kernel<false>, set_w);
@@ -206,7 +214,7 @@ PG_API int32_t pg_linear4_read(pg_ctx *ctx, const pg_linear4 *lin, float *d_w)
     PG_REQUIRE(lin && d_w && lin->device == ctx->device, "linear4_read: bad arguments");
     const int64_t total = lin->experts * lin->n * lin->k;
     PG_REQUIRE(total < (1ll << 31) * 256, "linear4_read: too many weights for one call");
-    return launch_whole(ctx, linear4_read_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, lin->q, lin->s, lin->row, (int)lin->n, (int)lin->k, (int)lin->group,
+    return launch_whole(ctx, linear4_read_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, lin->w, lin->row, (int)lin->n, (int)lin->k, (int)lin->record,
                         (int)lin->tiles, total, d_w);
 }
 

@@ -4,10 +4,10 @@
 //     tiles on the same unpacked quants.  Quants become f16 integers (exact), sums of a group are scaled in f32.
 //   * The activations are bf16 and enter as f16: a warp divides each row of its part of K by a power of two of its own (four_range) and
 //     multiplies the sums back, so nothing is rounded that could be seen in an f32 sum.
-//   * One persistent CTA of 16 warps per SM.  `kw` warps share a tile of 16 weight rows, each with one part of K of at most 256 elements, whose
-//     activations it keeps in registers; a fill of its ring is two bulk copies, quants (up to 2 KB) and scales.  The parts meet in shared memory
+//   * One persistent CTA of 16 warps per SM.  `kw` warps share a tile of 16 weight rows, each with one part of K of at most 512 elements (256 with more than
+//     eight rows), whose activations it keeps in registers; a fill of its ring is one bulk copy, quants and scales.  The parts meet in shared memory
 //     in a fixed order; the warps of a tile take turns in adding.
-//   * K beyond 16 x 256 (SPLIT): sp CTAs take the same tiles, their sums go to slabs, the last one in (a ticket) adds in a fixed order.
+//   * K beyond 16 such parts (SPLIT): sp CTAs take the same tiles, their sums go to slabs, the last one in (a ticket) adds in a fixed order.
 //   * ROUTED: rows come in blocks of 16 that share an expert.
 //
 // Every mbarrier wait is bounded; a warp that gave up goes on through the remaining barriers without computing.
@@ -19,32 +19,32 @@
 namespace {
 
 constexpr int V4_WARPS = 16, V4_THREADS = V4_WARPS * 32;
-constexpr int V4_SLOTS = 5;
-constexpr int V4_KW_MAX = 256;
-constexpr int V4_Q = V4_KW_MAX / 64 * 512, V4_SLOT = V4_Q + V4_KW_MAX / 32 * 32;   // quants, then scales of groups of 32 at worst
-constexpr int V4_RING = V4_WARPS * V4_SLOTS * V4_SLOT;
+constexpr int V4_SLOTS_MAX = 8;
+__host__ __device__ constexpr int v4_ring(int nt) { return nt == 1 ? 3 * 4352 : 5 * 2304; }   // bytes of a warp's ring
+__host__ __device__ constexpr int v4_kw_max(int nt) { return nt == 1 ? 512 : 256; }   // (what the registers hold of the activations)
 
 // shared memory: ring | partial sums [2][16 warps][32 lanes][4 NT] | barriers
 // slabs (SPLIT): [sp][items][32 lanes][4 NT]
 template <int ACT, int NT, bool ROUTED, bool SPLIT, typename TY>
 __global__ void __launch_bounds__(V4_THREADS, 1)
-    linear4_gemv_kernel(const bf16 *__restrict__ a, int64_t lda, int M, const uint4 *__restrict__ wq, const __half *__restrict__ ws, const float *__restrict__ wrow, int N,
-                        int K, int group, int tiles, int kw, int KW, int KH, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, int sp, float *slabs,
+    linear4_gemv_kernel(const bf16 *__restrict__ a, int64_t lda, int M, const unsigned char *__restrict__ w, const float *__restrict__ wrow, int N, int K, int group,
+                        int record, int tiles, int kw, int KW, int KH, int slots, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, int sp, float *slabs,
                         unsigned int *tickets, int32_t *status, unsigned long long limit_ns)
 {
     constexpr int CELL = 4 * NT;                          // floats per lane
+    constexpr int KWM = v4_kw_max(NT);
     extern __shared__ __align__(128) unsigned char smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
     const int my_part = SPLIT ? (int)blockIdx.x % sp : 0;
     const int groups = V4_WARPS / kw, slot_idx = warp / kw, kpart = warp - slot_idx * kw;
-    float *part = reinterpret_cast<float *>(smem + V4_RING);
+    float *part = reinterpret_cast<float *>(smem + V4_WARPS * v4_ring(NT));
     unsigned char *tail = reinterpret_cast<unsigned char *>(part + 2 * V4_WARPS * 32 * CELL);
-    const uint32_t my_bar = pg_smem(tail) + (uint32_t)warp * (V4_SLOTS * 8);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + V4_WARPS * V4_SLOTS * 8);
-    const uint32_t ring = pg_smem(smem) + (uint32_t)warp * (V4_SLOTS * V4_SLOT);
+    const uint32_t my_bar = pg_smem(tail) + (uint32_t)warp * (V4_SLOTS_MAX * 8);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + V4_WARPS * V4_SLOTS_MAX * 8);
+    const uint32_t ring = pg_smem(smem) + (uint32_t)(warp * v4_ring(NT));
     if (threadIdx.x == 0) {
-        for (int i = 0; i < V4_WARPS * V4_SLOTS; i++) pg_mbar_init(pg_smem(tail) + 8 * i, 1);
+        for (int i = 0; i < V4_WARPS * V4_SLOTS_MAX; i++) pg_mbar_init(pg_smem(tail) + 8 * i, 1);
         *abort_flag = 0;
         pg_mbar_fence();
     }
@@ -60,7 +60,8 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     const int64_t first = ROUTED ? (unit * groups + slot_idx) * per : unit * groups + slot_idx, step = ROUTED ? 1 : units * groups;
     const int mine = first >= items ? 0 : ROUTED ? (int)min(per, items - first) : (int)((items - first + step - 1) / step);
     const int total = klen > 0 ? mine : 0;
-    const uint32_t q_bytes = (uint32_t)klen * 8u, s_bytes = (uint32_t)(klen / group) * 32u;
+    const uint32_t fill_bytes = (uint32_t)(klen / 64 * record);
+    const int64_t row_bytes = (int64_t)(K / 64) * record;
 
     // row of the weights' layout: tile of an expert
     auto base_of = [&](int64_t it) -> int64_t {
@@ -68,21 +69,26 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
         const int blk = (int)(it / tiles);
         return (int64_t)__ldcg(rt.block_expert + blk) * tiles + (it - (int64_t)blk * tiles);
     };
-    auto issue = [&](int f) {
+    // fills follow one another through the slots; without a route they lie a constant distance apart
+    int fill_slot = 0, filled = 0;
+    const unsigned char *next = w + first * row_bytes + k0 / 64 * record;
+    auto issue = [&]() {
         if (lane == 0) {
-            const uint32_t bar = my_bar + (uint32_t)(f % V4_SLOTS) * 8, at = ring + (uint32_t)(f % V4_SLOTS) * V4_SLOT;
-            const int64_t base = base_of(first + f * step);
-            pg_mbar_expect(bar, q_bytes + s_bytes);
-            pg_bulk_load(at, wq + (base * (K / 64) + k0 / 64) * 32, q_bytes, bar);
-            pg_bulk_load(at + V4_Q, ws + (base * (K / group) + k0 / group) * 16, s_bytes, bar);
+            const uint32_t bar = my_bar + (uint32_t)fill_slot * 8;
+            if (ROUTED) next = w + base_of(first + filled) * row_bytes + k0 / 64 * record;
+            pg_mbar_expect(bar, fill_bytes);
+            pg_bulk_load(ring + (uint32_t)fill_slot * fill_bytes, next, fill_bytes, bar);
         }
+        if (!ROUTED) next += step * row_bytes;
+        filled++;
+        if (++fill_slot == slots) fill_slot = 0;
     };
-    for (int f = 0; f < V4_SLOTS; f++)
-        if (f < total) issue(f);
+    for (int f = 0; f < slots; f++)
+        if (f < total) issue();
     if (!ROUTED) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // activations of the warp's part of K: word 4 c + i of column r (and r + 8): the pairs of columns 32 c + 8 t + 2 i
-    uint32_t x[NT][V4_KW_MAX / 8];
+    uint32_t x[NT][KWM / 8];
     float back[NT][2];                                    // what the sums of columns 2 t and 2 t + 1 are multiplied by
     int have = -1;
     auto bring = [&](int blk) {
@@ -97,12 +103,12 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
                 at = rt.by_token ? p / rt.top : blk * PG_ROUTE_SMALL + r + 8 * j;
             }
             const bf16 *src = a + at * lda + k0 + t * 8;
-            uint4 v[V4_KW_MAX / 32];
+            uint4 v[KWM / 32];
             float top = 0.0f;
 #pragma unroll
-            for (int c = 0; c < V4_KW_MAX / 32; c++) v[c] = in && c * 32 < klen ? __ldcg(reinterpret_cast<const uint4 *>(src + c * 32)) : make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < KWM / 32; c++) v[c] = in && c * 32 < klen ? __ldcg(reinterpret_cast<const uint4 *>(src + c * 32)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-            for (int c = 0; c < V4_KW_MAX / 32; c++) {
+            for (int c = 0; c < KWM / 32; c++) {
                 const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) top = fmaxf(top, fmaxf(fabsf(pg_bf16_lo(w[i])), fabsf(pg_bf16_hi(w[i]))));
@@ -112,7 +118,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
             float down, up;
             four_range(top, down, up);
 #pragma unroll
-            for (int c = 0; c < V4_KW_MAX / 32; c++) {
+            for (int c = 0; c < KWM / 32; c++) {
                 const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[j][4 * c + i] = four_pack_f16(pg_bf16_lo(w[i]) * down, pg_bf16_hi(w[i]) * down);
@@ -142,12 +148,15 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     };
 
     bool ok = true, second = NT == 2;
+    const int gmask = group / 32 - 1;                     // (the group is a power of two)
+    int slot = 0;
+    uint32_t phase = 0;
     if (!ROUTED && mine > 0 && klen > 0) bring(0);
     for (int j = 0; j < mine; j++) {
         float acc[NT][4] = {};
         const int64_t it = first + j * step;
         const int blk = ROUTED ? (int)(it / tiles) : 0, tile = (int)(it - (int64_t)blk * tiles);
-        const int turn = (j + slot_idx) % kw;             // the warp that adds the parts up
+        const int turn = (j + slot_idx) & (kw - 1);            // the warp that adds the parts up
         if (klen > 0) {
             const float *fac = wrow + base_of(it) * 16 + r;
             const float f0 = __ldg(fac), f1 = __ldg(fac + 8) * 0.0625f;   // (sums of rows r + 8 are 16 times too large)
@@ -155,16 +164,14 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
                 bring(blk);
                 second = NT == 2 && __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + 8) >= 0;   // (a block's rows are filled from the first on)
             }
-            ok = ok && pg_mbar_wait(my_bar + (uint32_t)(j % V4_SLOTS) * 8, (uint32_t)(j / V4_SLOTS) & 1u, abort_flag, status, limit_ns);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = ok && pg_mbar_wait_warp(my_bar + (uint32_t)slot * 8, phase, abort_flag, status, limit_ns);
             if (ok) {
-                const uint32_t at = ring + (uint32_t)(j % V4_SLOTS) * V4_SLOT + (uint32_t)lane * 16, sc = ring + (uint32_t)(j % V4_SLOTS) * V4_SLOT + V4_Q + (uint32_t)r * 2;
+                const uint32_t slot_at = ring + (uint32_t)slot * fill_bytes, at = slot_at + 16u * (uint32_t)(4 * r + (t ^ (r >> 1 & 3))), s_at = slot_at + 512u + (uint32_t)r * 4;
                 float sum[NT][4] = {};
-                uint32_t s_at = sc;
 #pragma unroll
-                for (int b = 0; b < V4_KW_MAX / 64; b++) {
+                for (int b = 0; b < KWM / 64; b++) {
                     if (b * 64 >= klen) break;
-                    const uint4 q4 = pg_lds128(at + b * 512);
+                    const uint4 q4 = pg_lds128(at + b * record);
                     const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -176,12 +183,11 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
                             if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][8 * b + 2 * u], x[NT - 1][8 * b + 2 * u + 1]);
                         }
                         // (uniform: the group ends behind this half of the block)
-                        if ((2 * b + h + 1) * 32 % group == 0) {
-                            unsigned short u0, u1;
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u0) : "r"(s_at));
-                            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u1) : "r"(s_at + 16));
-                            s_at += 32;
-                            const float s0 = __half2float(__ushort_as_half(u0)), s1 = __half2float(__ushort_as_half(u1));
+                        if (((2 * b + h + 1) & gmask) == 0) {
+                            uint32_t both;                // the scales of rows r and r + 8
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(s_at + b * record + (record > 544 ? h * 32 : 0)));
+                            const float2 sc = __half22float2(*reinterpret_cast<const __half2 *>(&both));
+                            const float s0 = sc.x, s1 = sc.y;
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
                                 acc[n][0] = fmaf(s0, sum[n][0], acc[n][0]), acc[n][1] = fmaf(s0, sum[n][1], acc[n][1]);
@@ -192,7 +198,8 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
                     }
                 }
                 __syncwarp();                             // every lane has read the slot
-                if (j + V4_SLOTS < total) issue(j + V4_SLOTS);
+                if (j + slots < total) issue();
+                if (++slot == slots) slot = 0, phase ^= 1;
 #pragma unroll
                 for (int n = 0; n < NT; n++) {            // (the row's factor first: what is multiplied is never far beyond the result)
                     acc[n][0] = acc[n][0] * f0 * back[n][0], acc[n][1] = acc[n][1] * f0 * back[n][1];
@@ -285,16 +292,17 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
 struct Parts {
     int sp, KH, kw, KW;
 };
-Parts parts_of(const pg_linear4 *lin, int64_t items, int sms)
+int split_of(int64_t k, int nt) { return (int)((k + V4_WARPS * v4_kw_max(nt) - 1) / (V4_WARPS * v4_kw_max(nt))); }
+Parts parts_of(const pg_linear4 *lin, int64_t items, int sms, int nt)
 {
-    const int K = (int)lin->k, unit = (int)std::max<int64_t>(64, lin->group);
+    const int K = (int)lin->k, unit = (int)std::max<int64_t>(64, lin->group), most = v4_kw_max(nt);
     Parts p;
-    p.sp = (K + V4_WARPS * V4_KW_MAX - 1) / (V4_WARPS * V4_KW_MAX);
+    p.sp = split_of(K, nt);
     p.KH = p.sp > 1 ? (int)pg_up((K + p.sp - 1) / p.sp, unit) : K;
     const int64_t units = std::max(1, sms / p.sp);
     // as few parts as registers allow, more while every (tile, part) still finds a warp of its own
     p.kw = 1;
-    while (p.kw < V4_WARPS && pg_up((p.KH + p.kw - 1) / p.kw, unit) > V4_KW_MAX) p.kw *= 2;
+    while (p.kw < V4_WARPS && pg_up((p.KH + p.kw - 1) / p.kw, unit) > most) p.kw *= 2;
     while (p.kw < V4_WARPS && p.KH / (p.kw * 2) >= unit && items * (p.kw * 2) <= units * V4_WARPS) p.kw *= 2;
     p.KW = (int)pg_up((p.KH + p.kw - 1) / p.kw, unit);
     return p;
@@ -304,14 +312,15 @@ template <int ACT, int NT, bool ROUTED, bool SPLIT, typename TY>
 int32_t launch(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int M, const Parts &p, int grid, float limit, TY *y, int64_t ldy, const PgRouted &rt)
 {
     auto kern = linear4_gemv_kernel<ACT, NT, ROUTED, SPLIT, TY>;
-    constexpr int smem = V4_RING + 2 * V4_WARPS * 32 * 4 * NT * 4 + V4_WARPS * V4_SLOTS * 8 + 16;
+    constexpr int smem = V4_WARPS * v4_ring(NT) + 2 * V4_WARPS * 32 * 4 * NT * 4 + V4_WARPS * V4_SLOTS_MAX * 8 + 16;
     static_assert(smem <= 226 * 1024, "shared memory of the streaming form");
     static std::atomic<uint64_t> set{0};
     PG_CUDA(pg_max_smem_once(kern, smem, ctx->device, set));
+    const int slots = std::min(V4_SLOTS_MAX, v4_ring(NT) / (int)(p.KW / 64 * lin->record));
     unsigned int *tickets = reinterpret_cast<unsigned int *>(ctx->splitk);
     float *slabs = SPLIT ? reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES) : nullptr;
-    return launch_pdl(ctx, kern, dim3((unsigned)grid), dim3(V4_THREADS), (size_t)smem, a, lda, M, lin->q, lin->s, lin->row, (int)lin->n, (int)lin->k, (int)lin->group,
-                      (int)lin->tiles, p.kw, p.KW, p.KH, limit, y, ldy, rt, p.sp, slabs, tickets, ctx->d_status, ctx->wait_limit_ns);
+    return launch_pdl(ctx, kern, dim3((unsigned)grid), dim3(V4_THREADS), (size_t)smem, a, lda, M, lin->w, lin->row, (int)lin->n, (int)lin->k, (int)lin->group,
+                      (int)lin->record, (int)lin->tiles, p.kw, p.KW, p.KH, slots, limit, y, ldy, rt, p.sp, slabs, tickets, ctx->d_status, ctx->wait_limit_ns);
 }
 
 // slabs of a call
@@ -321,18 +330,17 @@ size_t slab_bytes(int sp, int64_t items, int nt) { return sp > 1 ? PG_LM_TICKET_
 
 size_t pgk_linear4_gemv_workspace(const pg_linear4 *lin)
 {
-    const int sp = (int)((lin->k + V4_WARPS * V4_KW_MAX - 1) / (V4_WARPS * V4_KW_MAX));
-    // (a route's blocks: as many as a route of 16 tokens can have would be 16 times the experts' rows; the experts' own number is the most)
-    return slab_bytes(sp, lin->tiles * lin->experts, 2);
+    // (a route of up to 16 tokens has a block per expert at most)
+    return std::max(slab_bytes(split_of(lin->k, 2), lin->tiles * lin->experts, 2), slab_bytes(split_of(lin->k, 1), lin->tiles, 1));
 }
 
 int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int64_t m, int act, float limit, void *y, int y_dtype, int64_t ldy,
                          const PgRouted *routed, int64_t max_blocks)
 {
     const int64_t items = lin->tiles * (routed ? max_blocks : 1);
-    const Parts p = parts_of(lin, items, ctx->sm_count);
     const int nt = m > 8 || routed ? 2 : 1;
-    PG_REQUIRE(p.KW <= V4_KW_MAX && p.sp <= 16, "linear4: K too long");
+    const Parts p = parts_of(lin, items, ctx->sm_count, nt);
+    PG_REQUIRE(p.KW <= v4_kw_max(nt) && p.sp <= 16, "linear4: K too long");
     if (p.sp > 1) {
         const int32_t rc = pg_splitk_reserve(ctx, slab_bytes(p.sp, items, nt));
         if (rc != PG_OK) return rc;

@@ -1,12 +1,13 @@
 // Product y = act(a W^T) with weights of 4 bits (csrc/pg_linear4.cu) and many rows, on the 5th-generation tensor cores.
 //
-//   * The weights are the M side: 128 rows to a tile, their quants unpacked to f16 in TMEM, 64 k at a time, by four warps (a thread per row);
-//     the activations are the N side, BN rows of f16 in shared memory by TMA.  scale * (q - 8) is an f16 number exactly (csrc/pg_linear4.cu), and
-//     linear4_rows_kernel writes the activations as f16 divided by a power of two per row, which holds bf16 numbers exactly down to 2^-29 of the
-//     row's largest: sums are those of the bf16 activations with the weights, in f32.
-//   * Warps 0 .. 3 unpack, 4 .. 7 write outputs (lane = weight row, so a store is 32 columns of one row of y), 8 copies, 9 issues the products.
-//     Two accumulators, so that outputs are written while the next tile is computed.
-//   * Few tiles: K is divided over CTAs; raw sums go to slabs, the last warp of a 32-row band to finish adds them in a fixed order.
+//   * The weights are the M side: a pair of CTAs has 256 rows, each unpacks its 128 to f16 in TMEM, 128 k at a time (a thread per row, sixteen warps in
+//     four teams that take the blocks in turn); the activations are the N side, BN rows of f16 in shared memory by TMA, half in each CTA.
+//     scale * (q - 8) is an f16 number exactly (csrc/pg_linear4.cu), and linear4_rows_kernel writes the activations as f16 divided by a power of two
+//     per row, which holds bf16 numbers exactly down to 2^-29 of the row's largest: sums are those of the bf16 activations with the weights.
+//   * An accumulator sums up 512 k; eight warps add the accumulators up in f32 registers.  (The tensor cores cut sums off: 4096 k in one
+//     accumulator were 3.9e-6 off 64 bits, 512 at a time 6e-7.)  They write the outputs: lane = weight row, so a store is 32 columns of one row of y.
+//   * Where whole tiles would leave SMs idle, the tiles' blocks of 128 k are divided evenly over the pairs of CTAs; sums of a tile that several share
+//     go to slabs, and the last warp to finish adds them in a fixed order.
 //   * ROUTED: BN rows belong to one expert; pieces of a 128-row block without a row are left out.
 //
 // Every mbarrier wait is bounded (pg_async.cuh).
@@ -18,29 +19,31 @@
 
 namespace {
 
-constexpr int T4_THREADS = 320;
-constexpr int BM = 128;                 // weight rows of a tile
-constexpr int W_BYTES = 8 * 512;        // quants of a tile and 64 k
-constexpr int S_BYTES = 8 * 32 * 2;     // scales of them (groups of 32: two to 64 k)
+constexpr int BM = 128;                 // weight rows of a CTA's tile
+constexpr int BK = 128;                 // columns of K in a block (the last one may have 64)
+constexpr int CHUNK = 4;                // blocks that one accumulator sums up
+constexpr int CG = 2;                   // CTAs of a pair
+constexpr int TEAMS = 4;                // of unpacking warps, four warps each; they take the blocks in turn
+constexpr int SLOTS = TEAMS;            // blocks in flight: activations in shared memory, unpacked weights in TMEM (64 columns each)
+// warps: the copies', the products' (and two without work), the unpacking ones, eight for the outputs
+constexpr int W_COPY = 0, W_MMA = 1, W_UNPACK = 4, W_OUT = W_UNPACK + 4 * TEAMS;
+constexpr int T4_THREADS = (W_OUT + 8) * 32;
+constexpr int DEPTH = 4, WARP_BLOCK = 4 * 576;         // blocks in an unpacking warp's own ring, bytes of one (32 rows x 128 k) at most
+constexpr int RING = 4 * TEAMS * DEPTH * WARP_BLOCK;
 
 template <int BN>
 struct Cfg {
-    static constexpr int X = BN * 128;
-    static constexpr int STAGE = X + W_BYTES + 1024;
-    static constexpr int ROOM = 227 * 1024 - 1024 - 512;
-    static constexpr int STAGES = ROOM / STAGE > 12 ? 12 : ROOM / STAGE;
-    static constexpr int A_SLOTS = BN > 128 ? 4 : 8;      // unpacked blocks of 64 k in TMEM, 32 columns each
+    static constexpr int XT = BN / CG * 128;              // 64 columns of a block of the activations, a CTA's half
     static constexpr int A_COL = 2 * BN;                  // behind the two accumulators
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE + 1024 + 512;
-    static_assert(A_COL + 32 * A_SLOTS <= 512, "TMEM");
+    static constexpr size_t SMEM = (size_t)SLOTS * 2 * XT + RING + 1024 + 256;
+    static constexpr int COLS = BN >= 64 ? BN / 2 : BN;   // accumulator columns of an output warp
+    // registers of a lane where the output warps' sums need more than an equal share: 28 x 72 of them, divided
+    static constexpr int R_UNPACK = 56, R_OUT = 120, R_REST = 40;
+    static constexpr bool SHARES = COLS >= 64;
+    static_assert(4 * TEAMS * R_UNPACK + 8 * R_OUT + 4 * R_REST == (W_OUT + 8) * 72, "no more registers than there are");
+    static_assert(A_COL + 64 * SLOTS <= 512 && SMEM <= 227 * 1024, "TMEM, shared memory");
 };
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *tmap, uint32_t bar, int x, int y, int z, int w)
-{
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(tmap),
-                 "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-                 : "memory");
-}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b)
 {
     uint32_t r;
@@ -107,99 +110,185 @@ __global__ void __launch_bounds__(RW_T)
     for (int at = threadIdx.x + RW_KEEP * RW_T; at < n; at += RW_T) put(at, __ldcg(row + at));
 }
 
-// How K is divided: parts of `blocks` 64-element blocks; slab of (unit, quarter): [BN][32 weight rows]
-struct KParts {
-    int parts, blocks;
+// How the work is divided.  blocks > 0: the tiles' blocks of 64 k, tile after tile, in stretches of `blocks`, one per pair of CTAs; a tile that several
+// pairs share is put together from slabs, [COLS][32 weight rows] for every (CTA, whether it is the first or the last of its stretch, output warp).
+// blocks == 0: whole tiles in turn.
+struct Share {
+    int blocks;
     float *slabs;
-    unsigned int *tickets;   // one per (tile, quarter), zero between calls
+    unsigned int *tickets;   // one per (tile, CTA of the pair, output warp), zero between calls
 };
+// a piece of a tile: blocks k0 .. k1 of 64 k
+struct Piece {
+    int tile, k0, k1;
+};
+
+// A warp's sums of weight rows n0 + lane with rows m0 .. of a (`left` of them exist) -> outputs
+template <int COLS, int ACT, bool ALL, typename TY>
+__device__ __forceinline__ void put_rows(const float (&v)[COLS], float fac, const float *xback, int m0, int left, bool in, TY *dst, int64_t ldy, int lane)
+{
+#pragma unroll
+    for (int c = 0; c < COLS; c += 16) {
+        if (!ALL && c >= left) break;                      // uniform over the warp
+        const float xb = ALL || (lane & 15) < left - c ? __ldcg(xback + m0 + c + (lane & 15)) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float o = v[c + j] * fac * __shfl_sync(0xffffffffu, xb, j);
+            if ((ALL || c + j < left) && in) pg_put(dst, o);
+            dst += ldy;
+        }
+    }
+}
+template <int COLS, int ACT, typename TY>
+__device__ __forceinline__ void put(const float (&v)[COLS], float fac, const float *xback, int m0, int left, int n0, int N, float limit, TY *y, int64_t ldy, int lane)
+{
+    const bool in = n0 + lane < N;
+    if constexpr (ACT == PG_ACT_NONE) {
+        TY *dst = y + (int64_t)m0 * ldy + n0 + lane;
+        if (left >= COLS)
+            put_rows<COLS, ACT, true>(v, fac, xback, m0, left, in, dst, ldy, lane);
+        else
+            put_rows<COLS, ACT, false>(v, fac, xback, m0, left, in, dst, ldy, lane);
+    } else {
+        // lanes l and l ^ 8 have a gate and its up: the gate's lane takes the even rows, the other the odd ones
+        const bool up = lane & 8;
+        TY *dst = y + (int64_t)(m0 + (up ? 1 : 0)) * ldy + n0 / 2 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 16) {
+            if (c >= left) break;                          // uniform over the warp
+            const float xb = (lane & 15) < left - c ? __ldcg(xback + m0 + c + (lane & 15)) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float v0 = v[c + j] * fac * __shfl_sync(0xffffffffu, xb, j), v1 = v[c + j + 1] * fac * __shfl_sync(0xffffffffu, xb, j + 1);
+                const float other = __shfl_xor_sync(0xffffffffu, up ? v0 : v1, 8);
+                const float o = pg_glu<ACT>(up ? other : v0, up ? v1 : other, limit);
+                if (c + j + (up ? 1 : 0) < left && in) pg_put(dst, o);
+                dst += 2 * ldy;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+    tmem_wait_ld();
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                 "r"(v[15]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+template <int N>
+__device__ __forceinline__ void set_regs_less()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_regs_more()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <int BN, int ACT, typename TY>
 __global__ void __launch_bounds__(T4_THREADS, 1)
-    linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_s,
-                      const float *__restrict__ wrow, const float *xback, int M, int N, int K, int group, int wtiles, float limit, TY *__restrict__ y, int64_t ldy,
-                      const PgRouted rt, const KParts kp, int32_t *status, unsigned long long limit_ns)
+    linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const unsigned char *__restrict__ w, const float *__restrict__ wrow, const float *xback, int M, int N,
+                      int K, int record, int wtiles, int alltiles, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, const Share sh, int32_t *status,
+                      unsigned long long limit_ns)
 {
     using C = Cfg<BN>;
-    constexpr int STAGES = C::STAGES, SLOTS = C::A_SLOTS;
+    constexpr int COLS = C::COLS;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = pg_smem(smem_raw), base = (raw_addr + 1023u) & ~1023u;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_raw + (base - raw_addr) + (size_t)STAGES * C::STAGE);
-    const uint32_t bar_full = pg_smem(bars), bar_empty = bar_full + 8 * STAGES, bar_afull = bar_empty + 8 * STAGES, bar_aempty = bar_afull + 8 * SLOTS,
-                   bar_tfull = bar_aempty + 8 * SLOTS, bar_tempty = bar_tfull + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2 * SLOTS + 4);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem_raw + (base - raw_addr) + SLOTS * 2 * C::XT + RING);
+    const uint32_t bar_full = pg_smem(bars), bar_free = bar_full + 8 * SLOTS, bar_tfull = bar_free + 8 * SLOTS, bar_tempty = bar_tfull + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * SLOTS + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    static_assert((2 * STAGES + 2 * SLOTS + 5) * 8 <= 512, "barriers");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (a shuffle's result is known to be the same in the whole warp: what follows from it stays in uniform registers)
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = (int)pg_cluster_rank();
+    constexpr int OUT_WARPS = BN >= 64 ? 8 : 4;           // that have columns
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; s++) {
-            pg_mbar_init(bar_full + 8 * s, 1);
-            pg_mbar_init(bar_empty + 8 * s, 1);
-        }
         for (int s = 0; s < SLOTS; s++) {
-            pg_mbar_init(bar_afull + 8 * s, 4);            // one arrival per unpacking warp
-            pg_mbar_init(bar_aempty + 8 * s, 1);
+            pg_mbar_init(bar_full + 8 * s, 4 * CG + 1);    // the warps of both CTAs' teams, and the copies of the activations
+            pg_mbar_init(bar_free + 8 * s, 1);
         }
         for (int i = 0; i < 2; i++) {
             pg_mbar_init(bar_tfull + 8 * i, 1);
-            pg_mbar_init(bar_tempty + 8 * i, 4);           // one arrival per output warp
+            pg_mbar_init(bar_tempty + 8 * i, OUT_WARPS * CG);
         }
         *abort_flag = 0;
         pg_mbar_fence();
     }
     __syncwarp();
-    if (warp == 9) tmem_alloc<1>(pg_smem(tmem_slot), 512);
+    if (warp == W_MMA) tmem_alloc<CG>(pg_smem(tmem_slot), 512);
     tc_fence_before();
-    __syncthreads();
+    pg_group_sync<CG>();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const bool routed = rt.blocks != nullptr;
     if (routed) asm volatile("griddepcontrol.wait;" ::: "memory");   // the list of tiles comes from the preceding kernels
-    const int tiles_m = routed ? __ldcg(rt.blocks) * (PG_ROUTE_BLOCK / BN) : (M + BN - 1) / BN;
-    const int tiles_n = (N + BM - 1) / BM;
-    const int sp = kp.parts, total = tiles_m * tiles_n * sp;   // unit u: part u % sp of tile u / sp
-    const int kblocks = K / 64;
+    constexpr int PER_BLOCK = PG_ROUTE_BLOCK / BN;
+    const int tiles_m = routed ? __shfl_sync(0xffffffffu, __ldcg(rt.blocks), 0) * PER_BLOCK : (M + BN - 1) / BN;
+    const int tiles_n = (N + CG * BM - 1) / (CG * BM);
+    const int total = tiles_m * tiles_n, unit0 = blockIdx.x / CG, units = gridDim.x / CG, kblocks = (K + BK - 1) / BK;
     const int rows = routed ? tiles_m * BN : M;
-    auto k_first = [&](int u) { return (u % sp) * kp.blocks; };
-    auto k_end = [&](int u) { return min(kblocks, (u % sp + 1) * kp.blocks); };
     // a piece of a route's block that has no row (they are filled from the first on)
-    auto nothing = [&](int u) { return routed && __ldcg(rt.row_pair + (int64_t)(u / sp % tiles_m) * BN) < 0; };
-    const int gs = group == 32 ? 2 : 1;                    // scales of a row to 64 k
-    const uint32_t stage_bytes = (uint32_t)(C::X + W_BYTES + 8 * 32 * gs);
+    auto nothing = [&](int tile) { return routed && __ldcg(rt.row_pair + (int64_t)(tile % tiles_m) * BN) < 0; };
+    // the pieces of this pair, in their order; at: block (or tile) that comes next
+    const int64_t at0 = sh.blocks ? (int64_t)unit0 * sh.blocks : unit0;
+    const int64_t at_end = sh.blocks ? min(at0 + sh.blocks, (int64_t)total * kblocks) : total;
+    auto next = [&](int64_t &at, Piece &p) {
+        if (sh.blocks) {
+            if (at >= at_end) return false;
+            p.tile = (int)(at / kblocks);
+            p.k0 = (int)(at - (int64_t)p.tile * kblocks);
+            p.k1 = (int)min((int64_t)kblocks, p.k0 + (at_end - at));
+            at += p.k1 - p.k0;
+            return true;
+        }
+        while (at < at_end && nothing((int)at)) at += units;
+        if (at >= at_end) return false;
+        p = {(int)at, 0, kblocks};
+        at += units;
+        return true;
+    };
+    // first of the CTA's 16-row tiles in the weights' layout
+    auto w_tile = [&](int tile) { return (routed ? __ldcg(rt.block_expert + tile % tiles_m / PER_BLOCK) * wtiles : 0) + (tile / tiles_m * CG + rank) * (BM / 16); };
+    const bool odd = (K / 64) & 1;                         // the last block has 64 columns
 
-    if (warp == 8) {
-        // ---------------------------------------------------------------- copies
-        if (lane == 0) {
-            uint32_t stage = 0, phase = 0;
+    if (warp < W_UNPACK) {
+        if constexpr (C::SHARES) set_regs_less<C::R_REST>();
+        if (warp == W_COPY && lane == 0) {
+            // ------------------------------------------------------------ activations
+            uint32_t slot = 0, phase = 1;
             bool ok = true;
-            auto weights = [&](uint32_t at, uint32_t bar, int kb, int tile) {
-                const int mt = tile % tiles_m, wt = (routed ? __ldcg(rt.block_expert + mt / (PG_ROUTE_BLOCK / BN)) * wtiles : 0) + tile / tiles_m * (BM / 16);
-                pg_mbar_expect(bar, stage_bytes);
-                tma_load_4d(at + C::X, &map_w, bar, 0, 0, kb, wt);
-                tma_load_3d(at + C::X + W_BYTES, &map_s, bar, 0, kb * 64 / group, wt);
-            };
-            int early = 0;
-            if (!routed) {
-                if ((int)blockIdx.x < total) {
-                    const int u = blockIdx.x, first = k_first(u);
-                    early = min(k_end(u) - first, STAGES);
-                    for (int i = 0; i < early; i++) weights(base + i * C::STAGE, bar_full + 8 * i, first + i, u / sp);
-                }
-                asm volatile("griddepcontrol.wait;" ::: "memory");
-            }
-            for (int u = blockIdx.x; ok && u < total; u += gridDim.x) {
-                if (nothing(u)) continue;
-                const int tile = u / sp, m0 = tile % tiles_m * BN;
-                for (int kb = k_first(u), end = k_end(u); kb < end; kb++) {
-                    if (!(ok = pg_mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, status, limit_ns))) break;
-                    const uint32_t at = base + stage * C::STAGE;
-                    if (early > 0)
-                        early--;
-                    else
-                        weights(at, bar_full + 8 * stage, kb, tile);
-                    tma_load_2d(at, &map_x, bar_full + 8 * stage, kb * 64, m0);
-                    if (++stage == STAGES) stage = 0, phase ^= 1;
+            const uint32_t full_leader = pg_leader<CG>(bar_full);
+            if (!routed) asm volatile("griddepcontrol.wait;" ::: "memory");
+            Piece p;
+            for (int64_t at = at0; ok && next(at, p);) {
+                const int m0 = p.tile % tiles_m * BN + rank * (BN / CG);
+                for (int kb = p.k0; kb < p.k1; kb++) {
+                    if (!(ok = pg_mbar_wait(bar_free + 8 * slot, phase, abort_flag, status, limit_ns))) break;
+                    const bool half = odd && kb == kblocks - 1;
+                    const uint32_t to = base + slot * (2 * C::XT), bar = full_leader + 8 * slot;
+                    if (rank == 0) pg_mbar_expect(bar_full + 8 * slot, half ? BN * 128 : BN * 256);
+                    tma_load_2d_to<CG>(to, &map_x, bar, kb * BK, m0);
+                    if (!half) tma_load_2d_to<CG>(to + C::XT, &map_x, bar, kb * BK + 64, m0);
+                    if (++slot == SLOTS) slot = 0, phase ^= 1;
                 }
             }
             if (!ok) {
@@ -208,253 +297,300 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
                 while (pg_globaltimer_ns() - t0 < 2000000ull) {
                 }
             }
-        }
-    } else if (warp == 9) {
-        // ---------------------------------------------------------------- products (the whole warp; one lane's count)
-        const uint32_t on = pg_elect();
-        constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);   // f16 operands, f32 sums
-        uint32_t stage = 0, phase = 0, slot = 0, aphase = 0, acc = 0, acc_phase = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; ok && u < total; u += gridDim.x) {
-            if (nothing(u)) continue;
-            if (!(ok = pg_mbar_wait_warp(bar_tempty + 8 * acc, acc_phase ^ 1, abort_flag, status, limit_ns))) break;
-            tc_fence_after();
-            const uint32_t d = tmem + acc * BN;
-            const int first = k_first(u), end = k_end(u);
-            for (int kb = first; kb < end; kb++) {
-                if (!(ok = pg_mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, status, limit_ns))) break;
-                if (!(ok = pg_mbar_wait_warp(bar_afull + 8 * slot, aphase, abort_flag, status, limit_ns))) break;
-                tc_fence_after();
-                const uint64_t db = make_smem_desc(base + stage * C::STAGE);
-                const uint32_t ta = tmem + C::A_COL + slot * 32;
+        } else if (warp == W_MMA && rank == 0) {
+            // ------------------------------------------------------------ products (the whole warp; one lane's count)
+            // This warp shares its scheduler with four that unpack and two that write: every instruction here counts, so one wait and one
+            // commit for 128 k (waits and commits of their own for the activations and for 64 k took 27 us instead of 17 rows x 14336 x 4096's 22).
+            const uint32_t on = pg_elect();
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CG * BM >> 4) << 24);   // f16 operands, f32 sums
+            uint32_t slot = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true;
+            Piece p;
+            for (int64_t at = at0; ok && next(at, p);) {
+                int in = 0;
+                for (int kb = p.k0; kb < p.k1; kb++) {
+                    const uint32_t d = tmem + acc * BN;
+                    if (in == 0) {
+                        if (!(ok = pg_mbar_wait_warp(bar_tempty + 8 * acc, acc_phase ^ 1, abort_flag, status, limit_ns))) break;
+                    }
+                    if (!(ok = pg_mbar_wait_warp(bar_full + 8 * slot, phase, abort_flag, status, limit_ns))) break;
+                    tc_fence_after();
+                    const uint64_t db = make_smem_desc(base + slot * (2 * C::XT));
+                    const uint32_t ta = tmem + C::A_COL + slot * 64;
 #pragma unroll
-                for (int j = 0; j < 4; j++) umma_f16_ta(d, ta + j * 8, db + (uint64_t)(j * 2), idesc, kb != first || j != 0 ? 1u : 0u, on);
-                umma_commit(bar_empty + 8 * stage, on);
-                umma_commit(bar_aempty + 8 * slot, on);
-                if (++stage == STAGES) stage = 0, phase ^= 1;
-                if (++slot == SLOTS) slot = 0, aphase ^= 1;
+                    for (int j = 0; j < 4; j++) umma_f16_ta_of<CG>(d, ta + j * 8, db + (uint64_t)(j * 2), idesc, in != 0 || j != 0 ? 1u : 0u, on);
+                    if (!(odd && kb == kblocks - 1)) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) umma_f16_ta_of<CG>(d, ta + 32 + j * 8, db + (uint64_t)((C::XT >> 4) + j * 2), idesc, 1u, on);
+                    }
+                    umma_commit_to<CG>(bar_free + 8 * slot, on);
+                    if (++slot == SLOTS) slot = 0, phase ^= 1;
+                    if (++in == CHUNK || kb == p.k1 - 1) {
+                        umma_commit_to<CG>(bar_tfull + 8 * acc, on);
+                        in = 0;
+                        if (++acc == 2) acc = 0, acc_phase ^= 1;
+                    }
+                }
             }
-            if (!ok) break;
-            umma_commit(bar_tfull + 8 * acc, on);
-            if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
-    } else if (warp < 4) {
+    } else if (warp < W_OUT) {
         // ---------------------------------------------------------------- quants -> f16 in TMEM: a thread per weight row
-        const int ti = 2 * warp + (lane >> 4), rr = lane & 15;
-        const uint32_t off = (uint32_t)(ti * 512 + (rr & 7) * 64), swz = (off >> 7 & 7u) << 4;   // (bits 7 .. 9 do not change over the row's 64 bytes)
+        if constexpr (C::SHARES) set_regs_less<C::R_UNPACK>();
+        // A warp copies what it unpacks itself: 32 rows of every fourth of the pieces' blocks, one after the other, through a ring of its own.
+        // (Tensor copies of the tiles, issued by one thread, took 385 to 520 cycles per 64 k.)
+        const int team = (warp - W_UNPACK) >> 2, quarter = warp & 3, ti = lane >> 4, rr = lane & 15;
+        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(warp - W_UNPACK) * (DEPTH * WARP_BLOCK);
+        const int chunks = 2 * record / 16;                    // 16-byte pieces of a 16-row tile's two records
+        const uint32_t off = (uint32_t)(ti * 2 * record + (rr & 7) * 64), swz = (uint32_t)(rr >> 1 & 3) << 4;
         const uint32_t mask = rr < 8 ? FOUR_LO : FOUR_HI, sub = rr < 8 ? FOUR_OFF_LO : FOUR_OFF_HI;
         const uint32_t less = rr < 8 ? 0x3c003c00u : 0x2c002c00u;     // 1, and 1 / 16
-        uint32_t stage = 0, phase = 0, slot = 0, aphase = 0;
+        const uint32_t s_off = (uint32_t)(ti * 2 * record + 512 + (rr & 7) * 4 + (rr >> 3) * 2), s_step = record > 544 ? 32u : 0u;
+        const uint32_t q_off[4] = {off + swz, off + (16u ^ swz), off + (32u ^ swz), off + (48u ^ swz)};
+        const uint32_t a_at = tmem + ((uint32_t)(quarter * 32) << 16) + C::A_COL + team * 64, full = pg_leader<CG>(bar_full) + 8 * team, free_at = bar_free + 8 * team;
+        // where copies go on: block kb of the piece `to`
+        const unsigned char *from = w;
+        uint32_t piece[5];                                     // where a lane's 16-byte pieces are, from `from` on
+        int64_t to_at = at0;
+        Piece to = {0, 0, 0};
+        int kb = team;
+        bool more = true;
+        auto seek = [&]() {                                    // to the piece that has the block
+            while (kb >= to.k1) {
+                kb -= to.k1;
+                if (!(more = next(to_at, to))) return;
+                kb += to.k0;
+                // (rows behind the last weights repeat the last ones, whose sums are dropped)
+                const int wt = min(w_tile(to.tile) + quarter * 2, alltiles - 1);
+                const uint32_t stride = wt + 1 < alltiles ? (uint32_t)(K / 64 * record) : 0u;
+                from = w + ((int64_t)wt * (K / 64) + 2 * kb) * record;
+#pragma unroll
+                for (int i = 0; i < 5; i++) {
+                    const int c = lane + 32 * i, second = c >= chunks ? 1 : 0;
+                    piece[i] = second * stride + (uint32_t)(c - second * chunks) * 16;
+                }
+            }
+        };
+        seek();
+        uint32_t put_at = ring, get_at = ring;
+        auto bring = [&]() {
+            if (more) {
+                const bool half = odd && kb == kblocks - 1;
+#pragma unroll
+                for (int i = 0; i < 5; i++) {
+                    const int c = lane + 32 * i, in = c >= chunks ? c - chunks : c;
+                    if (c < 2 * chunks && (!half || in < chunks / 2)) pg_cp16(put_at + (uint32_t)c * 16, from + piece[i]);
+                }
+                from += TEAMS * 2 * record;
+                kb += TEAMS;
+                if (kb >= to.k1) seek();
+            }
+            pg_cp_commit();
+            put_at += WARP_BLOCK;
+            if (put_at == ring + DEPTH * WARP_BLOCK) put_at = ring;
+        };
+        // the blocks that are unpacked: every fourth of all; of these the one that may be half
+        int64_t read_at = at0;
+        Piece now = {0, 0, 0};
+        int rb = team;
+        for (int i = 0; i < DEPTH - 1; i++) bring();
+        uint32_t phase = 1;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < total; u += gridDim.x) {
-            if (nothing(u)) continue;
-            for (int kb = k_first(u), end = k_end(u); kb < end; kb++) {
-                if (!(ok = pg_mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, status, limit_ns))) break;
-                const uint32_t at = base + stage * C::STAGE + C::X;
-                uint4 q[4];
+#pragma unroll 1
+        for (;; rb += TEAMS) {
+            while (rb >= now.k1) {
+                rb -= now.k1;
+                if (!next(read_at, now)) {
+                    rb = -1;
+                    break;
+                }
+                rb += now.k0;
+            }
+            if (rb < 0) break;
+            const int halves = odd && rb == kblocks - 1 ? 1 : 2;
+            pg_cp_wait<DEPTH - 2>();
+            __syncwarp();
+            // (the slot that is filled now was read in the last round)
+            bring();
+            uint32_t at = get_at, to_tmem = a_at;
+#pragma unroll 1
+            for (int c = 0; c < 2 * halves; c += 2) {          // 64 columns; then 32 at a time: words 2 i and 2 i + 1 of the row's four lanes
 #pragma unroll
-                for (int i = 0; i < 4; i++) q[i] = pg_lds128(at + ((off + i * 16) ^ swz));
-                uint32_t sc[2];
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
+                for (int e = 0; e < 2; e++) {
                     unsigned short h;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + W_BYTES + (uint32_t)((ti * gs + (gs == 2 ? c : 0)) * 32 + rr * 2)));
-                    sc[c] = mul_f16x2((uint32_t)h * 0x10001u, less);
-                }
-                uint32_t v[32];
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + s_off + e * s_step));
+                    const uint32_t sc = mul_f16x2((uint32_t)h * 0x10001u, less);
+                    uint32_t v[16];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+                    for (int i = 0; i < 4; i++) {
+                        const uint2 q = lds64(at + q_off[i] + e * 8);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int to = 16 * (j >> 1) + 4 * i + 2 * (j & 1);
-                        v[to] = mul_f16x2(four_sub_f16(four_lop(w[j], mask, FOUR_F16), sub), sc[j >> 1]);
-                        v[to + 1] = mul_f16x2(four_sub_f16(four_lop(w[j] >> 8, mask, FOUR_F16), sub), sc[j >> 1]);
-                    }
-                }
-                if (!(ok = pg_mbar_wait_warp(bar_aempty + 8 * slot, aphase ^ 1, abort_flag, status, limit_ns))) break;
-                tc_fence_after();
-                tmem_st32(tmem + ((uint32_t)(warp * 32) << 16) + C::A_COL + slot * 32, v);
-                tmem_wait_st();
-                tc_fence_before();
-                pg_mbar_arrive_warp(bar_afull + 8 * slot, lane);
-                if (++stage == STAGES) stage = 0, phase ^= 1;
-                if (++slot == SLOTS) slot = 0, aphase ^= 1;
-            }
-        }
-    } else {
-        // ---------------------------------------------------------------- outputs
-        const int q = warp & 3;
-        if (!routed) asm volatile("griddepcontrol.wait;" ::: "memory");   // y may still be read by the predecessor; xback is its work
-        uint32_t acc = 0, acc_phase = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; ok && u < total; u += gridDim.x) {
-            if (nothing(u)) continue;
-            const int tile = u / sp, mt = tile % tiles_m, m0 = mt * BN, n0 = tile / tiles_m * BM + q * 32;
-            const int64_t wt = (routed ? (int64_t)__ldcg(rt.block_expert + mt / (PG_ROUTE_BLOCK / BN)) * wtiles : 0) + n0 / 16;
-            const float fac = n0 + lane < wtiles * 16 ? __ldg(wrow + wt * 16 + lane) : 0.0f;
-            if (!(ok = pg_mbar_wait_warp(bar_tfull + 8 * acc, acc_phase, abort_flag, status, limit_ns))) break;
-            tc_fence_after();
-            // sums of weight row n0 + lane with rows m0 + c .. of a
-            auto put = [&](const uint32_t (&v)[32], int c) {
-                const int m = m0 + c, left = rows - m;
-                const float xb = lane < left ? __ldcg(xback + m + lane) : 0.0f;
-                if constexpr (ACT != PG_ACT_NONE) {
-                    // lanes l and l ^ 8 have a gate and its up: the gate's lane takes the even rows, the other the odd ones
-                    const bool up = lane & 8;
-                    TY *dst = y + (int64_t)m * ldy + n0 / 2 + (lane >> 4) * 8 + (lane & 7);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float b0 = __shfl_sync(0xffffffffu, xb, j), b1 = __shfl_sync(0xffffffffu, xb, j + 1);
-                        const float v0 = __uint_as_float(v[j]) * fac * b0, v1 = __uint_as_float(v[j + 1]) * fac * b1;
-                        const float other = __shfl_xor_sync(0xffffffffu, up ? v0 : v1, 8);
-                        const float o = up ? pg_glu<ACT>(other, v1, limit) : pg_glu<ACT>(v0, other, limit);
-                        const int jj = up ? j + 1 : j;
-                        if (jj < left && n0 + lane < N) pg_put(dst + (int64_t)jj * ldy, o);
-                    }
-                } else {
-                    TY *dst = y + (int64_t)m * ldy + n0 + lane;
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float b = __shfl_sync(0xffffffffu, xb, j);
-                        if (j < left && n0 + lane < N) pg_put(dst + (int64_t)j * ldy, __uint_as_float(v[j]) * fac * b);
-                    }
-                }
-            };
-#pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
-                if (m0 + c >= rows || n0 >= N) break;         // uniform over the warp
-                uint32_t v[32];
-                tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + acc * BN + c, v);
-                if (sp > 1) {
-                    float *slab = kp.slabs + (((int64_t)u * 4 + q) * BN + c) * 32 + lane;
-#pragma unroll
-                    for (int j = 0; j < 32; j++) __stcg(slab + j * 32, __uint_as_float(v[j]));
-                } else {
-                    put(v, c);
-                }
-            }
-            tc_fence_before();
-            pg_mbar_arrive_warp(bar_tempty + 8 * acc, lane);
-            if (sp > 1 && n0 < N) {
-                unsigned int *ticket = kp.tickets + tile * 4 + q;
-                __threadfence();
-                __syncwarp();
-                const unsigned int before = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(ticket, 1u) : 0u, 0);
-                if (before == (unsigned)(sp - 1)) {
-                    __threadfence();
-                    if (lane == 0) *ticket = 0;
-#pragma unroll 1
-                    for (int c = 0; c < BN; c += 32) {
-                        if (m0 + c >= rows) break;
-                        const float *slab = kp.slabs + (((int64_t)tile * sp * 4 + q) * BN + c) * 32 + lane;
-                        float sum[32];
-#pragma unroll
-                        for (int j = 0; j < 32; j++) sum[j] = __ldcg(slab + j * 32);
-                        for (int p = 1; p < sp; p++) {
-                            const float *at = slab + (int64_t)p * 4 * BN * 32;
-                            float b[32];
-#pragma unroll
-                            for (int j = 0; j < 32; j++) b[j] = __ldcg(at + j * 32);
-#pragma unroll
-                            for (int j = 0; j < 32; j++) sum[j] += b[j];
+                        for (int j = 0; j < 2; j++) {
+                            const uint32_t word = j ? q.y : q.x;
+                            v[4 * i + 2 * j] = mul_f16x2(four_sub_f16(four_lop(word, mask, FOUR_F16), sub), sc);
+                            v[4 * i + 2 * j + 1] = mul_f16x2(four_sub_f16(four_lop(word >> 8, mask, FOUR_F16), sub), sc);
                         }
-                        uint32_t v[32];
+                    }
+                    if (e == 0 && c == 0) {
+                        if (!(ok = pg_mbar_wait_warp(free_at, phase, abort_flag, status, limit_ns))) break;
+                        tc_fence_after();
+                    }
+                    tmem_st16(to_tmem + e * 16, v);
+                }
+                if (!ok) break;
+                at += record, to_tmem += 32;
+            }
+            if (!ok) break;
+            tmem_wait_st();
+            tc_fence_before();
+            pg_arrive_leader_warp<CG>(full, lane);
+            get_at += WARP_BLOCK;
+            if (get_at == ring + DEPTH * WARP_BLOCK) get_at = ring;
+            phase ^= 1;
+        }
+        pg_cp_wait<0>();
+    } else {
+        // ---------------------------------------------------------------- outputs: the accumulators' sums added up in registers, then written
+        if constexpr (C::SHARES) set_regs_more<C::R_OUT>();
+        const int q = warp & 3, half = (warp - W_OUT) >> 2;
+        if (!routed) asm volatile("griddepcontrol.wait;" ::: "memory");   // y may still be read by the predecessor; xback is its work
+        if (half == 0 || OUT_WARPS == 8) {
+            const uint32_t tempty_leader = pg_leader<CG>(bar_tempty);
+            uint32_t acc = 0, acc_phase = 0;
+            bool ok = true;
+            Piece p;
+            for (int64_t at = at0; ok && next(at, p);) {
+                const int m0 = p.tile % tiles_m * BN + half * COLS, n0 = (p.tile / tiles_m * CG + rank) * BM + q * 32;
+                const float fac = n0 + lane < wtiles * 16 ? __ldg(wrow + (int64_t)(w_tile(p.tile) + q * 2) * 16 + lane) : 0.0f;
+                float sum[COLS];
+                for (int left = p.k1 - p.k0, first = 1; left > 0; left -= CHUNK, first = 0) {
+                    if (!(ok = pg_mbar_wait_warp(bar_tfull + 8 * acc, acc_phase, abort_flag, status, limit_ns))) break;
+                    tc_fence_after();
 #pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = __float_as_uint(sum[j]);
-                        put(v, c);
+                    for (int c = 0; c < COLS; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + acc * BN + half * COLS + c, v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sum[c + j] = first ? __uint_as_float(v[j]) : sum[c + j] + __uint_as_float(v[j]);
+                    }
+                    tc_fence_before();
+                    pg_arrive_leader_warp<CG>(tempty_leader + 8 * acc, lane);
+                    if (++acc == 2) acc = 0, acc_phase ^= 1;
+                }
+                if (!ok) break;
+                if (n0 >= N || m0 >= rows) {
+                    // (nothing of the warp's piece lies inside y)
+                } else if (p.k1 - p.k0 == kblocks) {
+                    put<COLS, ACT>(sum, fac, xback, m0, rows - m0, n0, N, limit, y, ldy, lane);
+                } else {
+                    // the tile's pairs: a pair's piece is the first of its stretch unless that starts at the tile's beginning or in front of it
+                    const int64_t b0 = (int64_t)p.tile * kblocks;
+                    const int lo = (int)(b0 / sh.blocks), hi = (int)((b0 + kblocks - 1) / sh.blocks);
+                    auto slab_of = [&](int pair) {
+                        const int64_t last = (int64_t)pair * sh.blocks > b0 ? 0 : 1;
+                        return sh.slabs + ((((int64_t)pair * CG + rank) * 2 + last) * OUT_WARPS + (warp - W_OUT)) * (COLS * 32) + lane;
+                    };
+                    float *mine = slab_of(unit0);
+#pragma unroll
+                    for (int j = 0; j < COLS; j++) __stcg(mine + j * 32, sum[j]);
+                    unsigned int *ticket = sh.tickets + (p.tile * CG + rank) * OUT_WARPS + (warp - W_OUT);
+                    __threadfence();
+                    __syncwarp();
+                    const unsigned int before = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(ticket, 1u) : 0u, 0);
+                    if (before == (unsigned)(hi - lo)) {
+                        // the last one in adds them up in their order
+                        __threadfence();
+                        if (lane == 0) *ticket = 0;
+#pragma unroll
+                        for (int c = 0; c < COLS; c += 16) {
+                            float a[16];
+#pragma unroll
+                            for (int j = 0; j < 16; j++) a[j] = 0.0f;
+                            for (int pair = lo; pair <= hi; pair++) {
+                                const float *from = slab_of(pair) + c * 32;
+                                float b[16];
+#pragma unroll
+                                for (int j = 0; j < 16; j++) b[j] = __ldcg(from + j * 32);
+#pragma unroll
+                                for (int j = 0; j < 16; j++) a[j] += b[j];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 16; j++) sum[c + j] = a[j];
+                        }
+                        put<COLS, ACT>(sum, fac, xback, m0, rows - m0, n0, N, limit, y, ldy, lane);
                     }
                 }
             }
-            if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
     }
+    // (neither CTA of a pair may leave while the other can still touch its shared memory, barriers or TMEM)
     __syncwarp();
     tc_fence_before();
-    __syncthreads();
-    if (warp == 9) {
+    pg_group_sync<CG>();
+    if (warp == W_MMA) {
         tc_fence_after();
-        tmem_dealloc<1>(tmem, 512);
+        tmem_dealloc<CG>(tmem, 512);
     }
 }
 
 // ---------------------------------------------------------------- host side ----
-constexpr int SLAB_ROWS = 256;         // rows of slabs (128 weight rows each) per SM, at most
-
 template <int BN, int ACT, typename TY>
-int32_t launch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float *xback, int64_t m, float limit, TY *y, int64_t ldy, const PgRouted &rt, KParts kp)
+int32_t launch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float *xback, int64_t m, float limit, TY *y, int64_t ldy, const PgRouted &rt, Share sh)
 {
     using C = Cfg<BN>;
-    CUtensorMap mx, mw, ms;
+    CUtensorMap mx;
     const cuuint64_t xd[2] = {(cuuint64_t)lin->k, (cuuint64_t)m}, xs[1] = {(cuuint64_t)lin->k * 2};
-    const cuuint32_t xb[2] = {64, (cuuint32_t)BN};
+    const cuuint32_t xb[2] = {64, (cuuint32_t)(BN / CG)};
     int32_t rc = pg_encode_map(&mx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, 2, xd, xs, xb);
-    if (rc) return rc;
-    const cuuint64_t tiles = (cuuint64_t)(lin->experts * lin->tiles), kb = (cuuint64_t)(lin->k / 64), kg = (cuuint64_t)(lin->k / lin->group);
-    const cuuint64_t wd[4] = {32, 4, kb, tiles}, wst[3] = {128, 512, kb * 512};
-    const cuuint32_t wb[4] = {32, 4, 1, 8};
-    rc = pg_encode_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT32, lin->q, 4, wd, wst, wb);
-    if (rc) return rc;
-    const cuuint64_t sd[3] = {16, kg, tiles}, sst[2] = {32, kg * 32};
-    const cuuint32_t sb[3] = {16, lin->group == 32 ? 2u : 1u, 8};
-    rc = pg_encode_map(&ms, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, lin->s, 3, sd, sst, sb, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc) return rc;
     auto kern = linear4_tc_kernel<BN, ACT, TY>;
     static std::atomic<uint64_t> set{0};
     PG_CUDA(pg_max_smem_once(kern, (int)C::SMEM, ctx->device, set));
-    const int64_t units = ((m + BN - 1) / BN) * ((lin->n + BM - 1) / BM) * kp.parts;
-    PG_REQUIRE(units < (1ll << 31) - 65536, "linear4: too many tiles");
-    kp.tickets = reinterpret_cast<unsigned int *>(ctx->splitk);
-    kp.slabs = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES);
-    return launch_pdl(ctx, kern, dim3((unsigned)std::min<int64_t>(units, ctx->sm_count)), dim3(T4_THREADS), C::SMEM, mx, mw, ms, lin->row, xback, (int)m, (int)lin->n,
-                      (int)lin->k, (int)lin->group, (int)lin->tiles, limit, y, ldy, rt, kp, ctx->d_status, ctx->wait_limit_ns);
+    const int64_t tiles = ((m + BN - 1) / BN) * ((lin->n + CG * BM - 1) / (CG * BM)), pairs = ctx->sm_count / CG;
+    PG_REQUIRE(tiles < (1ll << 31) - 65536, "linear4: too many tiles");
+    const int64_t grid = sh.blocks ? (tiles * ((lin->k + BK - 1) / BK) + sh.blocks - 1) / sh.blocks : std::min<int64_t>(tiles, pairs);
+    sh.tickets = reinterpret_cast<unsigned int *>(ctx->splitk);
+    sh.slabs = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES);
+    return launch_pdl_cluster(ctx, kern, dim3((unsigned)(grid * CG)), dim3(T4_THREADS), C::SMEM, CG, mx, lin->w, lin->row, xback, (int)m, (int)lin->n, (int)lin->k,
+                              (int)lin->record, (int)lin->tiles, (int)(lin->experts * lin->tiles), limit, y, ldy, rt, sh, ctx->d_status, ctx->wait_limit_ns);
 }
 
 template <int ACT, typename TY>
 int32_t dispatch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float *xback, int64_t m, float limit, TY *y, int64_t ldy, const PgRouted &rt, int64_t pairs)
 {
-    const int kblocks = (int)(lin->k / 64);
-    const int64_t tiles_n = (lin->n + BM - 1) / BM;
-    KParts kp = {1, kblocks, nullptr, nullptr};
+    const int kblocks = (int)((lin->k + BK - 1) / BK);
+    Share sh = {0, nullptr, nullptr};
     int bn = 128;
     if (rt.blocks) {
         // rows an expert has on average
         const int64_t rows = (pairs + lin->experts - 1) / lin->experts;
-        bn = rows <= 24 ? 32 : rows <= 48 ? 64 : 128;
+        bn = rows <= 12 ? 16 : rows <= 24 ? 32 : rows <= 48 ? 64 : 128;
     } else {
-        // cycles of a block of 64 k: its products (2 BN), the unpacking, and its bytes at what L2 gives an SM; of a unit: its outputs
+        // cycles: of a block of 128 k, its products (4 BN) or the unpacking; of a pair's stretch, with what it costs to put shared tiles together
         double best = 1e30;
-        for (int cand : {32, 64, 128, 192}) {
-            const int64_t tiles = ((m + cand - 1) / cand) * tiles_n;
-            const double block = std::max({2.0 * cand, 190.0, (4600.0 + 128.0 * cand) / 60.0});
-            for (int parts = 1; parts <= std::min(16, kblocks / 4 > 0 ? kblocks / 4 : 1); parts++) {
-                const int blocks = (kblocks + parts - 1) / parts, real = (kblocks + blocks - 1) / blocks;
-                if (real != parts) continue;
-                if (parts > 1 && (tiles * parts * cand > (int64_t)ctx->sm_count * SLAB_ROWS || tiles > 4096)) break;
-                const int64_t rounds = (tiles * parts + ctx->sm_count - 1) / ctx->sm_count;
-                const double time = rounds * (blocks * block + (parts > 1 ? 300 + 8.0 * cand : 0)) + 1000 + 20.0 * cand + (parts > 1 ? 1500 + parts * 8.0 * cand : 0);
-                if (time < best) {
-                    best = time;
-                    bn = cand;
-                    kp.parts = parts;
-                    kp.blocks = blocks;
-                }
-            }
+        const int64_t sm_pairs = ctx->sm_count / CG;
+        for (int cand : {16, 32, 64, 128}) {
+            const int64_t tiles = ((m + cand - 1) / cand) * ((lin->n + CG * BM - 1) / (CG * BM)), rounds = (tiles + sm_pairs - 1) / sm_pairs;
+            const double block = std::max(4.0 * cand, 500.0), whole = (double)rounds * kblocks * block;
+            if (whole < best) best = whole, bn = cand, sh.blocks = 0;
+            if (tiles > 1024) continue;
+            const int64_t blocks = std::max<int64_t>(2, (tiles * kblocks + sm_pairs - 1) / sm_pairs);
+            const double time = blocks * block + 4000.0 + 16.0 * cand;
+            if (time < best) best = time, bn = cand, sh.blocks = (int)blocks;
         }
     }
-    if (kp.parts > 1) {
+    if (sh.blocks) {
         const int32_t rc = pg_splitk_reserve(ctx, pgk_linear4_tc_workspace(ctx));
         if (rc != PG_OK) return rc;
     }
-    if (bn == 192) return launch<192, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, kp);
-    if (bn == 128) return launch<128, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, kp);
-    if (bn == 64) return launch<64, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, kp);
-    return launch<32, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, kp);
+    if (bn == 128) return launch<128, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
+    if (bn == 64) return launch<64, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
+    if (bn == 32) return launch<32, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
+    return launch<16, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
 }
 
 }  // namespace
 
-size_t pgk_linear4_tc_workspace(const pg_ctx *ctx) { return PG_LM_TICKET_BYTES + (size_t)ctx->sm_count * SLAB_ROWS * BM * sizeof(float); }
+size_t pgk_linear4_tc_workspace(const pg_ctx *ctx) { return PG_LM_TICKET_BYTES + (size_t)ctx->sm_count * 2 * 128 * BM * sizeof(float); }
 
 int32_t pgk_linear4_tc(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int64_t m, int act, float limit, void *y, int y_dtype, int64_t ldy,
                        const PgRouted *routed, int64_t pairs)
