@@ -155,6 +155,31 @@ PG_API int64_t pg_attention_part_floats(pg_ctx *ctx, const pg_attention *p, int6
 PG_API int32_t pg_attention_run(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, const float *d_proj, int64_t ldp, void *d_kcache,
                                 void *d_vcache, void *d_out, int32_t dtype, int64_t ldo);
 
+/* ---- attention over a cache in 4 bits ----
+ * The same layers (pg_attention, bf16 steps) over keys and values that are held in 4 bits with a scale per 32 columns of a position: scale = bf16(v / -8),
+ * v the value of largest magnitude (the first of equals), a value is scale * (q - 8), q = clamp(rint(x / scale) + 8, 0, 15).  A step appends its positions and
+ * attends over all as they are held.  32 columns with a value that is not finite become not-a-number.
+ * Caches: [slot][G] parts of pg_cache4_bytes(width, cap) bytes, on 16-byte boundaries, zero at first.  Of 16 positions each: quants of 32 columns after 32
+ * columns, 256 bytes each, then for every pair of positions the bf16 scales of every 32 columns, both positions side by side.
+ *   keys    position 8 n + r, column 16 s + 4 t + 2 i + h of 32: byte [r][t][s][2 h + n], low half for i = 0
+ *   values  position 8 i + 2 t + h, column 16 s + 8 n + r of 32: byte [r][t][s][2 h + i], low half for n = 0
+ * pg_attention: d_q is used by pg_attention4_prompt only; d_part: pg_attention4_part_floats(...); d_tickets: [pg_attention4_tickets(...)], zero before the
+ * first call. */
+PG_API int64_t pg_cache4_bytes(int32_t width, int64_t positions);
+PG_API int64_t pg_attention4_part_floats(pg_ctx *ctx, const pg_attention *p);
+PG_API int64_t pg_attention4_tickets(pg_ctx *ctx);
+/* Appends every row of the batch, and attends for the sequences of up to `few` tokens in this step (chunked layers: few <= 1): short_rows tokens in all,
+ * at most short_len of one sequence.  Longer ones take pg_attention4_prompt behind it. */
+PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t few, int64_t short_rows, int64_t short_len, const float *d_proj,
+                                 int64_t ldp, void *d_kcache, void *d_vcache, void *d_out, int32_t dtype, int64_t ldo);
+/* Sequence `seq` of the batch: len tokens in this step, positions with them, in slot `slot`.  Its cache is unfolded to bf16 in d_work
+ * (pg_attention4_unfold_bytes(...) on a 128-byte boundary), one rounding. */
+PG_API int64_t pg_attention4_unfold_bytes(const pg_attention *p);
+PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t seq, int64_t len, int64_t positions, int64_t slot,
+                                    const void *d_kcache, const void *d_vcache, void *d_work, void *d_out, int32_t dtype, int64_t ldo);
+/* The values of the first `rows` rows of `parts` parts of a cache (values: of values, else of keys), f32 [parts][rows][width up to 32] */
+PG_API int32_t pg_cache4_read(pg_ctx *ctx, const void *d_cache, int32_t values, int32_t width, int64_t cap, int64_t parts, int64_t rows, float *d_out);
+
 /* ---- latent attention ----
  * A position's cache row is [c | rotated key part]: C = kv_rank columns padded to a multiple of 64, and rot_dim columns padded
  * to a multiple of 16, in the step's type: [slot][cap][cp + rp].

@@ -23,6 +23,8 @@ def main(argv=None) -> int:
     g.add_argument("--slots", type=int, default=0, help="sequences decoded together (default: one per prompt, at most 16)")
     g.add_argument("--capacity", type=int, default=0, help="positions per sequence (default: the model's)")
     g.add_argument("--portion", type=int, default=0, help="most prompt tokens of one step")
+    g.add_argument("--weight-bits", type=int, choices=[16, 4], default=16, help="of the layers' matrices (4: bfloat16 steps)")
+    g.add_argument("--cache-bits", type=int, choices=[16, 4], default=16, help="of the attention layers' keys and values (4: bfloat16 steps)")
     t = sub.add_parser("trace", help="replay steps of given token ids and write logits")
     t.add_argument("--model", required=True)
     t.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
@@ -37,7 +39,7 @@ def main(argv=None) -> int:
 
     ids = lambda text: [int(x) for x in text.split(",") if x.strip()]
     prompts = [ids(p) for p in a.prompt]
-    options = {"slots": a.slots or min(16, len(prompts)), "capacity": a.capacity}
+    options = {"slots": a.slots or min(16, len(prompts)), "capacity": a.capacity, "weight_bits": a.weight_bits, "cache_bits": a.cache_bits}
     if a.dtype:
         options["dtype"] = a.dtype
     if a.portion:

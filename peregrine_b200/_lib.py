@@ -208,6 +208,13 @@ LM_SIGNATURES = {
     "pg_delta_run_chunks": (_i32, [_vp, _pd, _pb, _vp, _i64, _vp, _vp, _vp, _i32, _i64]),
     "pg_attention_part_floats": (_i64, [_vp, _pa, _i64]),
     "pg_attention_run": (_i32, [_vp, _pa, _pb, _vp, _i64, _vp, _vp, _vp, _i32, _i64]),
+    "pg_cache4_bytes": (_i64, [_i32, _i64]),
+    "pg_attention4_part_floats": (_i64, [_vp, _pa]),
+    "pg_attention4_tickets": (_i64, [_vp]),
+    "pg_attention4_run": (_i32, [_vp, _pa, _pb, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i64]),
+    "pg_attention4_unfold_bytes": (_i64, [_pa]),
+    "pg_attention4_prompt": (_i32, [_vp, _pa, _pb, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i64]),
+    "pg_cache4_read": (_i32, [_vp, _vp, _i32, _i32, _i64, _i64, _i64, _vp]),
     "pg_latent_part_floats": (_i64, [_vp, _pl, _i32, _i64, _i64]),
     "pg_latent_run": (_i32, [_vp, _pl, _pb, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i32, _i64]),
     "pg_latent_prompt_supports": (_i32, [_pl]),

@@ -67,7 +67,7 @@ class BubotarModel(ResidualModel):
                 out["mixer"] = LatentAttention(d, p, mix, cfg.width, cfg.eps, self.capacity, self.slots, own=source is None)
             elif L["type"] == "attention":
                 out["mixer"] = Attention(d, p, mix, cfg.width, cfg.eps, self.capacity, self.slots, sink=False, norms=False,
-                                         slopes=halving_slopes(int(p["heads"])), chunk=int(p["mask"]["size"]))
+                                         slopes=halving_slopes(int(p["heads"])), chunk=int(p["mask"]["size"]), bits=self.cache_bits)
             else:
                 out["mixer"] = SelectiveScan(d, p, mix, cfg.width)
             out["state"] = out["mixer"].new_state(self.pool) if source is None else self.layers[source]["state"]

@@ -25,31 +25,6 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ float temperature(const AttnShape &s, int pos)
-{
-    if (s.every <= 0.0f) return 1.0f;
-    return 1.0f + s.coef * logf(floorf(__fdiv_rn((float)(pos + 1), s.every)) + 1.0f);
-}
-
-// One warp: dst = rms_norm(src[0 .. D)) * w * mul, or src * mul where w is null; columns D .. dp are zero (D <= 256).
-template <typename TA>
-__device__ __forceinline__ void head_norm(const float *src, const float *__restrict__ w, int D, int dp, float eps, float mul, TA *dst, int lane)
-{
-    float x[8], ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        x[i] = i * 32 + lane < D ? __ldcg(src + i * 32 + lane) : 0.0f;
-        ss += x[i] * x[i];
-    }
-    ss = pg_warp_sum(ss);
-    const float inv = w ? __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)D) + eps)) : 1.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int c = i * 32 + lane;
-        if (c < dp) pg_put(dst + c, c < D ? x[i] * inv * (w ? __ldg(w + c) : 1.0f) * mul : 0.0f);
-    }
-}
-
 // four columns per lane, four heads per warp with their loads in flight together (widths up to 128, all multiples of four)
 __device__ __forceinline__ void put4(float *p, const float4 &v) { *reinterpret_cast<float4 *>(p) = v; }
 __device__ __forceinline__ void put4(bf16 *p, const float4 &v) { *reinterpret_cast<uint2 *>(p) = make_uint2(pg_pack_bf16(v.x, v.y), pg_pack_bf16(v.z, v.w)); }
@@ -102,7 +77,7 @@ __global__ void __launch_bounds__(256)
         return;
     }
     const float *row = proj + (int64_t)m * ldp;
-    const float mul = temperature(s, pos);
+    const float mul = attn_temperature(s, pos);
     const int at = attn_row(s, pos);
     if (wide) {
         prep_heads4(s, row, (int64_t)m * s.H, slot * s.G * s.cap + at, mul, q, kc, vc, warp, lane);
@@ -110,10 +85,10 @@ __global__ void __launch_bounds__(256)
     }
     for (int i = warp; i < s.H + 2 * s.G; i += 8) {
         if (i < s.H) {
-            head_norm(row + i * s.D, s.qn, s.D, s.dp, s.eps, mul, q + ((int64_t)m * s.H + i) * s.dp, lane);
+            attn_head_norm(row + i * s.D, s.qn, s.D, s.dp, s.eps, mul, q + ((int64_t)m * s.H + i) * s.dp, lane);
         } else if (i < s.H + s.G) {
             const int g = i - s.H;
-            head_norm(row + i * s.D, s.kn, s.D, s.dp, s.eps, 1.0f, kc + ((slot * s.G + g) * s.cap + at) * s.dp, lane);
+            attn_head_norm(row + i * s.D, s.kn, s.D, s.dp, s.eps, 1.0f, kc + ((slot * s.G + g) * s.cap + at) * s.dp, lane);
         } else {
             const int g = i - s.H - s.G;
             const float *src = row + (int64_t)(s.H + s.G) * s.D + (int64_t)g * s.V;
@@ -561,7 +536,7 @@ __global__ void __launch_bounds__(AS_WARPS * 32)
     };
     prime();
     const float *row = proj + (int64_t)b * ldp;
-    if (newest && warp == 2) head_norm(row + (int64_t)(s.H + g) * s.D, s.kn, s.D, s.dp, s.eps, 1.0f, k_new, lane);
+    if (newest && warp == 2) attn_head_norm(row + (int64_t)(s.H + g) * s.D, s.kn, s.D, s.dp, s.eps, 1.0f, k_new, lane);
     if (newest && warp == 3) {
         const float *src = row + (int64_t)(s.H + s.G) * s.D + (int64_t)g * s.V;
         for (int c = lane; c < s.vp; c += 32) pg_put(v_new + c, c < s.V ? __ldcg(src + c) : 0.0f);
@@ -569,7 +544,7 @@ __global__ void __launch_bounds__(AS_WARPS * 32)
     for (int h = warp; h < heads; h += AS_WARPS) {
         bf16 *dst = qs + h * (s.dp + 8);
         if (FUSED) {
-            head_norm(row + (int64_t)(h0 + h) * s.D, s.qn, s.D, s.dp, s.eps, temperature(s, pos), dst, lane);
+            attn_head_norm(row + (int64_t)(h0 + h) * s.D, s.qn, s.D, s.dp, s.eps, attn_temperature(s, pos), dst, lane);
         } else {
             for (int i = lane; i < s.dp; i += 32) dst[i] = __float2bfloat16_rn(pg_get(q + ((int64_t)b * s.H + h0 + h) * s.dp + i));
         }
@@ -781,7 +756,9 @@ __global__ void __launch_bounds__(AS_WARPS * 32)
     }
 }
 
-AttnShape shape_of(const pg_attention *p)
+}  // namespace
+
+AttnShape pgk_attention_shape(const pg_attention *p)
 {
     AttnShape s;
     s.H = p->heads, s.G = p->kv_heads, s.rep = p->heads / p->kv_heads, s.D = p->dim, s.V = p->vdim;
@@ -792,6 +769,8 @@ AttnShape shape_of(const pg_attention *p)
     s.qn = p->d_q_norm, s.kn = p->d_k_norm;
     return s;
 }
+
+namespace {
 
 // slices of the context: enough CTAs for about two per SM, none shorter than 128 positions of the longest context
 int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s)
@@ -842,12 +821,19 @@ int32_t pgk_attention_f32(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, c
     return launch_pdl(ctx, attn_f32_kernel<1, 8>, dim3((unsigned)s.H, (unsigned)bt->rows), dim3(AF_T), (size_t)(s.dp + AF_T) * 4, s, *bt, q, kc, vc, out, ldo);
 }
 
+int32_t pgk_attention_prompt(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, const bf16 *q, const bf16 *kc, const bf16 *vc, bf16 *out, int64_t ldo)
+{
+    if (s.dp <= 64 && s.vp <= 64) return run_prompt<4, 8>(ctx, s, bt, q, kc, vc, out, ldo);
+    if (s.dp <= 128 && s.vp <= 128) return run_prompt<8, 16>(ctx, s, bt, q, kc, vc, out, ldo);
+    return run_prompt<16, 32>(ctx, s, bt, q, kc, vc, out, ldo);
+}
+
 extern "C" {
 
 PG_API int64_t pg_attention_part_floats(pg_ctx *ctx, const pg_attention *p, int64_t max_seqs)
 {
     if (!ctx || !p || p->kv_heads <= 0 || max_seqs <= 0) return 0;
-    const AttnShape s = shape_of(p);
+    const AttnShape s = pgk_attention_shape(p);
     const int64_t per = (int64_t)s.G * ((s.rep + 15) / 16);
     int64_t most = 0;
     for (int64_t rows = 1; rows <= max_seqs; rows++) most = std::max(most, rows * per * slices(ctx, rows * per, s));
@@ -866,7 +852,7 @@ PG_API int32_t pg_attention_run(pg_ctx *ctx, const pg_attention *p, const pg_bat
                "attention: a cache of %d rows for %d positions in chunks of %d", p->cap, p->positions, p->chunk);
     PG_REQUIRE(p->chunk == 0 || p->positions <= p->cap || ((int64_t)(p->chunk + batch->max_len - 2) / p->chunk + 1) * p->chunk <= p->cap,
                "attention: a step of %d tokens has more chunks of %d than the cache of %d rows", batch->max_len, p->chunk, p->cap);
-    const AttnShape s = shape_of(p);
+    const AttnShape s = pgk_attention_shape(p);
     PG_REQUIRE(ldp >= (int64_t)(s.H + s.G) * s.D + (int64_t)s.G * s.V && ldo >= (int64_t)s.H * s.V, "attention: rows too short");
     PG_REQUIRE(s.G <= 65535 && batch->rows >= 0 && batch->seqs <= 65535, "attention: too many heads or sequences");
     if (batch->rows == 0) return PG_OK;
@@ -885,11 +871,11 @@ PG_API int32_t pg_attention_run(pg_ctx *ctx, const pg_attention *p, const pg_bat
         if (rc != PG_OK) return rc;
     }
     if (!step && pgk_attention_prompt_tc_supports(s, batch, p->slots, ldo, out)) return pgk_attention_prompt_tc(ctx, s, batch, p->slots, q, kc, vc, out, ldo);
+    if (!step) return pgk_attention_prompt(ctx, s, batch, q, kc, vc, out, ldo);
 #define PG_AT(DC, VC)                                                                                                        \
     do {                                                                                                                     \
         if (fused) return run_step<DC, VC, true>(ctx, s, batch, d_proj, ldp, q, kc, vc, p->d_part, p->d_tickets, out, ldo);  \
         if (step) return run_step<DC, VC, false>(ctx, s, batch, d_proj, ldp, q, kc, vc, p->d_part, p->d_tickets, out, ldo);  \
-        return run_prompt<DC, VC>(ctx, s, batch, q, kc, vc, out, ldo);                                                       \
     } while (0)
     if (s.dp <= 64 && s.vp <= 64) PG_AT(4, 8);
     if (s.dp <= 128 && s.vp <= 128) PG_AT(8, 16);

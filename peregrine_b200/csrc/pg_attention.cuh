@@ -1,6 +1,8 @@
 // What the two attention files share.
 #pragma once
 
+#include <math.h>
+
 #include "pg_lm.cuh"
 
 struct AttnShape {
@@ -17,9 +19,36 @@ struct AttnShape {
 // A chunked layer keeps whole chunks only, position p in row p mod cap: the rows of a chunk lie next to each other.
 __device__ __forceinline__ int attn_low(const AttnShape &s, int pos) { return s.chunk ? pos - pos % s.chunk : 0; }
 __device__ __forceinline__ int attn_row(const AttnShape &s, int pos) { return s.chunk ? pos % s.cap : pos; }
+__device__ __forceinline__ float attn_temperature(const AttnShape &s, int pos)
+{
+    if (s.every <= 0.0f) return 1.0f;
+    return 1.0f + s.coef * logf(floorf(__fdiv_rn((float)(pos + 1), s.every)) + 1.0f);
+}
+
+// One warp: dst = rms_norm(src[0 .. D)) * w * mul, or src * mul where w is null; columns D .. dp are zero (D <= 256).
+template <typename TA>
+__device__ __forceinline__ void attn_head_norm(const float *src, const float *__restrict__ w, int D, int dp, float eps, float mul, TA *dst, int lane)
+{
+    float x[8], ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        x[i] = i * 32 + lane < D ? __ldcg(src + i * 32 + lane) : 0.0f;
+        ss += x[i] * x[i];
+    }
+    ss = pg_warp_sum(ss);
+    const float inv = w ? __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)D) + eps)) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int c = i * 32 + lane;
+        if (c < dp) pg_put(dst + c, c < D ? x[i] * inv * (w ? __ldg(w + c) : 1.0f) * mul : 0.0f);
+    }
+}
 #endif
 
-// pg_attention.cu: out [rows][H V] f32; every head's query is a row of s.dp floats
+// pg_attention.cu: the shape of a description; keys and values of prompts on mma.sync (any shape)
+AttnShape pgk_attention_shape(const pg_attention *p);
+int32_t pgk_attention_prompt(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, const bf16 *q, const bf16 *kc, const bf16 *vc, bf16 *out, int64_t ldo);
+// out [rows][H V] f32; every head's query is a row of s.dp floats
 int32_t pgk_attention_f32(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, const float *q, const float *kc, const float *vc, float *out, int64_t ldo);
 
 // pg_attention_tc.cu

@@ -1,0 +1,712 @@
+// Causal attention over a cache of keys and values in 4 bits (csrc/pg_four.cuh): a scale per 32 columns of a position, whose values are those of
+// its positions as they are held, a step's own among them.  What a layer may have besides is that of csrc/pg_attention.cu.
+//
+// A head's part of a cache comes in tiles of 16 positions, so that a tile is one bulk copy: the quants of 32 columns after those of 32 columns, 256
+// bytes each, then for the eight pairs of positions the scales of every 32 columns, both positions side by side.
+//   keys    position 8 n + r, column 16 s + 4 t + 2 i + h of its 32 -> byte [r][t][s][2 h + n], low half for i = 0
+//   values  position 8 i + 2 t + h, column 16 s + 8 n + r of its 32 -> byte [r][t][s][2 h + i], low half for n = 0
+// Those are operands of mma.sync m16n8k16 once the quants are numbers: keys the B side of S = Q K^T (16 rows of queries), values the A side of
+// O^T = V^T P^T, so that a lane's probabilities are the B operand as they come.  A byte belongs to one position: appending is byte stores.
+//
+//   few tokens of a sequence    attn4_few_kernel: streams the cache once, a block of 16 (token, head of the group) rows per CTA, the context in slices.
+//                               Keys as f16 integers (exact) times the query as f16 over a power of two, sums of 32 columns scaled in f32; values as
+//                               bf16 integers (exact) times bf16(probability * scale).  One token per sequence (FUSED): the CTA with the newest
+//                               position quantises and appends it.  The last CTA of a (sequence, rows) to finish merges the slices.
+//   longer portions             attn4_append_kernel, then per sequence attn4_unfold_kernel (the values as bf16, one rounding) and the kernels that
+//                               prompts over a bf16 cache run through.
+#include <algorithm>
+
+#include "pg_async.cuh"
+#include "pg_attention.cuh"
+#include "pg_four.cuh"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// what the 4-bit form has beyond AttnShape: groups of 32 columns, bytes of a tile
+struct Four {
+    int gk, gv;                // groups of a key and of a value
+    int kb, vb;                // bytes of a tile
+    int64_t kh, vh;            // bytes of a head's part of a slot
+};
+
+// ---- quantising and placing a position (one warp) -----------------------------------------------------------------------
+// x[i]: columns 32 i + lane; quants (a byte each) and scales to shared memory
+__device__ __forceinline__ void quantise_row(const float (&x)[8], int groups, uint8_t *quants, bf16 *scales, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (i >= groups) break;
+        const uint32_t mag = __float_as_uint(fabsf(x[i])), most = __reduce_max_sync(0xffffffffu, mag);   // (magnitudes order as integers; not-a-numbers are the largest)
+        const int first = __ffs(__ballot_sync(0xffffffffu, mag == most)) - 1;
+        const float scale = four_scale(__shfl_sync(0xffffffffu, x[i], first));
+        quants[32 * i + lane] = (uint8_t)four_quant(x[i], scale);
+        if (lane == 0) scales[i] = __float2bfloat16_rn(scale);
+    }
+    __syncwarp();
+}
+// into row `row` (0 .. 15) of a tile, in global or shared memory
+__device__ __forceinline__ void put_scales(unsigned char *tile, const bf16 *scales, int row, int groups, int lane)
+{
+    if (lane < groups) *reinterpret_cast<bf16 *>(tile + groups * 256 + (((row >> 1) * groups + lane) * 2 + (row & 1)) * 2) = scales[lane];
+}
+__device__ __forceinline__ void put_key(unsigned char *tile, const uint8_t *q, const bf16 *scales, int row, int groups, int lane)
+{
+    const int n = row >> 3, r = row & 7;
+    for (int i = lane; i < groups * 8; i += 32) {
+        const int g = i >> 3, t = i >> 1 & 3, s = i & 1, c = 32 * g + 16 * s + 4 * t;
+        unsigned char *at = tile + g * 256 + ((r * 4 + t) * 2 + s) * 4;
+        at[n] = q[c] | q[c + 2] << 4;
+        at[2 + n] = q[c + 1] | q[c + 3] << 4;
+    }
+    put_scales(tile, scales, row, groups, lane);
+}
+__device__ __forceinline__ void put_value(unsigned char *tile, const uint8_t *q, const bf16 *scales, int row, int groups, int lane)
+{
+    const int i8 = row >> 3, t = (row & 7) >> 1, h = row & 1;
+    for (int i = lane; i < groups * 16; i += 32) {
+        const int g = i >> 4, r = i >> 1 & 7, s = i & 1, c = 32 * g + 16 * s + r;
+        tile[g * 256 + ((r * 4 + t) * 2 + s) * 4 + 2 * h + i8] = q[c] | q[c + 8] << 4;
+    }
+    put_scales(tile, scales, row, groups, lane);
+}
+// a head's row of the projection: x[i] = column 32 i + lane, normalised where w is there; zero behind `width`
+__device__ __forceinline__ void load_row(const float *src, const float *__restrict__ w, int width, float eps, float (&x)[8], int lane)
+{
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        x[i] = 32 * i + lane < width ? __ldcg(src + 32 * i + lane) : 0.0f;
+        ss += x[i] * x[i];
+    }
+    if (!w) return;
+    const float inv = __fdiv_rn(1.0f, sqrtf(__fdiv_rn(pg_warp_sum(ss), (float)width) + eps));
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (32 * i + lane < width) x[i] *= inv * __ldg(w + 32 * i + lane);
+}
+
+// ---- append: a CTA per token, a warp per key or value head; with q: the queries too, as the prompt kernels read them ----------
+constexpr int AP_WARPS = 8;
+__global__ void __launch_bounds__(AP_WARPS * 32)
+    attn4_append_kernel(const AttnShape s, const Four f, const pg_batch bt, const float *__restrict__ proj, int64_t ldp, bf16 *__restrict__ q, unsigned char *kc,
+                        unsigned char *vc, int32_t *status)
+{
+    __shared__ uint8_t quants[AP_WARPS][256];
+    __shared__ bf16 scales[AP_WARPS][8];
+    pg_pdl_begin();
+    const int m = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pos = __ldcg(bt.d_pos + m);
+    const int64_t slot = __ldcg(bt.d_seq_slot + __ldcg(bt.d_row_seq + m));
+    if ((unsigned)pos >= (unsigned)s.limit) {   // outside the cache: record it, touch nothing
+        if (threadIdx.x == 0) atomicExch(status, (int32_t)PG_ERR_INVALID);
+        return;
+    }
+    const float *row = proj + (int64_t)m * ldp;
+    const int at = attn_row(s, pos);
+    for (int i = warp; i < 2 * s.G; i += AP_WARPS) {
+        const bool key = i < s.G;
+        const int g = key ? i : i - s.G;
+        float x[8];
+        load_row(key ? row + (int64_t)(s.H + g) * s.D : row + (int64_t)(s.H + s.G) * s.D + (int64_t)g * s.V, key ? s.kn : nullptr, key ? s.D : s.V, s.eps, x, lane);
+        quantise_row(x, key ? f.gk : f.gv, quants[warp], scales[warp], lane);
+        if (key)
+            put_key(kc + (slot * s.G + g) * f.kh + (int64_t)(at >> 4) * f.kb, quants[warp], scales[warp], at & 15, f.gk, lane);
+        else
+            put_value(vc + (slot * s.G + g) * f.vh + (int64_t)(at >> 4) * f.vb, quants[warp], scales[warp], at & 15, f.gv, lane);
+        __syncwarp();
+    }
+    if (q) {
+        const float mul = attn_temperature(s, pos);
+        for (int h = warp; h < s.H; h += AP_WARPS) attn_head_norm(row + (int64_t)h * s.D, s.qn, s.D, s.dp, s.eps, mul, q + ((int64_t)m * s.H + h) * s.dp, lane);
+    }
+}
+
+// ---- unfold: grid (tiles of 16 positions, heads); values of a slot's rows [0, rows) as TA, zeros up to row `padded` -----------------
+template <typename TA, bool VALUES>
+__global__ void __launch_bounds__(128) attn4_unfold_kernel(const unsigned char *__restrict__ cache, int groups, int tile_bytes, int64_t head_bytes, int rows, int padded,
+                                                           int width, int64_t head_stride, TA *__restrict__ out)
+{
+    __shared__ __align__(16) unsigned char tile[8 * 288];
+    pg_pdl_begin();
+    const uint4 *src = reinterpret_cast<const uint4 *>(cache + (int64_t)blockIdx.y * head_bytes + (int64_t)blockIdx.x * tile_bytes);
+    for (int i = threadIdx.x; i < tile_bytes / 16; i += 128) reinterpret_cast<uint4 *>(tile)[i] = __ldcg(src + i);
+    __syncthreads();
+    const bf16 *scales = reinterpret_cast<const bf16 *>(tile + groups * 256);
+    const int fours = width / 4, first = (int)blockIdx.x * 16, left = min(16, padded - first);
+    TA *dst = out + (int64_t)blockIdx.y * head_stride + (int64_t)blockIdx.x * 16 * width;
+    for (int i = threadIdx.x; i < left * fours; i += 128) {
+        const int p = i / fours, c = (i - p * fours) * 4, g = c >> 5, s = c >> 4 & 1;
+        const float scale = __bfloat162float(scales[((p >> 1) * groups + g) * 2 + (p & 1)]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            int q;
+            if (VALUES) {
+                const int col = (c + e) & 15, r = col & 7, n = col >> 3, i8 = p >> 3, t = (p & 7) >> 1, h = p & 1;
+                q = tile[g * 256 + ((r * 4 + t) * 2 + s) * 4 + 2 * h + i8] >> (4 * n) & 15;
+            } else {
+                const int t = (c & 15) >> 2, n = p >> 3, r = p & 7;
+                q = tile[g * 256 + ((r * 4 + t) * 2 + s) * 4 + 2 * (e & 1) + n] >> (4 * (e >> 1)) & 15;
+            }
+            pg_put(dst + (int64_t)p * width + c + e, first + p < rows ? scale * (float)(q - 8) : 0.0f);
+        }
+    }
+}
+
+// ---- few tokens: grid (slices, G * blocks of 16 rows, seqs) --------------------------------------------------------------------
+constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // most fills in flight of a warp; tiles of a fill
+
+// part [(seq, block)][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row
+template <int GK, int GV, bool HI, bool FUSED>
+__global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
+    attn4_few_kernel(const AttnShape s, const Four f, const pg_batch bt, int few, int stages, const float *__restrict__ proj, int64_t ldp, unsigned char *kc, unsigned char *vc,
+                     float *part, int32_t *tickets, bf16 *__restrict__ out, int64_t ldo, int32_t *status, unsigned long long limit_ns)
+{
+    constexpr int NT = HI ? 2 : 1;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t bars[A4_WARPS * A4_STAGES];
+    __shared__ float weight[16][A4_SLICES];
+    __shared__ float denom[16], back[16];
+    __shared__ int last_in;
+    __shared__ volatile int abort_flag;
+    __shared__ uint8_t new_q[2][256];
+    __shared__ bf16 new_s[2][8];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int split = blockIdx.x, S = gridDim.x, g = blockIdx.y % s.G, block = blockIdx.y / s.G, seq = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+    const int gk = f.gk, gv = f.gv, stage = A4_FILL * (f.kb + f.vb), vs = gv * 32;
+    const uint32_t ring = pg_smem(smem) + (uint32_t)(warp * stages) * stage, bar = pg_smem(bars) + (uint32_t)warp * A4_STAGES * 8;
+    const int qs = gk * 32 + 8;                                       // f16 elements between the rows of queries
+    __half *qrow = reinterpret_cast<__half *>(smem + A4_WARPS * stages * stage);
+    float *mg = reinterpret_cast<float *>(smem);                      // the merge reuses the rings
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < A4_WARPS * A4_STAGES; i++) pg_mbar_init(pg_smem(bars) + 8 * i, 1);
+        abort_flag = 0;
+        pg_mbar_fence();
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int row0 = __ldcg(bt.d_seq_row0 + seq), T = __ldcg(bt.d_seq_row0 + seq + 1) - row0;
+    const int count = min(16, T * s.rep - block * 16);               // rows: (token, head) = (block * 16 + c) / rep, % rep
+    if (T > few || count <= 0) return;
+    const int pos0 = __ldcg(bt.d_pos + row0), last = pos0 + T - 1;
+    const int64_t slot = __ldcg(bt.d_seq_slot + seq);
+    if (pos0 < 0 || last >= s.limit) {                                // outside the cache: record it, touch nothing (all CTAs of the sequence leave)
+        if (threadIdx.x == 0) atomicExch(status, (int32_t)PG_ERR_INVALID);
+        return;
+    }
+    // rows of the cache: x0 .. x1 - 1 hold the positions low .. of this block (in a chunked layer T is 1, and a chunk's rows lie together)
+    const int low = attn_low(s, pos0), x0 = attn_row(s, low), x1 = x0 + (pos0 + (block * 16 + count - 1) / s.rep) + 1 - low;
+    const int a0 = x0 & ~31;                                          // first row of the first fill
+    const int chunk = ((x1 - a0 + S - 1) / S + 255) & ~255;           // of a slice: a fill for every warp
+    const int t0 = a0 + split * chunk, t1 = min(x1, t0 + chunk), used = (x1 - a0 + chunk - 1) / chunk;
+    if (t0 >= t1) return;
+    const bool newest = FUSED && t1 == x1;
+    unsigned char *kb = kc + (slot * s.G + g) * f.kh, *vb = vc + (slot * s.G + g) * f.vh;
+
+    const int nfills = (t1 - t0 + 31) / 32, mine = nfills > warp ? (nfills - warp + A4_WARPS - 1) / A4_WARPS : 0;
+    const int tiles = (s.cap + 15) / 16;                              // of a head's part
+    auto fetch = [&](int i, int to) {
+        if (lane == 0) {
+            const uint32_t at = ring + (uint32_t)(to) * stage, on = bar + (uint32_t)(to) * 8;
+            const int tile = (t0 >> 4) + A4_FILL * (warp + A4_WARPS * i), n = min(A4_FILL, tiles - tile);
+            pg_mbar_expect(on, (uint32_t)(n * (f.kb + f.vb)));
+            pg_bulk_load(at, kb + (int64_t)tile * f.kb, (uint32_t)(n * f.kb), on);
+            pg_bulk_load(at + A4_FILL * f.kb, vb + (int64_t)tile * f.vb, (uint32_t)(n * f.vb), on);
+        }
+    };
+    for (int i = 0; i < stages && i < mine; i++) fetch(i, i);
+
+    // the rows' queries as f16 over a power of two, and what their scores are multiplied by
+    const float sl = s.scale * LOG2E;
+    for (int c = warp; c < 16; c += A4_WARPS) {
+        if (c < count) {
+            const int idx = block * 16 + c, token = idx / s.rep, h = g * s.rep + idx % s.rep;
+            float x[8], top = 0.0f;
+            load_row(proj + (int64_t)(row0 + token) * ldp + (int64_t)h * s.D, s.qn, s.D, s.eps, x, lane);
+            const float mul = attn_temperature(s, pos0 + token);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[i] *= mul;
+                top = fmaxf(top, fabsf(x[i]));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float down, up;
+            four_range(top, down, up);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < gk) qrow[c * qs + 32 * i + lane] = __float2half_rn(x[i] * down);
+            if (lane == 0) back[c] = up * sl;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < gk) qrow[c * qs + 32 * i + lane] = __float2half_rn(0.0f);
+            if (lane == 0) back[c] = 0.0f;
+        }
+    }
+    if (newest && warp >= A4_WARPS - 2) {
+        // the newest position: warp 6 its key, warp 7 its value
+        const bool key = warp == A4_WARPS - 2;
+        const float *row = proj + (int64_t)row0 * ldp;
+        float x[8];
+        load_row(key ? row + (int64_t)(s.H + g) * s.D : row + (int64_t)(s.H + s.G) * s.D + (int64_t)g * s.V, key ? s.kn : nullptr, key ? s.D : s.V, s.eps, x, lane);
+        quantise_row(x, key ? gk : gv, new_q[key ? 0 : 1], new_s[key ? 0 : 1], lane);
+    }
+    __syncthreads();
+    if (newest && block == 0 && warp >= A4_WARPS - 2) {
+        // appended for later steps; this step takes it from shared memory (below)
+        const int at = x1 - 1;
+        if (warp == A4_WARPS - 2)
+            put_key(kb + (int64_t)(at >> 4) * f.kb, new_q[0], new_s[0], at & 15, gk, lane);
+        else
+            put_value(vb + (int64_t)(at >> 4) * f.vb, new_q[1], new_s[1], at & 15, gv, lane);
+    }
+    uint32_t qf[GK][2][HI ? 4 : 2];
+#pragma unroll
+    for (int i = 0; i < GK; i++) {
+        if (i >= gk) break;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            // columns 4 t + {0, 1} and 4 t + {2, 3} of 16; the second pair's keys come 16 times too large
+            const uint2 lo = *reinterpret_cast<const uint2 *>(qrow + r * qs + 32 * i + 16 * e + 4 * t);
+            const __half2 less = __float2half2_rn(0.0625f);
+            __half2 b = __hmul2(*reinterpret_cast<const __half2 *>(&lo.y), less);
+            qf[i][e][0] = lo.x;
+            qf[i][e][1] = *reinterpret_cast<uint32_t *>(&b);
+            if constexpr (HI) {
+                const uint2 hi = *reinterpret_cast<const uint2 *>(qrow + (r + 8) * qs + 32 * i + 16 * e + 4 * t);
+                b = __hmul2(*reinterpret_cast<const __half2 *>(&hi.y), less);
+                qf[i][e][2] = hi.x;
+                qf[i][e][3] = *reinterpret_cast<uint32_t *>(&b);
+            }
+        }
+    }
+    float o[GV][2][NT][4];
+#pragma unroll
+    for (int i = 0; i < GV; i++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[i][e][n][j] = 0.0f;
+    // of the lane's rows r (and r + 8): factor of the scores, last row of the cache seen, slope
+    float fac[NT], m[NT], l[NT], bias[NT];
+    int seen[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int c = r + 8 * n, idx = block * 16 + min(c, count - 1);
+        fac[n] = back[c];
+        seen[n] = x0 + pos0 + idx / s.rep - low;
+        bias[n] = s.slopes ? __ldg(s.slopes + g * s.rep + idx % s.rep) * LOG2E : 0.0f;
+        m[n] = -1e30f, l[n] = 0.0f;                       // (finite: exp2(-inf - m) is 0 where a row sees nothing of a slice)
+    }
+    const int sees_all = x0 + pos0 + block * 16 / s.rep - low;        // of the block's first row: every row sees that far
+    bool ok = true;
+    int at_stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < mine; i++) {
+        ok = pg_mbar_wait_warp(bar + (uint32_t)at_stage * 8, phase, &abort_flag, status, limit_ns);
+        if (!ok) break;
+        const int j0 = t0 + 32 * (warp + A4_WARPS * i);
+        unsigned char *at = smem + (size_t)(warp * stages + at_stage) * stage;
+        if (newest && j0 + 32 >= x1) {
+            // the copies brought what the cache held at the newest position: put the new one in its place
+            const int row = x1 - 1 - j0;
+            put_key(at + (row >> 4) * f.kb, new_q[0], new_s[0], row & 15, gk, lane);
+            put_value(at + A4_FILL * f.kb + (row >> 4) * f.vb, new_q[1], new_s[1], row & 15, gv, lane);
+            __syncwarp();
+        }
+        const bool edge = j0 < x0 || j0 + 31 > sees_all || j0 + 31 >= t1;   // some row does not see all of these
+#pragma unroll
+        for (int h = 0; h < A4_FILL; h++) {
+            const int jt = j0 + 16 * h;
+            if (jt >= t1) break;                                      // (uniform)
+            const uint32_t kt = pg_smem(at) + (uint32_t)(h * f.kb), vt = pg_smem(at) + (uint32_t)(A4_FILL * f.kb + h * f.vb);
+            // scores of keys 8 n + 2 t and 8 n + 2 t + 1 with rows r and r + 8
+            float sc[2][4] = {};
+#pragma unroll
+            for (int x = 0; x < GK; x++) {
+                if (x >= gk) break;
+                float d[2][4] = {};
+                uint32_t w[2];
+                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(kt + x * 256 + lane * 8));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t w8 = w[e] >> 8;
+                    four_mma_f16(d[0], qf[x][e][0], HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, qf[x][e][1], HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u, four_f16_lo(w[e]), four_f16_hi(w[e]));
+                    four_mma_f16(d[1], qf[x][e][0], HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, qf[x][e][1], HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u, four_f16_lo(w8), four_f16_hi(w8));
+                }
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    uint32_t two;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(kt + (uint32_t)(gk * 256 + ((4 * n + t) * gk + x) * 4)));
+                    const float s0 = pg_bf16_lo(two), s1 = pg_bf16_hi(two);
+                    sc[n][0] = fmaf(s0, d[n][0], sc[n][0]), sc[n][1] = fmaf(s1, d[n][1], sc[n][1]);
+                    if (HI) sc[n][2] = fmaf(s0, d[n][2], sc[n][2]), sc[n][3] = fmaf(s1, d[n][3], sc[n][3]);
+                }
+            }
+            // to units of log 2, bias, mask
+            float top[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) top[n] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int x = jt + 8 * n + 2 * t + j;
+#pragma unroll
+                    for (int u = 0; u < NT; u++) {
+                        float v = fmaf(bias[u], (float)(x - seen[u]), sc[n][2 * u + j] * fac[u]);
+                        if (edge && (x < x0 || x >= t1 || x > seen[u])) v = -INFINITY;
+                        sc[n][2 * u + j] = v;
+                        top[u] = fmaxf(top[u], v);
+                    }
+                }
+            float corr[NT];
+#pragma unroll
+            for (int u = 0; u < NT; u++) {
+                top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+                top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+                const float next = fmaxf(m[u], top[u]);
+                corr[u] = pg_ex2(m[u] - next);
+                m[u] = next;
+                float ps = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        sc[n][2 * u + j] = pg_ex2(sc[n][2 * u + j] - next);
+                        ps += sc[n][2 * u + j];
+                    }
+                l[u] = fmaf(l[u], corr[u], ps);
+            }
+            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[NT - 1] != 1.0f)) {
+                // sums lie by row as columns: 2 t and 2 t + 1 of every eight
+#pragma unroll
+                for (int u = 0; u < NT; u++) {
+                    const float c0 = __shfl_sync(0xffffffffu, corr[u], 8 * t), c1 = __shfl_sync(0xffffffffu, corr[u], 8 * t + 4);
+#pragma unroll
+                    for (int x = 0; x < GV; x++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) o[x][e][u][0] *= c0, o[x][e][u][1] *= c1, o[x][e][u][2] *= c0, o[x][e][u][3] *= c1;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < GV; x++) {
+                if (x >= gv) break;
+                // probabilities times the scales of keys 2 t, 2 t + 1 and 8 + 2 t, 8 + 2 t + 1
+                uint32_t b[NT][2];
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    uint32_t two;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vt + (uint32_t)(gv * 256 + ((4 * n + t) * gv + x) * 4)));
+                    const float s0 = pg_bf16_lo(two), s1 = pg_bf16_hi(two);
+#pragma unroll
+                    for (int u = 0; u < NT; u++) {
+                        float p0 = sc[n][2 * u] * s0, p1 = sc[n][2 * u + 1] * s1;
+                        // (what a row does not see may hold anything)
+                        if (edge) p0 = sc[n][2 * u] == 0.0f ? 0.0f : p0, p1 = sc[n][2 * u + 1] == 0.0f ? 0.0f : p1;
+                        b[u][n] = pg_pack_bf16(p0, p1);
+                    }
+                }
+                uint32_t w[2];
+                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(vt + x * 256 + lane * 8));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t a0 = four_bf16_lo(w[e]), a1 = four_bf16_lo(w[e] >> 4), a2 = four_bf16_lo(w[e] >> 8), a3 = four_bf16_lo(w[e] >> 12);
+#pragma unroll
+                    for (int u = 0; u < NT; u++) pg_mma_bf16(o[x][e][u], a0, a1, a2, a3, b[u][0], b[u][1]);
+                }
+            }
+        }
+        __syncwarp();                                     // every lane is done with the stage before it is filled again
+        if (i + stages < mine) fetch(i + stages, at_stage);
+        if (++at_stage == stages) at_stage = 0, phase ^= 1;
+    }
+    if (!ok) {
+        // copies that are still in flight get a bounded time to land before their shared memory is used again
+        const unsigned long long w0 = pg_globaltimer_ns();
+        while (pg_globaltimer_ns() - w0 < 2000000ull) {
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+    }
+    __syncthreads();                                      // the rings are free
+    // warps meet in shared memory: [warp][16][vs + 4]
+    const int ms = vs + 4;
+    float *w0 = mg + (size_t)warp * 16 * ms;
+#pragma unroll
+    for (int x = 0; x < GV; x++) {
+        if (x >= gv) break;
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int u = 0; u < NT; u++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) w0[(8 * u + 2 * t + (j & 1)) * ms + 32 * x + 16 * e + r + 8 * (j >> 1)] = o[x][e][u][j];
+    }
+    if (t == 0) {
+#pragma unroll
+        for (int u = 0; u < NT; u++) w0[(r + 8 * u) * ms + vs] = m[u], w0[(r + 8 * u) * ms + vs + 1] = l[u];
+    }
+    __syncthreads();
+    const int64_t unit = (int64_t)seq * gridDim.y + blockIdx.y;
+    float *mine_part = part + (unit * S + split) * 16 * ms;
+    const int vq = vs / 4;
+    auto put = [&](int c, int col, const float4 &a, float by) {
+        const int idx = block * 16 + c;
+        bf16 *dst = out + (int64_t)(row0 + idx / s.rep) * ldo + (int64_t)(g * s.rep + idx % s.rep) * s.V + col;
+        const float y[4] = {a.x * by, a.y * by, a.z * by, a.w * by};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (col + i < s.V) pg_put(dst + i, y[i]);
+    };
+    for (int x = threadIdx.x; x < count * vq; x += A4_WARPS * 32) {
+        const int c = x / vq, col = (x - c * vq) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; w++) top = fmaxf(top, mg[((size_t)w * 16 + c) * ms + vs]);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; w++) {
+            const float *from = mg + ((size_t)w * 16 + c) * ms;
+            const float by = pg_ex2(from[vs] - top);      // 0 for a warp that saw nothing
+            const float4 v = *reinterpret_cast<const float4 *>(from + col);
+            a.x = fmaf(by, v.x, a.x), a.y = fmaf(by, v.y, a.y), a.z = fmaf(by, v.z, a.z), a.w = fmaf(by, v.w, a.w);
+            sum = fmaf(by, from[vs + 1], sum);
+        }
+        if (used == 1) {
+            float by = 1.0f;
+            if (s.sink) {
+                const float mm = fmaxf(top, 0.0f);
+                by = pg_ex2(top - mm);
+                sum = sum * by + pg_ex2(-mm);
+            }
+            put(c, col, a, __fdiv_rn(by, sum));
+        } else {
+            *reinterpret_cast<float4 *>(mine_part + (size_t)c * ms + col) = a;
+            if (col == 0) *reinterpret_cast<float2 *>(mine_part + (size_t)c * ms + vs) = make_float2(top, sum);
+        }
+    }
+    if (used == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last_in = atomicAdd(tickets + unit, 1) == used - 1;
+    }
+    __syncthreads();
+    if (!last_in) return;
+    __threadfence();
+    if (threadIdx.x == 0) tickets[unit] = 0;
+    // a warp per row: the slices' weights; then all columns with their loads in flight together
+    const float *parts = part + unit * S * 16 * ms;
+    for (int c = warp; c < count; c += A4_WARPS) {
+        float2 ml[A4_SLICES / 32];
+        float top = s.sink ? 0.0f : -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < A4_SLICES / 32; i++) {
+            const int k = i * 32 + lane;
+            ml[i] = k < used ? __ldcg(reinterpret_cast<const float2 *>(parts + ((size_t)k * 16 + c) * ms + vs)) : make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, ml[i].x);
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+#pragma unroll
+        for (int i = 0; i < A4_SLICES / 32; i++) {
+            const float by = pg_ex2(ml[i].x - top);
+            weight[c][i * 32 + lane] = by;
+            sum = fmaf(by, ml[i].y, sum);
+        }
+        sum = pg_warp_sum(sum) + (s.sink ? pg_ex2(-top) : 0.0f);
+        if (lane == 0) denom[c] = __fdiv_rn(1.0f, sum);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < count * vq; x += A4_WARPS * 32) {
+        const int c = x / vq, col = (x - c * vq) * 4;
+        const float *from = parts + (size_t)c * ms + col;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < used; k0 += 8) {            // eight loads in flight; behind the last slice its weight is 0
+            float4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)min(k0 + k, used - 1) * 16 * ms));
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float by = k0 + k < used ? weight[c][k0 + k] : 0.0f;
+                a.x = fmaf(by, v[k].x, a.x), a.y = fmaf(by, v[k].y, a.y), a.z = fmaf(by, v[k].z, a.z), a.w = fmaf(by, v[k].w, a.w);
+            }
+        }
+        put(c, col, a, denom[c]);
+    }
+}
+
+Four four_of(const AttnShape &s)
+{
+    Four f;
+    f.gk = (s.D + 31) / 32, f.gv = (s.V + 31) / 32;
+    f.kb = (int)pg_cache4_tile_bytes(f.gk * 32), f.vb = (int)pg_cache4_tile_bytes(f.gv * 32);
+    const int64_t tiles = (s.cap + 15) / 16;
+    f.kh = tiles * f.kb, f.vh = tiles * f.vb;
+    return f;
+}
+
+// slices of the context: about two CTAs per SM, none shorter than 256 positions
+int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s)
+{
+    const int64_t cap = s.chunk && s.chunk < s.cap ? s.chunk : s.cap;
+    const int64_t S = std::min<int64_t>(2 * (int64_t)ctx->sm_count / std::max<int64_t>(1, units), cap / 256);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(S, A4_SLICES));
+}
+
+template <int GK, int GV, bool HI, bool FUSED>
+int32_t run_few(pg_ctx *ctx, const AttnShape &s, const Four &f, const pg_batch *bt, int few, int blocks, const float *proj, int64_t ldp, unsigned char *kc,
+                unsigned char *vc, float *part, int32_t *tickets, bf16 *out, int64_t ldo)
+{
+    auto kern = attn4_few_kernel<GK, GV, HI, FUSED>;
+    // (two CTAs to an SM where the widths allow)
+    const int fill = A4_WARPS * A4_FILL * (f.kb + f.vb), stages = 3 * fill <= 100 * 1024 ? 3 : 2, rings = stages * fill;
+    const int smem = std::max(rings + 16 * (f.gk * 32 + 8) * 2, A4_WARPS * 16 * (f.gv * 32 + 4) * 4);
+    static std::atomic<uint64_t> set{0};
+    PG_CUDA(pg_max_smem_once(kern, 220 * 1024, ctx->device, set));   // (widths of 256: 157 KB)
+    const int S = slices(ctx, (int64_t)bt->seqs * s.G * blocks, s);
+    return launch_pdl(ctx, kern, dim3((unsigned)S, (unsigned)(s.G * blocks), (unsigned)bt->seqs), dim3(A4_WARPS * 32), (size_t)smem, s, f, *bt, few, stages, proj, ldp, kc,
+                      vc, part, tickets, out, ldo, ctx->d_status, ctx->wait_limit_ns);
+}
+
+int32_t check(const pg_attention *p, const pg_batch *batch, const void *kc, const void *vc, const void *out, int32_t dtype, int64_t ldo)
+{
+    PG_REQUIRE(p && batch && kc && vc && out && p->d_q && p->d_part && p->d_tickets, "attention4: null pointer");
+    PG_REQUIRE(dtype == PG_BF16, "attention4: steps are bf16");
+    PG_REQUIRE(p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0 && p->dim > 0 && p->dim <= 256 && p->vdim > 0 && p->vdim <= 256 && p->cap > 0 && p->slots > 0,
+               "attention4: bad shape (heads %d / %d, dim %d and vdim %d at most 256)", p->heads, p->kv_heads, p->dim, p->vdim);
+    PG_REQUIRE(p->chunk >= 0 && (p->chunk == 0 ? p->positions <= p->cap : p->cap % p->chunk == 0), "attention4: a cache of %d rows for %d positions in chunks of %d",
+               p->cap, p->positions, p->chunk);
+    PG_REQUIRE(p->chunk == 0 || p->positions <= p->cap || ((int64_t)(p->chunk + batch->max_len - 2) / p->chunk + 1) * p->chunk <= p->cap,
+               "attention4: a step of %d tokens has more chunks of %d than the cache of %d rows", batch->max_len, p->chunk, p->cap);
+    PG_REQUIRE(((uintptr_t)kc & 15) == 0 && ((uintptr_t)vc & 15) == 0, "attention4: caches start on 16-byte boundaries");
+    PG_REQUIRE(ldo >= (int64_t)p->heads * p->vdim, "attention4: rows too short");
+    PG_REQUIRE(p->kv_heads <= 65535 && batch->rows >= 0 && batch->seqs >= 0 && batch->seqs <= 65535, "attention4: too many heads or sequences");
+    return PG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+PG_API int64_t pg_cache4_bytes(int32_t width, int64_t positions)
+{
+    return width > 0 && positions > 0 ? pg_up(positions, 16) / 16 * pg_cache4_tile_bytes(pg_up(width, 32)) : 0;
+}
+
+PG_API int64_t pg_attention4_part_floats(pg_ctx *ctx, const pg_attention *p)
+{
+    // (slices only where there are fewer units than two per SM)
+    return ctx && p && p->vdim > 0 ? (int64_t)2 * ctx->sm_count * 16 * (pg_up(p->vdim, 32) + 4) : 0;
+}
+
+PG_API int64_t pg_attention4_tickets(pg_ctx *ctx) { return ctx ? (int64_t)2 * ctx->sm_count + 1 : 0; }
+
+PG_API int64_t pg_attention4_unfold_bytes(const pg_attention *p)
+{
+    return p && p->kv_heads > 0 && p->cap > 0 ? (int64_t)p->kv_heads * p->cap * (pg_up(p->dim, 16) + pg_up(p->vdim, 16)) * 2 : 0;
+}
+
+PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t few, int64_t short_rows, int64_t short_len, const float *d_proj,
+                                 int64_t ldp, void *d_kcache, void *d_vcache, void *d_out, int32_t dtype, int64_t ldo)
+{
+    PG_ENTER(ctx);
+    const int32_t rc = check(p, batch, d_kcache, d_vcache, d_out, dtype, ldo);
+    if (rc != PG_OK) return rc;
+    const AttnShape s = pgk_attention_shape(p);
+    const Four f = four_of(s);
+    PG_REQUIRE(d_proj && ldp >= (int64_t)(s.H + s.G) * s.D + (int64_t)s.G * s.V, "attention4: rows too short");
+    PG_REQUIRE(few >= 0 && few <= 4096 && short_rows >= 0 && short_rows <= batch->rows && short_len >= 0 && short_len <= few && (short_len == 0) == (short_rows == 0),
+               "attention4: %lld rows of up to %lld tokens among sequences of up to %lld", (long long)short_rows, (long long)short_len, (long long)few);
+    PG_REQUIRE(s.chunk == 0 || few <= 1, "attention4: a chunked layer takes one token of a sequence here");
+    if (batch->rows == 0) return PG_OK;
+    unsigned char *kc = (unsigned char *)d_kcache, *vc = (unsigned char *)d_vcache;
+    const bool fused = batch->max_len == 1 && few >= 1;
+    if (!fused) {
+        const int32_t ra = launch_pdl(ctx, attn4_append_kernel, dim3((unsigned)batch->rows), dim3(AP_WARPS * 32), 0, s, f, *batch, d_proj, ldp,
+                                      short_rows < batch->rows ? (bf16 *)p->d_q : (bf16 *)nullptr, kc, vc, ctx->d_status);
+        if (ra != PG_OK || short_rows == 0) return ra;
+    }
+    const int64_t cols = (fused ? 1 : short_len) * s.rep;
+    const int blocks = (int)((cols + 15) / 16);
+    PG_REQUIRE((int64_t)s.G * blocks <= 65535, "attention4: too many heads");
+    const bool hi = cols > 8;
+    float *part = p->d_part;
+    int32_t *tickets = p->d_tickets;
+    bf16 *out = (bf16 *)d_out;
+#define PG_A4(GK, GV, HI)                                                                                                                                     \
+    do {                                                                                                                                                      \
+        if (fused) return run_few<GK, GV, HI, true>(ctx, s, f, batch, (int)few, blocks, d_proj, ldp, kc, vc, part, tickets, out, ldo);                        \
+        return run_few<GK, GV, HI, false>(ctx, s, f, batch, (int)few, blocks, d_proj, ldp, kc, vc, part, tickets, out, ldo);                                  \
+    } while (0)
+#define PG_A4_HI(GK, GV)             \
+    do {                             \
+        if (hi) PG_A4(GK, GV, true); \
+        PG_A4(GK, GV, false);        \
+    } while (0)
+    if (f.gk <= 2 && f.gv <= 2) PG_A4_HI(2, 2);
+    if (f.gk <= 4 && f.gv <= 4) PG_A4_HI(4, 4);
+    PG_A4_HI(8, 8);
+#undef PG_A4
+#undef PG_A4_HI
+}
+
+PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t seq, int64_t len, int64_t positions, int64_t slot,
+                                    const void *d_kcache, const void *d_vcache, void *d_work, void *d_out, int32_t dtype, int64_t ldo)
+{
+    PG_ENTER(ctx);
+    const int32_t rc = check(p, batch, d_kcache, d_vcache, d_out, dtype, ldo);
+    if (rc != PG_OK) return rc;
+    const AttnShape s = pgk_attention_shape(p);
+    const Four f = four_of(s);
+    PG_REQUIRE(d_work && ((uintptr_t)d_work & 127) == 0, "attention4: no workspace, or not on a 128-byte boundary");
+    PG_REQUIRE(seq >= 0 && seq < batch->seqs && len > 0 && len <= batch->max_len && positions >= len && positions <= s.limit && slot >= 0 && slot < p->slots,
+               "attention4: sequence %lld with %lld tokens and %lld positions in slot %lld", (long long)seq, (long long)len, (long long)positions, (long long)slot);
+    // the slot's rows that hold something, in the order that they have there
+    const int rows = (int)std::min<int64_t>(positions, s.cap), padded = (int)std::min<int64_t>(rows + 128, s.cap);   // (a tile of keys may end behind them)
+    bf16 *k = (bf16 *)d_work, *v = k + (int64_t)s.G * s.cap * s.dp;
+    const dim3 grid((unsigned)((padded + 15) / 16), (unsigned)s.G);
+    int32_t ru = launch_pdl(ctx, attn4_unfold_kernel<bf16, false>, grid, dim3(128), 0, (const unsigned char *)d_kcache + slot * s.G * f.kh, f.gk, f.kb, f.kh, rows, padded,
+                            s.dp, (int64_t)s.cap * s.dp, k);
+    if (ru == PG_OK)
+        ru = launch_pdl(ctx, attn4_unfold_kernel<bf16, true>, grid, dim3(128), 0, (const unsigned char *)d_vcache + slot * s.G * f.vh, f.gv, f.vb, f.vh, rows, padded,
+                        s.vp, (int64_t)s.cap * s.vp, v);
+    if (ru != PG_OK) return ru;
+    // the sequence as a batch of its own, its cache in slot 0 (the last ticket is always zero)
+    pg_batch one = *batch;
+    one.seqs = 1;
+    one.max_len = (int32_t)len;
+    one.d_seq_row0 += seq;
+    one.d_seq_slot = p->d_tickets + 2 * ctx->sm_count;
+    bf16 *out = (bf16 *)d_out;
+    if (pgk_attention_prompt_tc_supports(s, &one, 1, ldo, out)) return pgk_attention_prompt_tc(ctx, s, &one, 1, (const bf16 *)p->d_q, k, v, out, ldo);
+    return pgk_attention_prompt(ctx, s, &one, (const bf16 *)p->d_q, k, v, out, ldo);
+}
+
+PG_API int32_t pg_cache4_read(pg_ctx *ctx, const void *d_cache, int32_t values, int32_t width, int64_t cap, int64_t parts, int64_t rows, float *d_out)
+{
+    PG_ENTER(ctx);
+    PG_REQUIRE(d_cache && d_out && ((uintptr_t)d_cache & 15) == 0, "cache4_read: null pointer, or not on a 16-byte boundary");
+    PG_REQUIRE(width > 0 && width <= 256 && cap > 0 && parts > 0 && parts <= 65535 && rows > 0 && rows <= cap, "cache4_read: bad shape");
+    const int w = (int)pg_up(width, 32), tile = (int)pg_cache4_tile_bytes(w);
+    const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)parts);
+    const int64_t head = pg_up(cap, 16) / 16 * tile;
+    if (values)
+        return launch_whole(ctx, attn4_unfold_kernel<float, true>, grid, dim3(128), 0, (const unsigned char *)d_cache, w / 32, tile, head, (int)rows, (int)rows, w, rows * w,
+                            d_out);
+    return launch_whole(ctx, attn4_unfold_kernel<float, false>, grid, dim3(128), 0, (const unsigned char *)d_cache, w / 32, tile, head, (int)rows, (int)rows, w, rows * w,
+                            d_out);
+}
+
+}  // extern "C"

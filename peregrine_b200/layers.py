@@ -1,10 +1,10 @@
 """The layer mechanisms of the bf16 / f32 language models: device weights and state of each, and its calls into
 libperegrine_b200_lm.  A model puts a list of them together (peregrine_b200/sonalorn.py); constants are parameters.
 
-    Linear        y = a W^T, plain or gated, one matrix or one per expert
+    Linear        y = a W^T, plain or gated, one matrix or one per expert; Linear4: weights held in 4 bits
     GatedDelta    gated delta rule with short convolutions (recurrent state)
     SelectiveScan selective scan with a short convolution (recurrent state)
-    Attention     per-head norms, query temperature, softmax sink, distance bias, chunks (key / value cache)
+    Attention     per-head norms, query temperature, softmax sink, distance bias, chunks (key / value cache, of 16 bits or of 4)
     LatentAttention  keys and values from a latent per position, rotated key part (latent cache, which layers may share)
     DenseFF       gated feed-forward, clamped or not
     MoeFF         router with corrected, grouped choice and identity experts; clamped gated experts
@@ -30,11 +30,15 @@ class Device:
 
     Activation buffers are kept per width, zero behind the true width: products read K rounded up to 64."""
 
-    def __init__(self, gpu, dtype: str, step_rows: int):
+    def __init__(self, gpu, dtype: str, step_rows: int, bits: int = 16):
+        """bits: of the matrices that a step's layers multiply with, 16 or (bfloat16 steps) 4."""
         import torch
 
         if dtype not in ("bfloat16", "float32"):
             raise ValueError(f"dtype {dtype!r}: bfloat16 or float32")
+        if bits not in (16, 4) or (bits == 4 and dtype != "bfloat16"):
+            raise ValueError(f"weights of {bits} bits in {dtype} steps: 16, or 4 in bfloat16")
+        self.bits = bits
         self.torch, self.gpu, self.lib = torch, gpu, gpu.lib
         self.dev = torch.device("cuda", gpu.device)
         self.code = _lib.BF16 if dtype == "bfloat16" else _lib.F32
@@ -209,6 +213,11 @@ class Linear4:
         return self._bytes
 
 
+def linear(d: Device, w, gated: bool = False):
+    """A product with the weights in the form that the model holds them in (Device.bits)."""
+    return Linear4(d, w, gated) if d.bits == 4 else Linear(d, w, gated)
+
+
 def stack_rows(d: Device, parts, multiple: int = 4):
     """Matrices that read the same input as one, rows padded with zeros to `multiple`."""
     t = d.torch
@@ -232,8 +241,8 @@ class GatedDelta:
         expect("delta mixer", W, {"q": (G * D, width), "k": (G * D, width), "v": (H * V, width), "g": (H * V, width), "b": (H, width), "a": (H, width),
                                   "o": (width, H * V), "q.conv": (G * D, taps), "k.conv": (G * D, taps), "v.conv": (H * V, taps), "A_log": (H,), "dt_bias": (H,),
                                   "norm": (V,)})
-        self.proj = Linear(d, stack_rows(d, [d.bf16(W[n]) for n in ("q", "k", "v", "g", "b", "a")]))
-        self.out = Linear(d, d.bf16(W["o"]))
+        self.proj = linear(d, stack_rows(d, [d.bf16(W[n]) for n in ("q", "k", "v", "g", "b", "a")]))
+        self.out = linear(d, d.bf16(W["o"]))
         self.conv = d.torch.cat([d.f32(W[n + ".conv"]) for n in ("q", "k", "v")], dim=0).t().contiguous()
         self.a_log, self.dt_bias, self.norm = d.f32(W["A_log"]), d.f32(W["dt_bias"]), d.f32(W["norm"])
         self.c = _lib.PgDelta(H, G, D, V, taps, self.eps, self.UNIT_EPS, self.conv.data_ptr(), self.a_log.data_ptr(), self.dt_bias.data_ptr(),
@@ -272,13 +281,67 @@ def halving_slopes(heads: int) -> np.ndarray:
     return (2.0 ** (-8.0 * np.arange(1, heads + 1) / heads)).astype(np.float32)
 
 
+class Attention4Plan:
+    """Attention over keys and values in 4 bits (csrc/pg_attention4.cu): shape, workspaces and the calls of a step.  Caches are uint8
+    [slots, kv_heads, key_bytes] and [.., value_bytes]; cap: rows of a slot, positions: most positions of a sequence (0: cap)."""
+
+    def __init__(self, d: Device, heads: int, kv_heads: int, dim: int, vdim: int, cap: int, slots: int, max_seqs: int, scale: float, sink: bool = False, slopes=None,
+                 chunk: int = 0, positions: int = 0, eps: float = 0.0, q_norm=None, k_norm=None, temp=(0.0, 0.0)):
+        if d.code != _lib.BF16:
+            raise ValueError("a cache in 4 bits is for bfloat16 steps")
+        self.d, self.cap = d, int(cap)
+        ptr = lambda t: t.data_ptr() if t is not None else 0
+        self.keep = (q_norm, k_norm, slopes)
+        self.c = _lib.PgAttention(heads, kv_heads, dim, vdim, self.cap, slots, float(eps), float(scale), float(temp[0]), float(temp[1]), int(sink), int(chunk),
+                                  int(positions), ptr(q_norm), ptr(k_norm), ptr(slopes), 0, 0, 0)
+        self.key_bytes, self.value_bytes = int(d.lib.pg_cache4_bytes(dim, self.cap)), int(d.lib.pg_cache4_bytes(vdim, self.cap))
+        # sequences of up to so many tokens in a step read the cache as it is: four blocks of 16 (token, head) rows
+        self.few = 1 if chunk else max(1, 64 * kv_heads // heads)
+        t = d.torch
+        self.q_cols = heads * up(dim, 16)
+        d.buffer("attn.q", self.q_cols)
+        d.buffer("attn4.part", 1, max(1, d.lib.pg_attention4_part_floats(d.gpu.handle, C.byref(self.c))), t.float32)
+        d.buffer("attn4.tickets", 1, d.lib.pg_attention4_tickets(d.gpu.handle), t.int32)
+        # (elements of 2 bytes; torch's allocations start on 512-byte boundaries)
+        self.work = int(d.lib.pg_attention4_unfold_bytes(C.byref(self.c))) // 2
+        d.buffer("attn4.work", 1, self.work)
+
+    def run(self, batch, proj, kcache, vcache, out) -> None:
+        """proj [rows, q | k | v] f32 -> out [rows, heads * vdim] bf16."""
+        d, c = self.d, self.c
+        c.d_q = d.buffer("attn.q", self.q_cols).data_ptr()
+        c.d_part, c.d_tickets = d.buffer("attn4.part", 1, 1, d.torch.float32).data_ptr(), d.buffer("attn4.tickets", 1, 1, d.torch.int32).data_ptr()
+        lens = [n for _slot, _pos, n in batch.parts if n <= self.few]
+        d.check(d.lib.pg_attention4_run(d.gpu.handle, C.byref(c), C.byref(batch.c), self.few, sum(lens), max(lens, default=0), proj.data_ptr(), proj.stride(0),
+                                        kcache.data_ptr(), vcache.data_ptr(), out.data_ptr(), d.code, out.stride(0)))
+        if len(lens) < len(batch.parts):
+            work = d.buffer("attn4.work", 1, 1)
+            for seq, (slot, pos, n) in enumerate(batch.parts):
+                if n > self.few:
+                    d.check(d.lib.pg_attention4_prompt(d.gpu.handle, C.byref(c), C.byref(batch.c), seq, n, pos + n, slot, kcache.data_ptr(), vcache.data_ptr(),
+                                                       work.data_ptr(), out.data_ptr(), d.code, out.stride(0)))
+
+    def values(self, cache, rows: int, of_values: bool):
+        """What the first rows of every slot and head hold: f32 [slots, kv_heads, rows, width]."""
+        d, t = self.d, self.d.torch
+        width = self.c.vdim if of_values else self.c.dim
+        parts = cache.shape[0] * self.c.kv_heads
+        out = t.empty(parts, rows, up(width, 32), dtype=t.float32, device=d.dev)
+        d.check(d.lib.pg_cache4_read(d.gpu.handle, cache.data_ptr(), int(of_values), width, self.cap, parts, rows, out.data_ptr()))
+        d.gpu.sync()
+        return out.view(cache.shape[0], self.c.kv_heads, rows, -1)[..., :width]
+
+    def free(self) -> None:
+        pass
+
+
 class Attention:
     """p: heads, kv_heads, dim, vdim, scale and, if the query temperature grows, q_temp {coef, every}.  norms: per-head query
     and key norms; slopes: [heads] of a bias slope * distance that is taken off the score; chunk: a position sees the
-    positions of its own chunk only, and the cache keeps the chunks that a step can touch."""
+    positions of its own chunk only, and the cache keeps the chunks that a step can touch.  bits: 16, or 4 for a cache in 4 bits."""
 
     def __init__(self, d: Device, p: dict, W, width: int, eps: float, capacity: int, max_seqs: int, sink: bool = True, norms: bool = True, slopes=None,
-                 chunk: int = 0):
+                 chunk: int = 0, bits: int = 16):
         self.d, self.p = d, p
         H, G, D, V = (int(p[k]) for k in ("heads", "kv_heads", "dim", "vdim"))
         if H % G:
@@ -289,23 +352,32 @@ class Attention:
             self.cap = chunk * min((chunk + d.rows - 2) // chunk + 1, (int(capacity) + chunk - 1) // chunk)
         expect("attention mixer", W, {"q": (H * D, width), "k": (G * D, width), "v": (G * V, width), "o": (width, H * V),
                                       **({"q.norm": (D,), "k.norm": (D,)} if norms else {})})
-        self.proj = Linear(d, stack_rows(d, [d.bf16(W[n]) for n in ("q", "k", "v")]))
-        self.out = Linear(d, d.bf16(W["o"]))
+        self.proj = linear(d, stack_rows(d, [d.bf16(W[n]) for n in ("q", "k", "v")]))
+        self.out = linear(d, d.bf16(W["o"]))
         self.qn, self.kn = (d.f32(W["q.norm"]), d.f32(W["k.norm"])) if norms else (None, None)
         self.slopes = d.f32(slopes) if slopes is not None else None
-        ptr = lambda t: t.data_ptr() if t is not None else 0
         temp = p.get("q_temp") or {}
         self.dp, self.vp = up(D, 16), up(V, 16)
         f32 = d.torch.float32
+        d.buffer("proj", self.proj.n, dtype=f32)
+        d.buffer("mixed", self.out.k)
+        self.plan = None
+        if bits == 4:
+            self.plan = Attention4Plan(d, H, G, D, V, self.cap, 1, max_seqs, p["scale"], sink, self.slopes, chunk, capacity, eps, self.qn, self.kn,
+                                       (temp.get("coef", 0.0), temp.get("every", 0.0)))
+            return
+        ptr = lambda t: t.data_ptr() if t is not None else 0
         self.c = _lib.PgAttention(H, G, D, V, self.cap, 0, float(eps), float(p["scale"]), float(temp.get("coef", 0.0)), float(temp.get("every", 0.0)), int(sink),
                                   int(chunk), int(capacity), ptr(self.qn), ptr(self.kn), ptr(self.slopes), 0, 0, 0)
         d.buffer("attn.part", 1, max(1, d.lib.pg_attention_part_floats(d.gpu.handle, C.byref(self.c), max_seqs)), f32)
         d.buffer("attn.tickets", 1, max_seqs * G * ((H // G + 15) // 16), d.torch.int32)
         d.buffer("attn.q", H * self.dp)
-        d.buffer("proj", self.proj.n, dtype=f32)
-        d.buffer("mixed", self.out.k)
 
     def new_state(self, pool):
+        if self.plan is not None:
+            u8 = self.d.torch.uint8
+            self.plan.c.slots = pool.slots
+            return {"k": pool.tensor((self.G, self.plan.key_bytes), u8), "v": pool.tensor((self.G, self.plan.value_bytes), u8)}
         a = self.d.act
         return {"k": pool.tensor((self.G, self.cap, self.dp), a), "v": pool.tensor((self.G, self.cap, self.vp), a)}
 
@@ -315,6 +387,10 @@ class Attention:
         proj = d.buffer("proj", self.proj.n, dtype=d.torch.float32)
         mixed = d.buffer("mixed", self.out.k)
         self.proj.run(h, rows, proj)
+        if self.plan is not None:
+            self.plan.run(batch, proj, state["k"], state["v"], mixed)
+            self.out.run(mixed, rows, y)
+            return
         self.c.d_q = d.buffer("attn.q", self.H * self.dp).data_ptr()
         self.c.d_part = d.buffer("attn.part", 1, 1, d.torch.float32).data_ptr()
         self.c.d_tickets = d.buffer("attn.tickets", 1, 1, d.torch.int32).data_ptr()
@@ -349,8 +425,8 @@ class LatentAttention:
             raise ValueError(f"latent attention mixer: {p['rot']['dims']} rotated dimensions of {R}")
         expect("latent attention mixer", W, {"q": (H * (D + R), width), "uk": (H * D, K), "uv": (H * V, K), "g": (H * V, width), "o": (width, H * V),
                                              **({"dkv": (K + R, width), "dkv.norm": (K,)} if own else {})})
-        self.proj = Linear(d, stack_rows(d, [d.bf16(W[n]) for n in (("q", "dkv", "g") if own else ("q", "g"))]))
-        self.out = Linear(d, d.bf16(W["o"]))
+        self.proj = linear(d, stack_rows(d, [d.bf16(W[n]) for n in (("q", "dkv", "g") if own else ("q", "g"))]))
+        self.out = linear(d, d.bf16(W["o"]))
         self.norm = d.f32(W["dkv.norm"]) if own else None
         self.cp, self.ck = up(K, 64), up(K, 64) + up(R, 16)
         bf, dev = t.bfloat16, d.dev
@@ -426,8 +502,8 @@ class SelectiveScan:
         self.I, self.N, self.taps = I, N, taps
         expect("scan mixer", W, {"in": (2 * I, width), "conv": (I, taps), "conv.b": (I,), "x": (R + 2 * N, I), "dt": (I, R), "dt.b": (I,), "A_log": (I, N),
                                  "D": (I,), "o": (width, I)})
-        self.proj = Linear(d, stack_rows(d, [d.bf16(W["in"])]))
-        self.out = Linear(d, d.bf16(W["o"]))
+        self.proj = linear(d, stack_rows(d, [d.bf16(W["in"])]))
+        self.out = linear(d, d.bf16(W["o"]))
         # [dt, padded to 64 rows | B | C]: one product where a token decodes, two where a prompt needs dt as an operand
         self.dtp = up(R, 64)
         x = d.bf16(W["x"])
@@ -496,8 +572,8 @@ class DenseFF:
         expect("feed-forward", W, {"gate": (F, width), "up": (F, width), "down": (width, F)})
         self.limit = float(mlp.get("limit", 0.0))
         self.act = _lib.ACT_CLAMPED_SWISH_GLU if "limit" in mlp else _lib.ACT_GELU_TANH_GLU
-        self.gate_up = Linear(d, (d.bf16(W["gate"]), d.bf16(W["up"])), gated=True)
-        self.down = Linear(d, d.bf16(W["down"]))
+        self.gate_up = linear(d, (d.bf16(W["gate"]), d.bf16(W["up"])), gated=True)
+        self.down = linear(d, d.bf16(W["down"]))
         d.buffer("act", self.down.k)
 
     def run(self, batch, h, y, add) -> None:
@@ -533,8 +609,8 @@ class MoeFF:
         every = lambda name: d.torch.stack([d.bf16(W[f"e{e}.{name}"]) for e in range(self.E)])
         self.router = Linear(d, stack_rows(d, [d.bf16(W["router"])]))
         self.correction = d.f32(W["correction"])
-        self.gate_up = Linear(d, (every("gate"), every("up")), gated=True)
-        self.down = Linear(d, every("down"))
+        self.gate_up = linear(d, (every("gate"), every("up")), gated=True)
+        self.down = linear(d, every("down"))
         h = C.c_void_p()
         d.check(d.lib.pg_route_create(d.gpu.handle, d.rows, self.E, self.I, self.top, C.byref(h)))
         self.route = h

@@ -30,10 +30,11 @@ def file_model(architecture: str):
     return put
 
 
-def _slot_engine(model, path, gpu=None, dtype="bfloat16", slots=1, capacity=0, step_rows=2048, portion=0, **_):
+def _slot_engine(model, path, gpu=None, dtype="bfloat16", slots=1, capacity=0, step_rows=2048, portion=0, weight_bits=16, cache_bits=16, **_):
     from .engine import Engine
 
-    return Engine(model.load(path, gpu or GpuContext(component="lm"), dtype=dtype, slots=slots, capacity=capacity, step_rows=step_rows), portion=portion)
+    return Engine(model.load(path, gpu or GpuContext(component="lm"), dtype=dtype, slots=slots, capacity=capacity, step_rows=step_rows,
+                             weight_bits=weight_bits, cache_bits=cache_bits), portion=portion)
 
 
 @folder_model("Sonalorn")
@@ -51,18 +52,21 @@ def _bubotar(path, **options):
 
 
 @file_model("llama")
-def _llama(path, gpu=None, dtype="int8", slots=1, capacity=0, gguf=None, **_):
+def _llama(path, gpu=None, dtype="int8", slots=1, capacity=0, gguf=None, weight_bits=16, cache_bits=16, **_):
     from . import llama_gguf
     from .engine import LockstepEngine
 
     if dtype != "int8":
         raise ValueError("llama runs on the int8 path (dtype int8)")
+    if weight_bits != 16 or cache_bits != 16:
+        raise ValueError("llama runs on the int8 path: no weights or caches of 4 bits")
     decoder, _gguf = llama_gguf.from_gguf(gguf if gguf is not None else path, gpu or init_gpu(), batch=slots, capacity=capacity or None)
     return LockstepEngine(decoder)
 
 
 def load_engine(path: str, **options):
-    """options: gpu, dtype, slots (sequences at once), capacity (positions of each), step_rows, portion."""
+    """options: gpu, dtype, slots (sequences at once), capacity (positions of each), step_rows, portion;
+    weight_bits and cache_bits (folders): 16, or 4 in bfloat16 steps."""
     if os.path.isdir(path):
         with open(os.path.join(path, "config.json")) as f:
             arch = json.load(f).get("architecture")

@@ -71,17 +71,22 @@ class Below:
 class ResidualModel(SlotModel):
     """weights: mapping name -> host array (bf16 bits as uint16, or f32, which is rounded to bf16 where a product reads it).
     slots / capacity: sequences alive at once and positions of each; step_rows: most tokens of one step; max_wanted: most
-    rows of logits of one `head` call.
+    rows of logits of one `head` call.  weight_bits: of the layers' matrices (embedding, head, routers and a latent's or a scan's low-rank
+    matrices stay bf16), cache_bits: of the attention layers' keys and values; 16 or, in bfloat16 steps, 4.
 
     A subclass names its configuration class (`Config`), builds `layers` -- dicts with at least mixer, ff (or None) and state
     -- in `build(weights)`, and enqueues them in `step_ops`."""
 
     Config = None
 
-    def __init__(self, cfg, weights, gpu, dtype: str = "bfloat16", slots: int = 1, capacity: int = 0, step_rows: int = 2048, max_wanted: int = 64):
+    def __init__(self, cfg, weights, gpu, dtype: str = "bfloat16", slots: int = 1, capacity: int = 0, step_rows: int = 2048, max_wanted: int = 64,
+                 weight_bits: int = 16, cache_bits: int = 16):
         self.cfg, self.gpu, self.lib, self.weights = cfg, gpu, gpu.lib, weights
         self.dtype, self.vocab, self.step_rows, self.slots = dtype, cfg.vocab, max(int(step_rows), slots + 1), int(slots)
-        d = self.d = Device(gpu, dtype, self.step_rows)
+        d = self.d = Device(gpu, dtype, self.step_rows, weight_bits)
+        if cache_bits not in (16, 4) or (cache_bits == 4 and dtype != "bfloat16"):
+            raise ValueError(f"a cache of {cache_bits} bits in {dtype} steps: 16, or 4 in bfloat16")
+        self.cache_bits = cache_bits
         torch = self.torch = d.torch
         f32 = torch.float32
         self.capacity = min(int(capacity or cfg.max_positions), cfg.max_positions)

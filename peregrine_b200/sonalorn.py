@@ -69,7 +69,7 @@ class SonalornModel(ResidualModel):
             if L["type"] == "delta":
                 out["mixer"] = GatedDelta(d, L["mixer"], mix, cfg.width, cfg.eps, chunks=not routed)
             else:
-                out["mixer"] = Attention(d, L["mixer"], mix, cfg.width, cfg.eps, self.capacity, self.slots)
+                out["mixer"] = Attention(d, L["mixer"], mix, cfg.width, cfg.eps, self.capacity, self.slots, bits=self.cache_bits)
             if L.get("mlp"):
                 out["ff"] = (DenseFF if L["mlp"]["kind"] == "dense" else MoeFF)(d, L["mlp"], Below(weights, f"l{i}.mlp."), cfg.width)
                 out["norm2"], out["ls2"] = self.vector(f"l{i}.norm2"), self.vector(f"l{i}.ls2")
