@@ -24,9 +24,9 @@ inline int64_t pg_cache4_tile_bytes(int64_t width) { return width * 9; }
 int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int64_t m, int act, float limit, void *y, int y_dtype, int64_t ldy,
                          const PgRouted *routed, int64_t max_blocks);
 size_t pgk_linear4_gemv_workspace(const pg_linear4 *lin);
-// pg_linear4_tc.cu: any number of rows, or the 128-row blocks of a route of `pairs` pairs (m: the rows that it can have)
+// pg_linear4_tc.cu: any number of rows, or the 128-row blocks of a route (m: the rows that it can have)
 int32_t pgk_linear4_tc(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int64_t m, int act, float limit, void *y, int y_dtype, int64_t ldy,
-                       const PgRouted *routed, int64_t pairs);
+                       const PgRouted *routed, const pg_route *route);
 size_t pgk_linear4_tc_workspace(const pg_ctx *ctx);
 
 #ifdef __CUDACC__

@@ -4,10 +4,10 @@
 // W[n][k] = s[n][k / group] (q[n][k] - 8).  A record is 16 rows x 64 k: 512 bytes of quants, then one or (groups of 32) two times 16 scales.
 //
 // Quants: lane (r = lane / 4, t = lane % 4) of a warp has 16 bytes, at 16 (4 r + (t ^ (r / 2 & 3))): in this order neither a warp that reads all of
-// them nor threads that each read the 64 bytes of a row meet a bank twice.  Of its four words, word 2 c + h holds rows r and r + 8, columns
-// 32 c + 8 t + 4 h + {0, 1, 2, 3}: bits 0-3 row r, columns 0 (low half) and 1 (high half); bits 4-7 row r + 8, the same; bits 8-11 and 12-15 the two
-// rows' columns 2 and 3.  That is an A operand of mma.sync m16n8k16 once the quants are f16 numbers.  Scales: rows r and r + 8 side by side; where a
-// group is 128 long its two records both have them, so that a record is all that a block of 64 k needs.
+// them nor threads that each read their row's eight bytes of the four lanes meet a bank twice.  Words c = 0, 1 hold row r, words 2 + c row r + 8, columns
+// 32 c + 8 t + {0 .. 7}: bits 0-3 columns 0 (low half) and 1 (high half), bits 4-7 columns 2 and 3, bits 8-11 4 and 5, bits 12-15 6 and 7.  Once the
+// quants are f16 numbers that is an A operand of mma.sync m16n8k16, and a row's words are its columns in their order.  Scales: rows r and r + 8 side
+// by side; where a group is 128 long its two records both have them, so that a record is all that a block of 64 k needs.
 //
 // Scales are kept as f16 divided by a power of two per row, which brings the row's largest to [2^11, 2^12): scale * (q - 8) is then at most 8 + 3
 // significant bits, so an f16 number, exactly, as long as the row's scales are within 2^21 of each other (below, the smaller ones lose bits
@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(128)
         for (int j = 0; j < 4; j++) {
             w[j] = 0;
 #pragma unroll
-            for (int x = 0; x < 8; x++) {                // x: row half, column 0 .. 3
-                const int rr = r + 8 * (x & 1), c = x >> 1, at = tile * 16 + rr, col = b * 64 + 32 * (j >> 1) + 8 * t + 4 * (j & 1) + c;
+            for (int c = 0; c < 8; c++) {
+                const int rr = r + 8 * (j >> 1), at = tile * 16 + rr, col = b * 64 + 32 * (j & 1) + 8 * t + c;
                 uint32_t v = 8;
                 if (at < n) {
                     if constexpr (QUANTS) {
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(128)
                         v = four_quant(__bfloat162float(reinterpret_cast<const bf16 *>(src)[(e * n + at) * (int64_t)k + col]), sm[(col / group) * 16 + rr]);
                     }
                 }
-                w[j] |= v << ((c & 1) * 16 + (c >> 1) * 8 + (x & 1) * 4);
+                w[j] |= v << ((c & 1) * 16 + (c >> 1) * 4);
             }
         }
         *reinterpret_cast<uint4 *>(dst + (int64_t)b * record + 16 * (4 * r + (t ^ (r >> 1 & 3)))) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -106,9 +106,9 @@ __global__ void __launch_bounds__(256) linear4_read_kernel(const unsigned char *
     const int64_t at = i / k, e = at / n;
     const int rr = (int)(at - e * n), tile = rr / 16, x = rr % 16, r = x % 8, hi = x / 8;
     const int64_t base = e * tiles + tile;
-    const int b = col / 64, c = col % 64, t = c % 32 / 8, j = 2 * (c / 32) + c % 8 / 4, y = c % 4;
+    const int b = col / 64, c = col % 64, t = c % 32 / 8, j = 2 * hi + c / 32, y = c % 8;
     const unsigned char *rec = w + (base * (k / 64) + b) * record;
-    const uint32_t v = *reinterpret_cast<const uint32_t *>(rec + 16 * (4 * r + (t ^ (r >> 1 & 3))) + 4 * j) >> ((y & 1) * 16 + (y >> 1) * 8 + hi * 4) & 15u;
+    const uint32_t v = *reinterpret_cast<const uint32_t *>(rec + 16 * (4 * r + (t ^ (r >> 1 & 3))) + 4 * j) >> ((y & 1) * 16 + (y >> 1) * 4) & 15u;
     const __half s = reinterpret_cast<const __half *>(rec + 512)[(record > 544 ? c / 32 * 16 : 0) + 2 * r + hi];
     out[i] = __half2float(s) * row[base * 16 + x] * (float)((int)v - 8);
 }
@@ -229,7 +229,7 @@ PG_API int32_t pg_linear4_run(pg_ctx *ctx, const pg_linear4 *lin, const void *d_
                (long long)lin->k);
     if (m == 0) return PG_OK;
     if (m <= 16) return pgk_linear4_gemv(ctx, lin, (const bf16 *)d_a, lda, m, act, limit, d_y, y_dtype, ldy, nullptr, 1);
-    return pgk_linear4_tc(ctx, lin, (const bf16 *)d_a, lda, m, act, limit, d_y, y_dtype, ldy, nullptr, 0);
+    return pgk_linear4_tc(ctx, lin, (const bf16 *)d_a, lda, m, act, limit, d_y, y_dtype, ldy, nullptr, nullptr);
 }
 
 PG_API int32_t pg_linear4_run_routed(pg_ctx *ctx, const pg_linear4 *lin, const pg_route *route, const void *d_a, int32_t dtype, int32_t by_token, int32_t act, float limit,
@@ -246,7 +246,7 @@ PG_API int32_t pg_linear4_run_routed(pg_ctx *ctx, const pg_linear4 *lin, const p
         return pgk_linear4_gemv(ctx, lin, (const bf16 *)d_a, lin->k, route->m, act, limit, d_y, y_dtype, ldy, &rt, pairs < route->experts ? pairs : route->experts);
     const int64_t rows = pg_route_rows(pairs, route->experts);
     PG_REQUIRE(rows <= route->max_rows, "linear4: the route is larger than it was created for");
-    return pgk_linear4_tc(ctx, lin, (const bf16 *)d_a, lin->k, rows, act, limit, d_y, y_dtype, ldy, &rt, pairs);
+    return pgk_linear4_tc(ctx, lin, (const bf16 *)d_a, lin->k, rows, act, limit, d_y, y_dtype, ldy, &rt, route);
 }
 
 }  // extern "C"

@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
         if (f < total) issue();
     if (!ROUTED) asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // activations of the warp's part of K: word 4 c + i of column r (and r + 8): the pairs of columns 32 c + 8 t + 2 i
+    // activations of the warp's part of K: word 4 c + i of column r (and r + 8): the pairs of columns 32 c + 8 t + 2 i, every second one over 16 (the
+    // quants beside it come 16 times too large)
     uint32_t x[NT][KWM / 8];
     float back[NT][2];                                    // what the sums of columns 2 t and 2 t + 1 are multiplied by
     int have = -1;
@@ -121,7 +122,10 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
             for (int c = 0; c < KWM / 32; c++) {
                 const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[j][4 * c + i] = four_pack_f16(pg_bf16_lo(w[i]) * down, pg_bf16_hi(w[i]) * down);
+                for (int i = 0; i < 4; i++) {
+                    const float by = i & 1 ? down * 0.0625f : down;
+                    x[j][4 * c + i] = four_pack_f16(pg_bf16_lo(w[i]) * by, pg_bf16_hi(w[i]) * by);
+                }
             }
             back[j][0] = __shfl_sync(0xffffffffu, up, 8 * t);          // (lane 4 c has column c)
             back[j][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
@@ -159,7 +163,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
         const int turn = (j + slot_idx) & (kw - 1);            // the warp that adds the parts up
         if (klen > 0) {
             const float *fac = wrow + base_of(it) * 16 + r;
-            const float f0 = __ldg(fac), f1 = __ldg(fac + 8) * 0.0625f;   // (sums of rows r + 8 are 16 times too large)
+            const float f0 = __ldg(fac), f1 = __ldg(fac + 8);
             if (ROUTED && blk != have) {
                 bring(blk);
                 second = NT == 2 && __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + 8) >= 0;   // (a block's rows are filled from the first on)
@@ -176,11 +180,11 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
 #pragma unroll
-                        for (int u = 2 * h; u < 2 * h + 2; u++) {
-                            const uint32_t w = q[u], w8 = w >> 8;
-                            const uint32_t a0 = four_f16_lo(w), a1 = four_f16_hi(w), a2 = four_f16_lo(w8), a3 = four_f16_hi(w8);
-                            four_mma_f16(sum[0], a0, a1, a2, a3, x[0][8 * b + 2 * u], x[0][8 * b + 2 * u + 1]);
-                            if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][8 * b + 2 * u], x[NT - 1][8 * b + 2 * u + 1]);
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t w0 = u ? q[h] >> 8 : q[h], w1 = u ? q[2 + h] >> 8 : q[2 + h];
+                            const uint32_t a0 = four_f16_lo(w0), a1 = four_f16_lo(w1), a2 = four_f16_hi(w0), a3 = four_f16_hi(w1);
+                            four_mma_f16(sum[0], a0, a1, a2, a3, x[0][8 * b + 4 * h + 2 * u], x[0][8 * b + 4 * h + 2 * u + 1]);
+                            if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][8 * b + 4 * h + 2 * u], x[NT - 1][8 * b + 4 * h + 2 * u + 1]);
                         }
                         // (uniform: the group ends behind this half of the block)
                         if (((2 * b + h + 1) & gmask) == 0) {

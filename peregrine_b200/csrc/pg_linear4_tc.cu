@@ -35,7 +35,7 @@ template <int BN>
 struct Cfg {
     static constexpr int XT = BN / CG * 128;              // 64 columns of a block of the activations, a CTA's half
     static constexpr int A_COL = 2 * BN;                  // behind the two accumulators
-    static constexpr size_t SMEM = (size_t)SLOTS * 2 * XT + RING + 1024 + 256;
+    static constexpr size_t SMEM = (size_t)SLOTS * 2 * XT + RING + 1024 + (2 * SLOTS + 5 + 4 * TEAMS * DEPTH) * 8;
     static constexpr int COLS = BN >= 64 ? BN / 2 : BN;   // accumulator columns of an output warp
     // registers of a lane where the output warps' sums need more than an equal share: 28 x 72 of them, divided
     static constexpr int R_UNPACK = 56, R_OUT = 120, R_REST = 40;
@@ -51,25 +51,18 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b)
     return r;
 }
 
-// ---- rows of a as f16 over a power of two: a CTA per row ----------------------------------------------------------------
-constexpr int RW_T = 256, RW_KEEP = 8;
+// ---- rows of a as f16 over a power of two: a CTA per row of a.  With a route: to the rows of the token's pairs, or (by_token == 0) per pair; rows
+// without a pair keep what is there, and nobody reads their outputs -----------------------------------------------------------------
+constexpr int RW_T = 128, RW_KEEP = 4;
 __global__ void __launch_bounds__(RW_T)
-    linear4_rows_kernel(const bf16 *__restrict__ a, int64_t lda, int k, const PgRouted rt, uint4 *__restrict__ out, float *__restrict__ back)
+    linear4_rows_kernel(const bf16 *__restrict__ a, int64_t lda, int k, const PgRouted rt, const int32_t *pair_row, uint4 *__restrict__ out, float *__restrict__ back)
 {
-    __shared__ float red[8];
+    __shared__ float red[RW_T / 32];
     pg_pdl_begin();
-    const int64_t m = blockIdx.x;
-    int64_t src = m;
-    const bool routed = rt.blocks != nullptr;
-    if (routed) {
-        if (m >= (int64_t)__ldcg(rt.blocks) * PG_ROUTE_BLOCK) return;
-        const int p = __ldcg(rt.row_pair + m);
-        if (p < 0) {                                       // a row of zeros
-            for (int i = threadIdx.x; i < k / 8; i += RW_T) out[m * (k / 8) + i] = make_uint4(0u, 0u, 0u, 0u);
-            if (threadIdx.x == 0) back[m] = 1.0f;
-            return;
-        }
-        if (rt.by_token) src = p / rt.top;
+    int64_t src = blockIdx.x, to = src;
+    if (pair_row && !rt.by_token) {
+        src = to = __ldcg(pair_row + src);
+        if (to < 0) return;
     }
     const uint4 *row = reinterpret_cast<const uint4 *>(a + src * lda);
     const int n = k / 8;
@@ -87,27 +80,35 @@ __global__ void __launch_bounds__(RW_T)
     }
 #pragma unroll
     for (int i = 0; i < RW_KEEP; i++) look(keep[i]);
+#pragma unroll 4
     for (int at = threadIdx.x + RW_KEEP * RW_T; at < n; at += RW_T) look(__ldcg(row + at));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = fmaxf(top, red[i]);
+    for (int i = 0; i < RW_T / 32; i++) top = fmaxf(top, red[i]);
     float down, up;
     four_range(top, down, up);
-    if (threadIdx.x == 0) back[m] = up;
-    auto put = [&](int at, const uint4 &v) {
+    auto f16 = [&](const uint4 &v) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t o[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = four_pack_f16(pg_bf16_lo(w[i]) * down, pg_bf16_hi(w[i]) * down);
-        out[m * n + at] = make_uint4(o[0], o[1], o[2], o[3]);
+        return make_uint4(o[0], o[1], o[2], o[3]);
     };
 #pragma unroll
-    for (int i = 0; i < RW_KEEP; i++)
-        if (threadIdx.x + i * RW_T < n) put(threadIdx.x + i * RW_T, keep[i]);
-    for (int at = threadIdx.x + RW_KEEP * RW_T; at < n; at += RW_T) put(at, __ldcg(row + at));
+    for (int i = 0; i < RW_KEEP; i++) keep[i] = f16(keep[i]);
+    const int copies = pair_row && rt.by_token ? rt.top : 1;
+    for (int c = 0; c < copies; c++) {
+        if (pair_row && rt.by_token) to = __ldcg(pair_row + src * rt.top + c);
+        if (to < 0) continue;
+        if (threadIdx.x == 0) back[to] = up;
+#pragma unroll
+        for (int i = 0; i < RW_KEEP; i++)
+            if (threadIdx.x + i * RW_T < n) out[to * n + threadIdx.x + i * RW_T] = keep[i];
+        for (int at = threadIdx.x + RW_KEEP * RW_T; at < n; at += RW_T) out[to * n + at] = f16(__ldcg(row + at));
+    }
 }
 
 // How the work is divided.  blocks > 0: the tiles' blocks of 64 k, tile after tile, in stretches of `blocks`, one per pair of CTAs; a tile that several
@@ -215,8 +216,9 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = pg_smem(smem_raw), base = (raw_addr + 1023u) & ~1023u;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem_raw + (base - raw_addr) + SLOTS * 2 * C::XT + RING);
-    const uint32_t bar_full = pg_smem(bars), bar_free = bar_full + 8 * SLOTS, bar_tfull = bar_free + 8 * SLOTS, bar_tempty = bar_tfull + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * SLOTS + 4);
+    const uint32_t bar_full = pg_smem(bars), bar_free = bar_full + 8 * SLOTS, bar_tfull = bar_free + 8 * SLOTS, bar_tempty = bar_tfull + 16,
+                   bar_ring = bar_tempty + 16;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * SLOTS + 4 + 4 * TEAMS * DEPTH);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     // (a shuffle's result is known to be the same in the whole warp: what follows from it stays in uniform registers)
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = (int)pg_cluster_rank();
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
             pg_mbar_init(bar_tfull + 8 * i, 1);
             pg_mbar_init(bar_tempty + 8 * i, OUT_WARPS * CG);
         }
+        for (int i = 0; i < 4 * TEAMS * DEPTH; i++) pg_mbar_init(bar_ring + 8 * i, 1);
         *abort_flag = 0;
         pg_mbar_fence();
     }
@@ -336,20 +339,17 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
     } else if (warp < W_OUT) {
         // ---------------------------------------------------------------- quants -> f16 in TMEM: a thread per weight row
         if constexpr (C::SHARES) set_regs_less<C::R_UNPACK>();
-        // A warp copies what it unpacks itself: 32 rows of every fourth of the pieces' blocks, one after the other, through a ring of its own.
-        // (Tensor copies of the tiles, issued by one thread, took 385 to 520 cycles per 64 k.)
+        // A warp copies what it unpacks itself: 32 rows of every fourth of the pieces' blocks, one after the other, through a ring of its own, two bulk
+        // copies a block.  (Tensor copies of the tiles, issued by one thread, took 385 to 520 cycles per 64 k.)
         const int team = (warp - W_UNPACK) >> 2, quarter = warp & 3, ti = lane >> 4, rr = lane & 15;
-        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(warp - W_UNPACK) * (DEPTH * WARP_BLOCK);
-        const int chunks = 2 * record / 16;                    // 16-byte pieces of a 16-row tile's two records
-        const uint32_t off = (uint32_t)(ti * 2 * record + (rr & 7) * 64), swz = (uint32_t)(rr >> 1 & 3) << 4;
-        const uint32_t mask = rr < 8 ? FOUR_LO : FOUR_HI, sub = rr < 8 ? FOUR_OFF_LO : FOUR_OFF_HI;
-        const uint32_t less = rr < 8 ? 0x3c003c00u : 0x2c002c00u;     // 1, and 1 / 16
+        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(warp - W_UNPACK) * (DEPTH * WARP_BLOCK), bar_w = bar_ring + (uint32_t)(warp - W_UNPACK) * (DEPTH * 8);
+        const uint32_t off = (uint32_t)(ti * 2 * record + (rr & 7) * 64 + (rr >> 3) * 8), swz = (uint32_t)(rr >> 1 & 3) << 4;
         const uint32_t s_off = (uint32_t)(ti * 2 * record + 512 + (rr & 7) * 4 + (rr >> 3) * 2), s_step = record > 544 ? 32u : 0u;
         const uint32_t q_off[4] = {off + swz, off + (16u ^ swz), off + (32u ^ swz), off + (48u ^ swz)};
         const uint32_t a_at = tmem + ((uint32_t)(quarter * 32) << 16) + C::A_COL + team * 64, full = pg_leader<CG>(bar_full) + 8 * team, free_at = bar_free + 8 * team;
         // where copies go on: block kb of the piece `to`
         const unsigned char *from = w;
-        uint32_t piece[5];                                     // where a lane's 16-byte pieces are, from `from` on
+        uint32_t stride = 0;                                   // from the quarter's first 16-row tile to its second
         int64_t to_at = at0;
         Piece to = {0, 0, 0};
         int kb = team;
@@ -361,39 +361,32 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
                 kb += to.k0;
                 // (rows behind the last weights repeat the last ones, whose sums are dropped)
                 const int wt = min(w_tile(to.tile) + quarter * 2, alltiles - 1);
-                const uint32_t stride = wt + 1 < alltiles ? (uint32_t)(K / 64 * record) : 0u;
+                stride = wt + 1 < alltiles ? (uint32_t)(K / 64 * record) : 0u;
                 from = w + ((int64_t)wt * (K / 64) + 2 * kb) * record;
-#pragma unroll
-                for (int i = 0; i < 5; i++) {
-                    const int c = lane + 32 * i, second = c >= chunks ? 1 : 0;
-                    piece[i] = second * stride + (uint32_t)(c - second * chunks) * 16;
-                }
             }
         };
         seek();
-        uint32_t put_at = ring, get_at = ring;
+        uint32_t put_at = 0;
         auto bring = [&]() {
-            if (more) {
-                const bool half = odd && kb == kblocks - 1;
-#pragma unroll
-                for (int i = 0; i < 5; i++) {
-                    const int c = lane + 32 * i, in = c >= chunks ? c - chunks : c;
-                    if (c < 2 * chunks && (!half || in < chunks / 2)) pg_cp16(put_at + (uint32_t)c * 16, from + piece[i]);
-                }
-                from += TEAMS * 2 * record;
-                kb += TEAMS;
-                if (kb >= to.k1) seek();
+            if (!more) return;
+            const uint32_t bytes = (uint32_t)(odd && kb == kblocks - 1 ? record : 2 * record);
+            if (lane == 0) {
+                const uint32_t bar = bar_w + put_at * 8, at = ring + put_at * WARP_BLOCK;
+                pg_mbar_expect(bar, 2 * bytes);
+                pg_bulk_load(at, from, bytes, bar);
+                pg_bulk_load(at + 2 * record, from + stride, bytes, bar);
             }
-            pg_cp_commit();
-            put_at += WARP_BLOCK;
-            if (put_at == ring + DEPTH * WARP_BLOCK) put_at = ring;
+            if (++put_at == DEPTH) put_at = 0;
+            from += TEAMS * 2 * record;
+            kb += TEAMS;
+            if (kb >= to.k1) seek();
         };
         // the blocks that are unpacked: every fourth of all; of these the one that may be half
         int64_t read_at = at0;
         Piece now = {0, 0, 0};
         int rb = team;
         for (int i = 0; i < DEPTH - 1; i++) bring();
-        uint32_t phase = 1;
+        uint32_t phase = 1, get_at = 0, get_phase = 0;
         bool ok = true;
 #pragma unroll 1
         for (;; rb += TEAMS) {
@@ -407,28 +400,28 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
             }
             if (rb < 0) break;
             const int halves = odd && rb == kblocks - 1 ? 1 : 2;
-            pg_cp_wait<DEPTH - 2>();
-            __syncwarp();
+            if (!(ok = pg_mbar_wait_warp(bar_w + get_at * 8, get_phase, abort_flag, status, limit_ns))) break;
             // (the slot that is filled now was read in the last round)
             bring();
-            uint32_t at = get_at, to_tmem = a_at;
+            uint32_t at = ring + get_at * WARP_BLOCK, to_tmem = a_at;
 #pragma unroll 1
-            for (int c = 0; c < 2 * halves; c += 2) {          // 64 columns; then 32 at a time: words 2 i and 2 i + 1 of the row's four lanes
+            for (int c = 0; c < halves; c++) {                 // 64 columns, then 32 at a time: word e of the row's four lanes
+                uint2 q[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[i] = lds64(at + q_off[i]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     unsigned short h;
                     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + s_off + e * s_step));
-                    const uint32_t sc = mul_f16x2((uint32_t)h * 0x10001u, less);
+                    const uint32_t sc = (uint32_t)h * 0x10001u, less = mul_f16x2(sc, 0x2c002c00u);   // times 1 / 16
                     uint32_t v[16];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const uint2 q = lds64(at + q_off[i] + e * 8);
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const uint32_t word = j ? q.y : q.x;
-                            v[4 * i + 2 * j] = mul_f16x2(four_sub_f16(four_lop(word, mask, FOUR_F16), sub), sc);
-                            v[4 * i + 2 * j + 1] = mul_f16x2(four_sub_f16(four_lop(word >> 8, mask, FOUR_F16), sub), sc);
-                        }
+                        const uint32_t word = e ? q[i].y : q[i].x, word8 = word >> 8;
+                        v[4 * i] = mul_f16x2(four_f16_lo(word), sc);
+                        v[4 * i + 1] = mul_f16x2(four_f16_hi(word), less);
+                        v[4 * i + 2] = mul_f16x2(four_f16_lo(word8), sc);
+                        v[4 * i + 3] = mul_f16x2(four_f16_hi(word8), less);
                     }
                     if (e == 0 && c == 0) {
                         if (!(ok = pg_mbar_wait_warp(free_at, phase, abort_flag, status, limit_ns))) break;
@@ -443,11 +436,15 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
             tmem_wait_st();
             tc_fence_before();
             pg_arrive_leader_warp<CG>(full, lane);
-            get_at += WARP_BLOCK;
-            if (get_at == ring + DEPTH * WARP_BLOCK) get_at = ring;
+            if (++get_at == DEPTH) get_at = 0, get_phase ^= 1;
             phase ^= 1;
         }
-        pg_cp_wait<0>();
+        if (!ok) {
+            // give copies that are still in flight a bounded time to land before the CTA exits
+            const unsigned long long t0 = pg_globaltimer_ns();
+            while (pg_globaltimer_ns() - t0 < 2000000ull) {
+            }
+        }
     } else {
         // ---------------------------------------------------------------- outputs: the accumulators' sums added up in registers, then written
         if constexpr (C::SHARES) set_regs_more<C::R_OUT>();
@@ -593,15 +590,17 @@ int32_t dispatch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float 
 size_t pgk_linear4_tc_workspace(const pg_ctx *ctx) { return PG_LM_TICKET_BYTES + (size_t)ctx->sm_count * 2 * 128 * BM * sizeof(float); }
 
 int32_t pgk_linear4_tc(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int64_t m, int act, float limit, void *y, int y_dtype, int64_t ldy,
-                       const PgRouted *routed, int64_t pairs)
+                       const PgRouted *routed, const pg_route *route)
 {
     static const PgRouted no_route = {};
     const PgRouted &rt = routed ? *routed : no_route;
+    const int64_t pairs = route ? route->m * route->top : 0;
     const size_t xbytes = (size_t)m * lin->k * 2;
     int32_t rc = pg_scratch_reserve_recording(ctx, xbytes + (size_t)m * sizeof(float));
     if (rc != PG_OK) return rc;
     float *back = reinterpret_cast<float *>((unsigned char *)ctx->scratch + xbytes);
-    rc = launch_pdl(ctx, linear4_rows_kernel, dim3((unsigned)m), dim3(RW_T), 0, a, lda, (int)lin->k, rt, (uint4 *)ctx->scratch, back);
+    rc = launch_pdl(ctx, linear4_rows_kernel, dim3((unsigned)(route ? rt.by_token ? route->m : pairs : m)), dim3(RW_T), 0, a, lda, (int)lin->k, rt,
+                    route ? (const int32_t *)route->pair_row : (const int32_t *)nullptr, (uint4 *)ctx->scratch, back);
     if (rc != PG_OK) return rc;
     if (act == PG_ACT_GELU_TANH_GLU) return dispatch<PG_ACT_GELU_TANH_GLU, bf16>(ctx, lin, ctx->scratch, back, m, limit, (bf16 *)y, ldy, rt, pairs);
     if (act == PG_ACT_CLAMPED_SWISH_GLU) return dispatch<PG_ACT_CLAMPED_SWISH_GLU, bf16>(ctx, lin, ctx->scratch, back, m, limit, (bf16 *)y, ldy, rt, pairs);
