@@ -23,24 +23,24 @@ constexpr int BM = 128;                 // weight rows of a CTA's tile
 constexpr int BK = 128;                 // columns of K in a block (the last one may have 64)
 constexpr int CHUNK = 4;                // blocks that one accumulator sums up
 constexpr int CG = 2;                   // CTAs of a pair
-constexpr int TEAMS = 4;                // of unpacking warps, four warps each; they take the blocks in turn
-constexpr int SLOTS = TEAMS;            // blocks in flight: activations in shared memory, unpacked weights in TMEM (64 columns each)
-// warps: the copies', the products' (and two without work), the unpacking ones, eight for the outputs
-constexpr int W_COPY = 0, W_MMA = 1, W_UNPACK = 4, W_OUT = W_UNPACK + 4 * TEAMS;
-constexpr int T4_THREADS = (W_OUT + 8) * 32;
-constexpr int DEPTH = 4, WARP_BLOCK = 4 * 576;         // blocks in an unpacking warp's own ring, bytes of one (32 rows x 128 k) at most
-constexpr int RING = 4 * TEAMS * DEPTH * WARP_BLOCK;
+constexpr int W_COPY = 0, W_MMA = 1, W_WEIGHTS = 2, W_UNPACK = 4;   // warps: activations, products, weights (two), then the unpacking ones, eight for the outputs
+constexpr int W_BLOCK = 16 * 576;       // bytes of a CTA's weights of a block, at most
 
 template <int BN>
 struct Cfg {
+    static constexpr int TEAMS = BN > 64 ? 2 : 3;         // of unpacking warps, four warps each; they take the blocks in turn
+    static constexpr int SLOTS = 2 * TEAMS;               // blocks in flight: activations in shared memory, unpacked weights in TMEM (64 columns each)
+    static constexpr int OUT = W_UNPACK + 4 * TEAMS, THREADS = (OUT + 8) * 32;
+    static constexpr int DEPTH = 14;                      // blocks in the weights' ring
+    static constexpr int RING = DEPTH * W_BLOCK;
     static constexpr int XT = BN / CG * 128;              // 64 columns of a block of the activations, a CTA's half
     static constexpr int A_COL = 2 * BN;                  // behind the two accumulators
-    static constexpr size_t SMEM = (size_t)SLOTS * 2 * XT + RING + 1024 + (2 * SLOTS + 5 + 4 * TEAMS * DEPTH) * 8;
+    static constexpr size_t SMEM = (size_t)SLOTS * 2 * XT + RING + 1024 + (2 * SLOTS + 5 + 2 * DEPTH) * 8;
     static constexpr int COLS = BN >= 64 ? BN / 2 : BN;   // accumulator columns of an output warp
-    // registers of a lane where the output warps' sums need more than an equal share: 28 x 72 of them, divided
-    static constexpr int R_UNPACK = 56, R_OUT = 120, R_REST = 40;
+    // registers of a lane where the output warps' sums need more than an equal share: 20 x 96 of them, divided
+    static constexpr int R_UNPACK = 80, R_OUT = 128, R_REST = 64;
     static constexpr bool SHARES = COLS >= 64;
-    static_assert(4 * TEAMS * R_UNPACK + 8 * R_OUT + 4 * R_REST == (W_OUT + 8) * 72, "no more registers than there are");
+    static_assert(!SHARES || 4 * TEAMS * R_UNPACK + 8 * R_OUT + 4 * R_REST == (OUT + 8) * 96, "no more registers than there are");
     static_assert(A_COL + 64 * SLOTS <= 512 && SMEM <= 227 * 1024, "TMEM, shared memory");
 };
 
@@ -205,23 +205,23 @@ __device__ __forceinline__ void set_regs_more()
 }
 
 template <int BN, int ACT, typename TY>
-__global__ void __launch_bounds__(T4_THREADS, 1)
+__global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
     linear4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const unsigned char *__restrict__ w, const float *__restrict__ wrow, const float *xback, int M, int N,
                       int K, int record, int wtiles, int alltiles, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, const Share sh, int32_t *status,
                       unsigned long long limit_ns)
 {
     using C = Cfg<BN>;
-    constexpr int COLS = C::COLS;
+    constexpr int COLS = C::COLS, TEAMS = C::TEAMS, SLOTS = C::SLOTS, DEPTH = C::DEPTH, RING = C::RING, W_OUT = C::OUT;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = pg_smem(smem_raw), base = (raw_addr + 1023u) & ~1023u;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem_raw + (base - raw_addr) + SLOTS * 2 * C::XT + RING);
     const uint32_t bar_full = pg_smem(bars), bar_free = bar_full + 8 * SLOTS, bar_tfull = bar_free + 8 * SLOTS, bar_tempty = bar_tfull + 16,
-                   bar_ring = bar_tempty + 16;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * SLOTS + 4 + 4 * TEAMS * DEPTH);
+                   bar_w = bar_tempty + 16, bar_read = bar_w + 8 * DEPTH;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * SLOTS + 4 + 2 * DEPTH);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     // (a shuffle's result is known to be the same in the whole warp: what follows from it stays in uniform registers)
-    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = (int)pg_cluster_rank();
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, rank = __shfl_sync(0xffffffffu, (int)pg_cluster_rank(), 0);
     constexpr int OUT_WARPS = BN >= 64 ? 8 : 4;           // that have columns
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; s++) {
@@ -232,7 +232,10 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
             pg_mbar_init(bar_tfull + 8 * i, 1);
             pg_mbar_init(bar_tempty + 8 * i, OUT_WARPS * CG);
         }
-        for (int i = 0; i < 4 * TEAMS * DEPTH; i++) pg_mbar_init(bar_ring + 8 * i, 1);
+        for (int i = 0; i < DEPTH; i++) {
+            pg_mbar_init(bar_w + 8 * i, 1);
+            pg_mbar_init(bar_read + 8 * i, 4);             // the warps of a team
+        }
         *abort_flag = 0;
         pg_mbar_fence();
     }
@@ -300,6 +303,40 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
                 while (pg_globaltimer_ns() - t0 < 2000000ull) {
                 }
             }
+        } else if (warp >= W_WEIGHTS) {
+            // ------------------------------------------------------------ weights: every second block, a 16-row tile's two records by a lane each
+            // (Copied by the warps that unpack them, a lane's two copies took 450 cycles of a block's 2700; tensor copies of the tile, issued by one
+            // thread, 385 to 520 per 64 k.)
+            int64_t at = at0;
+            Piece p = {0, 0, 0};
+            int kb = warp - W_WEIGHTS;
+            uint32_t entry = (uint32_t)kb, phase = 1;
+            bool ok = true;
+            while (ok) {
+                bool more = true;
+                while (kb >= p.k1 && more) {
+                    kb -= p.k1;
+                    if ((more = next(at, p))) kb += p.k0;
+                }
+                if (!more) break;
+                // (rows behind the last weights repeat the last ones, whose sums are dropped)
+                const unsigned char *from = w + (int64_t)min(w_tile(p.tile) + (lane & 7), alltiles - 1) * (K / 64) * record;
+                for (; kb < p.k1; kb += 2) {
+                    if (!(ok = pg_mbar_wait_warp(bar_read + 8 * entry, phase, abort_flag, status, limit_ns))) break;
+                    const uint32_t bytes = (uint32_t)(odd && kb == kblocks - 1 ? record : 2 * record), bar = bar_w + 8 * entry;
+                    if (lane == 0) pg_mbar_expect(bar, 8 * bytes);
+                    __syncwarp();
+                    if (lane < 8) pg_bulk_load(base + SLOTS * 2 * C::XT + entry * W_BLOCK + (uint32_t)lane * 2 * record, from + (int64_t)(2 * kb) * record, bytes, bar);
+                    entry += 2;
+                    if (entry >= (uint32_t)DEPTH) entry -= DEPTH, phase ^= 1;
+                }
+            }
+            if (!ok) {
+                // give copies that are still in flight a bounded time to land before the CTA exits
+                const unsigned long long t0 = pg_globaltimer_ns();
+                while (pg_globaltimer_ns() - t0 < 2000000ull) {
+                }
+            }
         } else if (warp == W_MMA && rank == 0) {
             // ------------------------------------------------------------ products (the whole warp; one lane's count)
             // This warp shares its scheduler with four that unpack and two that write: every instruction here counts, so one wait and one
@@ -339,54 +376,18 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
     } else if (warp < W_OUT) {
         // ---------------------------------------------------------------- quants -> f16 in TMEM: a thread per weight row
         if constexpr (C::SHARES) set_regs_less<C::R_UNPACK>();
-        // A warp copies what it unpacks itself: 32 rows of every fourth of the pieces' blocks, one after the other, through a ring of its own, two bulk
-        // copies a block.  (Tensor copies of the tiles, issued by one thread, took 385 to 520 cycles per 64 k.)
         const int team = (warp - W_UNPACK) >> 2, quarter = warp & 3, ti = lane >> 4, rr = lane & 15;
-        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(warp - W_UNPACK) * (DEPTH * WARP_BLOCK), bar_w = bar_ring + (uint32_t)(warp - W_UNPACK) * (DEPTH * 8);
+        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(quarter * 4 * record);
         const uint32_t off = (uint32_t)(ti * 2 * record + (rr & 7) * 64 + (rr >> 3) * 8), swz = (uint32_t)(rr >> 1 & 3) << 4;
         const uint32_t s_off = (uint32_t)(ti * 2 * record + 512 + (rr & 7) * 4 + (rr >> 3) * 2), s_step = record > 544 ? 32u : 0u;
         const uint32_t q_off[4] = {off + swz, off + (16u ^ swz), off + (32u ^ swz), off + (48u ^ swz)};
         const uint32_t a_at = tmem + ((uint32_t)(quarter * 32) << 16) + C::A_COL + team * 64, full = pg_leader<CG>(bar_full) + 8 * team, free_at = bar_free + 8 * team;
-        // where copies go on: block kb of the piece `to`
-        const unsigned char *from = w;
-        uint32_t stride = 0;                                   // from the quarter's first 16-row tile to its second
-        int64_t to_at = at0;
-        Piece to = {0, 0, 0};
-        int kb = team;
-        bool more = true;
-        auto seek = [&]() {                                    // to the piece that has the block
-            while (kb >= to.k1) {
-                kb -= to.k1;
-                if (!(more = next(to_at, to))) return;
-                kb += to.k0;
-                // (rows behind the last weights repeat the last ones, whose sums are dropped)
-                const int wt = min(w_tile(to.tile) + quarter * 2, alltiles - 1);
-                stride = wt + 1 < alltiles ? (uint32_t)(K / 64 * record) : 0u;
-                from = w + ((int64_t)wt * (K / 64) + 2 * kb) * record;
-            }
-        };
-        seek();
-        uint32_t put_at = 0;
-        auto bring = [&]() {
-            if (!more) return;
-            const uint32_t bytes = (uint32_t)(odd && kb == kblocks - 1 ? record : 2 * record);
-            if (lane == 0) {
-                const uint32_t bar = bar_w + put_at * 8, at = ring + put_at * WARP_BLOCK;
-                pg_mbar_expect(bar, 2 * bytes);
-                pg_bulk_load(at, from, bytes, bar);
-                pg_bulk_load(at + 2 * record, from + stride, bytes, bar);
-            }
-            if (++put_at == DEPTH) put_at = 0;
-            from += TEAMS * 2 * record;
-            kb += TEAMS;
-            if (kb >= to.k1) seek();
-        };
-        // the blocks that are unpacked: every fourth of all; of these the one that may be half
+        uint32_t turn = 0;                                     // which of the team's two slots
+        // the team's blocks of the pieces' blocks, one after the other
         int64_t read_at = at0;
         Piece now = {0, 0, 0};
         int rb = team;
-        for (int i = 0; i < DEPTH - 1; i++) bring();
-        uint32_t phase = 1, get_at = 0, get_phase = 0;
+        uint32_t phase = 1, entry = (uint32_t)team, w_phase = 0;
         bool ok = true;
 #pragma unroll 1
         for (;; rb += TEAMS) {
@@ -400,10 +401,8 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
             }
             if (rb < 0) break;
             const int halves = odd && rb == kblocks - 1 ? 1 : 2;
-            if (!(ok = pg_mbar_wait_warp(bar_w + get_at * 8, get_phase, abort_flag, status, limit_ns))) break;
-            // (the slot that is filled now was read in the last round)
-            bring();
-            uint32_t at = ring + get_at * WARP_BLOCK, to_tmem = a_at;
+            if (!(ok = pg_mbar_wait_warp(bar_w + entry * 8, w_phase, abort_flag, status, limit_ns))) break;
+            uint32_t at = ring + entry * W_BLOCK, to_tmem = a_at + turn * (64 * TEAMS);
 #pragma unroll 1
             for (int c = 0; c < halves; c++) {                 // 64 columns, then 32 at a time: word e of the row's four lanes
                 uint2 q[4];
@@ -424,7 +423,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
                         v[4 * i + 3] = mul_f16x2(four_f16_hi(word8), less);
                     }
                     if (e == 0 && c == 0) {
-                        if (!(ok = pg_mbar_wait_warp(free_at, phase, abort_flag, status, limit_ns))) break;
+                        if (!(ok = pg_mbar_wait_warp(free_at + turn * (8 * TEAMS), phase, abort_flag, status, limit_ns))) break;
                         tc_fence_after();
                     }
                     tmem_st16(to_tmem + e * 16, v);
@@ -433,17 +432,14 @@ __global__ void __launch_bounds__(T4_THREADS, 1)
                 at += record, to_tmem += 32;
             }
             if (!ok) break;
+            pg_mbar_arrive_warp(bar_read + entry * 8, lane);
             tmem_wait_st();
             tc_fence_before();
-            pg_arrive_leader_warp<CG>(full, lane);
-            if (++get_at == DEPTH) get_at = 0, get_phase ^= 1;
-            phase ^= 1;
-        }
-        if (!ok) {
-            // give copies that are still in flight a bounded time to land before the CTA exits
-            const unsigned long long t0 = pg_globaltimer_ns();
-            while (pg_globaltimer_ns() - t0 < 2000000ull) {
-            }
+            pg_arrive_leader_warp<CG>(full + turn * (8 * TEAMS), lane);
+            entry += TEAMS;
+            if (entry >= (uint32_t)DEPTH) entry -= DEPTH, w_phase ^= 1;
+            phase ^= turn;
+            turn ^= 1;
         }
     } else {
         // ---------------------------------------------------------------- outputs: the accumulators' sums added up in registers, then written
@@ -547,7 +543,7 @@ int32_t launch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float *x
     const int64_t grid = sh.blocks ? (tiles * ((lin->k + BK - 1) / BK) + sh.blocks - 1) / sh.blocks : std::min<int64_t>(tiles, pairs);
     sh.tickets = reinterpret_cast<unsigned int *>(ctx->splitk);
     sh.slabs = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES);
-    return launch_pdl_cluster(ctx, kern, dim3((unsigned)(grid * CG)), dim3(T4_THREADS), C::SMEM, CG, mx, lin->w, lin->row, xback, (int)m, (int)lin->n, (int)lin->k,
+    return launch_pdl_cluster(ctx, kern, dim3((unsigned)(grid * CG)), dim3(C::THREADS), C::SMEM, CG, mx, lin->w, lin->row, xback, (int)m, (int)lin->n, (int)lin->k,
                               (int)lin->record, (int)lin->tiles, (int)(lin->experts * lin->tiles), limit, y, ldy, rt, sh, ctx->d_status, ctx->wait_limit_ns);
 }
 
