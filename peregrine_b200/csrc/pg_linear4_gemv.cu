@@ -7,7 +7,7 @@
 //   * One persistent CTA of 16 warps per SM.  `kw` warps share a tile of 16 weight rows, each with one part of K of at most 512 elements (256 with more than
 //     eight rows), whose activations it keeps in registers; a fill of its ring is one bulk copy, quants and scales.  The parts meet in shared memory
 //     in a fixed order; the warps of a tile take turns in adding.
-//   * K beyond 16 such parts (SPLIT): sp CTAs take the same tiles, their sums go to slabs, the last one in (a ticket) adds in a fixed order.
+//   * K beyond 16 such parts: sp CTAs take the same tiles, their sums go to slabs, the last one in (a ticket) adds in a fixed order.
 //   * ROUTED: rows come in blocks of 16 that share an expert.
 //
 // Every mbarrier wait is bounded; a warp that gave up goes on through the remaining barriers without computing.
@@ -20,31 +20,35 @@ namespace {
 
 constexpr int V4_WARPS = 16, V4_THREADS = V4_WARPS * 32;
 constexpr int V4_SLOTS_MAX = 8;
-__host__ __device__ constexpr int v4_ring(int nt) { return nt == 1 ? 3 * 4352 : 5 * 2304; }   // bytes of a warp's ring
+constexpr int V4_CELLS = 4;                               // tiles whose parts may be on their way at once
+__host__ __device__ constexpr int v4_ring(int nt) { return nt == 1 ? 2 * 4608 : 4 * 2304; }    // bytes of a warp's ring
 __host__ __device__ constexpr int v4_kw_max(int nt) { return nt == 1 ? 512 : 256; }   // (what the registers hold of the activations)
 
-// shared memory: ring | partial sums [2][16 warps][32 lanes][4 NT] | barriers
-// slabs (SPLIT): [sp][items][32 lanes][4 NT]
-template <int ACT, int NT, bool ROUTED, bool SPLIT, typename TY>
+// shared memory: ring | parts of a tile [V4_CELLS][16 warps][32 lanes][4 NT] | barriers
+// slabs (K over several CTAs): [sp][items][32 lanes][4 NT]
+template <int ACT, int NT, bool ROUTED, int G32, typename TY>
 __global__ void __launch_bounds__(V4_THREADS, 1)
-    linear4_gemv_kernel(const bf16 *__restrict__ a, int64_t lda, int M, const unsigned char *__restrict__ w, const float *__restrict__ wrow, int N, int K, int group,
-                        int record, int tiles, int kw, int KW, int KH, int slots, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, int sp, float *slabs,
+    linear4_gemv_kernel(const bf16 *__restrict__ a, int64_t lda, int M, const unsigned char *__restrict__ w, const float *__restrict__ wrow, int N, int K, int record,
+                        int tiles, int kw, int KW, int KH, int slots, float limit, TY *__restrict__ y, int64_t ldy, const PgRouted rt, int sp, float *slabs,
                         unsigned int *tickets, int32_t *status, unsigned long long limit_ns)
 {
     constexpr int CELL = 4 * NT;                          // floats per lane
     constexpr int KWM = v4_kw_max(NT);
     extern __shared__ __align__(128) unsigned char smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, t = lane & 3;
-    const int my_part = SPLIT ? (int)blockIdx.x % sp : 0;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), r = lane >> 2, t = lane & 3;
+    const int my_part = sp > 1 ? (int)blockIdx.x % sp : 0;
     const int groups = V4_WARPS / kw, slot_idx = warp / kw, kpart = warp - slot_idx * kw;
     float *part = reinterpret_cast<float *>(smem + V4_WARPS * v4_ring(NT));
-    unsigned char *tail = reinterpret_cast<unsigned char *>(part + 2 * V4_WARPS * 32 * CELL);
+    unsigned char *tail = reinterpret_cast<unsigned char *>(part + V4_CELLS * V4_WARPS * 32 * CELL);
     const uint32_t my_bar = pg_smem(tail) + (uint32_t)warp * (V4_SLOTS_MAX * 8);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + V4_WARPS * V4_SLOTS_MAX * 8);
+    const uint32_t cell_full = pg_smem(tail) + V4_WARPS * V4_SLOTS_MAX * 8 + (uint32_t)slot_idx * (V4_CELLS * 16), cell_free = cell_full + V4_CELLS * 8;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + V4_WARPS * V4_SLOTS_MAX * 8 + V4_WARPS * V4_CELLS * 16);
     const uint32_t ring = pg_smem(smem) + (uint32_t)(warp * v4_ring(NT));
     if (threadIdx.x == 0) {
         for (int i = 0; i < V4_WARPS * V4_SLOTS_MAX; i++) pg_mbar_init(pg_smem(tail) + 8 * i, 1);
+        for (int i = 0; i < groups * V4_CELLS * 2; i++)
+            pg_mbar_init(pg_smem(tail) + V4_WARPS * V4_SLOTS_MAX * 8 + 8 * i, i / V4_CELLS % 2 ? 1 : max(1, kw - 1));   // the parts are there; they have been added
         *abort_flag = 0;
         pg_mbar_fence();
     }
@@ -52,7 +56,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
 
     const int ka0 = my_part * KH, k0 = ka0 + kpart * KW;
     const int klen = max(0, min(KW, min(K, ka0 + KH) - k0));   // a multiple of 64 and of the group; 0 only in a short last range
-    const int64_t unit = SPLIT ? blockIdx.x / sp : blockIdx.x, units = SPLIT ? gridDim.x / sp : gridDim.x;
+    const int64_t unit = blockIdx.x / sp, units = gridDim.x / sp;
     if (ROUTED) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int nblk = ROUTED ? __ldcg(rt.blocks) : 1;
     const int64_t items = (int64_t)nblk * tiles, per = (items + units * groups - 1) / (units * groups);
@@ -152,30 +156,30 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     };
 
     bool ok = true, second = NT == 2;
-    const int gmask = group / 32 - 1;                     // (the group is a power of two)
-    int slot = 0;
-    uint32_t phase = 0;
+    int slot = 0, cell = 0;
+    uint32_t phase = 0, cell_phase = 0;
     if (!ROUTED && mine > 0 && klen > 0) bring(0);
     for (int j = 0; j < mine; j++) {
         float acc[NT][4] = {};
         const int64_t it = first + j * step;
         const int blk = ROUTED ? (int)(it / tiles) : 0, tile = (int)(it - (int64_t)blk * tiles);
-        const int turn = (j + slot_idx) & (kw - 1);            // the warp that adds the parts up
+        const int turn = (j + slot_idx) & (kw - 1);       // the warp that adds the parts up
         if (klen > 0) {
             const float *fac = wrow + base_of(it) * 16 + r;
             const float f0 = __ldg(fac), f1 = __ldg(fac + 8);
             if (ROUTED && blk != have) {
                 bring(blk);
-                second = NT == 2 && __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + 8) >= 0;   // (a block's rows are filled from the first on)
+                second = NT == 2 && __shfl_sync(0xffffffffu, __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + 8), 0) >= 0;   // (a block's rows are filled from the first on)
             }
             ok = ok && pg_mbar_wait_warp(my_bar + (uint32_t)slot * 8, phase, abort_flag, status, limit_ns);
             if (ok) {
-                const uint32_t slot_at = ring + (uint32_t)slot * fill_bytes, at = slot_at + 16u * (uint32_t)(4 * r + (t ^ (r >> 1 & 3))), s_at = slot_at + 512u + (uint32_t)r * 4;
-                float sum[NT][4] = {};
+                const uint32_t slot_at = ring + (uint32_t)slot * fill_bytes;
+                uint32_t at = slot_at + 16u * (uint32_t)(4 * r + (t ^ (r >> 1 & 3))), s_at = slot_at + 512u + (uint32_t)r * 4;
+                float sum[NT][4];
 #pragma unroll
                 for (int b = 0; b < KWM / 64; b++) {
                     if (b * 64 >= klen) break;
-                    const uint4 q4 = pg_lds128(at + b * record);
+                    const uint4 q4 = pg_lds128(at);
                     const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -183,23 +187,28 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
                         for (int u = 0; u < 2; u++) {
                             const uint32_t w0 = u ? q[h] >> 8 : q[h], w1 = u ? q[2 + h] >> 8 : q[2 + h];
                             const uint32_t a0 = four_f16_lo(w0), a1 = four_f16_lo(w1), a2 = four_f16_hi(w0), a3 = four_f16_hi(w1);
-                            four_mma_f16(sum[0], a0, a1, a2, a3, x[0][8 * b + 4 * h + 2 * u], x[0][8 * b + 4 * h + 2 * u + 1]);
-                            if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][8 * b + 4 * h + 2 * u], x[NT - 1][8 * b + 4 * h + 2 * u + 1]);
+                            const int i = 8 * b + 4 * h + 2 * u;
+                            if ((2 * b + h) % G32 == 0 && u == 0) {
+                                four_mma_f16_first(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);
+                                if (NT == 2 && (!ROUTED || second)) four_mma_f16_first(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][i], x[NT - 1][i + 1]);
+                            } else {
+                                four_mma_f16(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);
+                                if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][i], x[NT - 1][i + 1]);
+                            }
                         }
-                        // (uniform: the group ends behind this half of the block)
-                        if (((2 * b + h + 1) & gmask) == 0) {
+                        if ((2 * b + h + 1) % G32 == 0) { // the group ends behind this half of the record
                             uint32_t both;                // the scales of rows r and r + 8
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(s_at + b * record + (record > 544 ? h * 32 : 0)));
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(s_at + (G32 == 1 ? h * 32 : 0)));
                             const float2 sc = __half22float2(*reinterpret_cast<const __half2 *>(&both));
-                            const float s0 = sc.x, s1 = sc.y;
 #pragma unroll
                             for (int n = 0; n < NT; n++) {
-                                acc[n][0] = fmaf(s0, sum[n][0], acc[n][0]), acc[n][1] = fmaf(s0, sum[n][1], acc[n][1]);
-                                acc[n][2] = fmaf(s1, sum[n][2], acc[n][2]), acc[n][3] = fmaf(s1, sum[n][3], acc[n][3]);
-                                sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.0f;
+                                if (n == 1 && ROUTED && !second) break;
+                                acc[n][0] = fmaf(sc.x, sum[n][0], acc[n][0]), acc[n][1] = fmaf(sc.x, sum[n][1], acc[n][1]);
+                                acc[n][2] = fmaf(sc.y, sum[n][2], acc[n][2]), acc[n][3] = fmaf(sc.y, sum[n][3], acc[n][3]);
                             }
                         }
                     }
+                    at += record, s_at += record;
                 }
                 __syncwarp();                             // every lane has read the slot
                 if (j + slots < total) issue();
@@ -212,40 +221,49 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
             }
         }
         if (kw > 1) {
-            float *cells = part + ((size_t)((j & 1) * V4_WARPS + slot_idx * kw) * 32 + lane) * CELL;
+            // the others leave their parts and go on; the warp whose turn it is waits for them.  It too waits until the cell's last use is over: before
+            // that the phase of cell_full that it would wait on has not begun
+            float *cells = part + ((size_t)(cell * V4_WARPS + slot_idx * kw) * 32 + lane) * CELL;
+            ok = ok && pg_mbar_wait_warp(cell_free + 8 * cell, cell_phase ^ 1, abort_flag, status, limit_ns);
             if (kpart != turn) {
+                if (ok) {
 #pragma unroll
-                for (int n = 0; n < NT; n++) reinterpret_cast<float4 *>(cells + (size_t)kpart * 32 * CELL)[n] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-            }
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + slot_idx), "r"(kw * 32) : "memory");
-            if (kpart == turn) {
-                float all[NT][4] = {};
-#pragma unroll 4
-                for (int p = 0; p < kw; p++) {            // in the order of K, its own where its turn is
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        float4 v = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-                        if (p != turn) v = reinterpret_cast<const float4 *>(cells + (size_t)p * 32 * CELL)[n];
-                        all[n][0] += v.x, all[n][1] += v.y, all[n][2] += v.z, all[n][3] += v.w;
-                    }
+                    for (int n = 0; n < NT; n++) reinterpret_cast<float4 *>(cells + (size_t)kpart * 32 * CELL)[n] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+                    pg_mbar_arrive_warp(cell_full + 8 * cell, lane);
                 }
+            } else {
+                ok = ok && pg_mbar_wait_warp(cell_full + 8 * cell, cell_phase, abort_flag, status, limit_ns);
+                if (ok) {
+                    float all[NT][4] = {};
+#pragma unroll 4
+                    for (int p = 0; p < kw; p++) {        // in the order of K, its own where its turn is
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                        for (int n = 0; n < NT; n++) {
+                            float4 v = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+                            if (p != turn) v = reinterpret_cast<const float4 *>(cells + (size_t)p * 32 * CELL)[n];
+                            all[n][0] += v.x, all[n][1] += v.y, all[n][2] += v.z, all[n][3] += v.w;
+                        }
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[n][i] = all[n][i];
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[n][i] = all[n][i];
+                    pg_mbar_arrive_warp(cell_free + 8 * cell, lane);
+                }
             }
+            if (++cell == V4_CELLS) cell = 0, cell_phase ^= 1;
         }
-        if (kpart == turn) {
-            if (SPLIT) {
+        if (kpart == turn && ok) {
+            if (sp > 1) {
                 float4 *dst = reinterpret_cast<float4 *>(slabs + (((int64_t)my_part * items + it) * 32 + lane) * CELL);
 #pragma unroll
                 for (int n = 0; n < NT; n++) dst[n] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-            } else if (ok) {
+            } else {
                 finish(acc, blk, tile);
             }
         }
     }
-    if (SPLIT) {
+    if (sp > 1) {
         __shared__ int last_in;
         __threadfence();
         __syncthreads();
@@ -312,18 +330,18 @@ Parts parts_of(const pg_linear4 *lin, int64_t items, int sms, int nt)
     return p;
 }
 
-template <int ACT, int NT, bool ROUTED, bool SPLIT, typename TY>
+template <int ACT, int NT, bool ROUTED, int G32, typename TY>
 int32_t launch(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_t lda, int M, const Parts &p, int grid, float limit, TY *y, int64_t ldy, const PgRouted &rt)
 {
-    auto kern = linear4_gemv_kernel<ACT, NT, ROUTED, SPLIT, TY>;
-    constexpr int smem = V4_WARPS * v4_ring(NT) + 2 * V4_WARPS * 32 * 4 * NT * 4 + V4_WARPS * V4_SLOTS_MAX * 8 + 16;
+    auto kern = linear4_gemv_kernel<ACT, NT, ROUTED, G32, TY>;
+    constexpr int smem = V4_WARPS * v4_ring(NT) + V4_CELLS * V4_WARPS * 32 * 4 * NT * 4 + V4_WARPS * (V4_SLOTS_MAX * 8 + V4_CELLS * 16) + 16;
     static_assert(smem <= 226 * 1024, "shared memory of the streaming form");
     static std::atomic<uint64_t> set{0};
     PG_CUDA(pg_max_smem_once(kern, smem, ctx->device, set));
     const int slots = std::min(V4_SLOTS_MAX, v4_ring(NT) / (int)(p.KW / 64 * lin->record));
     unsigned int *tickets = reinterpret_cast<unsigned int *>(ctx->splitk);
-    float *slabs = SPLIT ? reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES) : nullptr;
-    return launch_pdl(ctx, kern, dim3((unsigned)grid), dim3(V4_THREADS), (size_t)smem, a, lda, M, lin->w, lin->row, (int)lin->n, (int)lin->k, (int)lin->group,
+    float *slabs = p.sp > 1 ? reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(ctx->splitk) + PG_LM_TICKET_BYTES) : nullptr;
+    return launch_pdl(ctx, kern, dim3((unsigned)grid), dim3(V4_THREADS), (size_t)smem, a, lda, M, lin->w, lin->row, (int)lin->n, (int)lin->k,
                       (int)lin->record, (int)lin->tiles, p.kw, p.KW, p.KH, slots, limit, y, ldy, rt, p.sp, slabs, tickets, ctx->d_status, ctx->wait_limit_ns);
 }
 
@@ -355,8 +373,9 @@ int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int6
     const PgRouted &rt = routed ? *routed : no_route;
 #define PG_V4(ACT, NT, RT, TY)                                                                                                                   \
     do {                                                                                                                                         \
-        if (p.sp > 1) return launch<ACT, NT, RT, true, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                          \
-        return launch<ACT, NT, RT, false, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                                       \
+        if (lin->group == 32) return launch<ACT, NT, RT, 1, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                     \
+        if (lin->group == 64) return launch<ACT, NT, RT, 2, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                     \
+        return launch<ACT, NT, RT, 4, TY>(ctx, lin, a, lda, (int)m, p, grid, limit, (TY *)y, ldy, rt);                                           \
     } while (0)
 #define PG_V4_ACT(ACT, TY)                  \
     do {                                    \

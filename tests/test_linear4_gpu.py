@@ -206,6 +206,22 @@ def test_large_tiles_and_parts(lm, m):
         lin.free()
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 12005, 8192), (8, 12005, 8192), (16, 16000, 4096), (11, 24000, 2048)])
+def test_many_tiles_of_a_block(lm, m, n, k):
+    """Several times more tiles than a block holds sums of at once, K in as many parts as it has warps; again with the same result."""
+    d = device(lm)
+    g = rng(m + n)
+    q, s, w = quants(g, 1, n, k, group=64)
+    lin = handle(d, q, s)
+    x = bf16(d, g.standard_normal((m, k)))
+    want, bound = sums(x.double().cpu().numpy(), w[0])
+    first = run(d, lin, x, m, n)
+    within(first, want, bound)
+    for _ in range(3):
+        assert np.array_equal(run(d, lin, x, m, n), first)
+    lin.free()
+
+
 @pytest.mark.parametrize("m", [3, 20])
 def test_activations_of_any_size(lm, m):
     """Rows of the largest and smallest magnitudes; an infinity or a not-a-number stays in its row."""
