@@ -163,7 +163,7 @@ PG_API int32_t pg_attention_run(pg_ctx *ctx, const pg_attention *p, const pg_bat
  * columns, 256 bytes each, then for every pair of positions the bf16 scales of every 32 columns, both positions side by side.
  *   keys    position 8 n + r, column 16 s + 4 t + 2 i + h of 32: byte [r][t][s][2 h + n], low half for i = 0
  *   values  position 8 i + 2 t + h, column 16 s + 8 n + r of 32: byte [r][t][s][2 h + i], low half for n = 0
- * pg_attention: d_q is used by pg_attention4_prompt only; d_part: pg_attention4_part_floats(...); d_tickets: [pg_attention4_tickets(...)], zero before the
+ * pg_attention: d_q, [max_rows][H][dp + 2] halves on a 16-byte boundary, is used where pg_attention4_prompt follows only; d_part: pg_attention4_part_floats(...); d_tickets: [pg_attention4_tickets(...)], zero before the
  * first call. */
 PG_API int64_t pg_cache4_bytes(int32_t width, int64_t positions);
 PG_API int64_t pg_attention4_part_floats(pg_ctx *ctx, const pg_attention *p);
@@ -172,8 +172,8 @@ PG_API int64_t pg_attention4_tickets(pg_ctx *ctx);
  * at most short_len of one sequence.  Longer ones take pg_attention4_prompt behind it. */
 PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t few, int64_t short_rows, int64_t short_len, const float *d_proj,
                                  int64_t ldp, void *d_kcache, void *d_vcache, void *d_out, int32_t dtype, int64_t ldo);
-/* Sequence `seq` of the batch: len tokens in this step, positions with them, in slot `slot`.  Its cache is unfolded to bf16 in d_work
- * (pg_attention4_unfold_bytes(...) on a 128-byte boundary), one rounding. */
+/* Sequence `seq` of the batch: len tokens in this step, positions with them, in slot `slot`.  Its cache is unfolded in d_work
+ * (pg_attention4_unfold_bytes(...) on a 128-byte boundary) as f16 over a power of two of each head. */
 PG_API int64_t pg_attention4_unfold_bytes(const pg_attention *p);
 PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t seq, int64_t len, int64_t positions, int64_t slot,
                                     const void *d_kcache, const void *d_vcache, void *d_work, void *d_out, int32_t dtype, int64_t ldo);

@@ -278,7 +278,15 @@ __global__ void __launch_bounds__(AF_T, QT > 1 ? 4 : 8)
 __device__ __forceinline__ uint32_t tile_at(uint32_t base, int stride, int row, int elem) { return base + (uint32_t)(row * stride + elem * 2); }
 
 // S[16 x 16 keys] of one row tile: two 8-key accumulators
-template <int DC>
+template <bool HALF>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if (HALF)
+        four_mma_f16(d, a0, a1, a2, a3, b0, b1);
+    else
+        pg_mma_bf16(d, a0, a1, a2, a3, b0, b1);
+}
+template <int DC, bool HALF = false>
 __device__ __forceinline__ void scores16(const uint32_t (&qf)[DC][4], int nk, uint32_t kt, int kstride, int key0, int lane, float (&s0)[4], float (&s1)[4])
 {
     const int row = key0 + (lane & 7) + ((lane >> 4) << 3), el = ((lane >> 3) & 1) * 8;
@@ -287,13 +295,13 @@ __device__ __forceinline__ void scores16(const uint32_t (&qf)[DC][4], int nk, ui
         if (i < nk) {
             uint32_t b[4];
             pg_ldsm4(b, tile_at(kt, kstride, row, i * 16 + el));
-            pg_mma_bf16(s0, qf[i][0], qf[i][1], qf[i][2], qf[i][3], b[0], b[1]);
-            pg_mma_bf16(s1, qf[i][0], qf[i][1], qf[i][2], qf[i][3], b[2], b[3]);
+            mma16<HALF>(s0, qf[i][0], qf[i][1], qf[i][2], qf[i][3], b[0], b[1]);
+            mma16<HALF>(s1, qf[i][0], qf[i][1], qf[i][2], qf[i][3], b[2], b[3]);
         }
     }
 }
 // O[16 x V] += P[16 x 16 keys] V
-template <int VC>
+template <int VC, bool HALF = false>
 __device__ __forceinline__ void values16(float (&o)[VC][4], int nv, const uint32_t (&p)[4], uint32_t vt, int vstride, int key0, int lane)
 {
     const int row = key0 + (lane & 7) + ((lane >> 3) & 1) * 8, el = (lane >> 4) * 8;
@@ -302,8 +310,8 @@ __device__ __forceinline__ void values16(float (&o)[VC][4], int nv, const uint32
         if (i < nv) {
             uint32_t b[4];
             pg_ldsm4_t(b, tile_at(vt, vstride, row, i * 8 + el));
-            pg_mma_bf16(o[i], p[0], p[1], p[2], p[3], b[0], b[1]);
-            pg_mma_bf16(o[i + 1], p[0], p[1], p[2], p[3], b[2], b[3]);
+            mma16<HALF>(o[i], p[0], p[1], p[2], p[3], b[0], b[1]);
+            mma16<HALF>(o[i + 1], p[0], p[1], p[2], p[3], b[2], b[3]);
         }
     }
 }
@@ -311,7 +319,8 @@ __device__ __forceinline__ void values16(float (&o)[VC][4], int nv, const uint32
 // ---- prompts: grid (row tiles, G, seqs) --------------------------------------------------------------------------
 constexpr int AP_KEYS = 64;
 
-template <int DC, int VC, int WARPS>
+// HALF: f16 queries, keys, values and probabilities, in bf16's place (AttnShape)
+template <int DC, int VC, int WARPS, bool HALF>
 __global__ void __launch_bounds__(WARPS * 32)
     attn_prompt_kernel(const AttnShape s, const pg_batch bt, const bf16 *__restrict__ q, const bf16 *__restrict__ kc, const bf16 *__restrict__ vc,
                        bf16 *__restrict__ out, int64_t ldo)
@@ -377,9 +386,17 @@ __global__ void __launch_bounds__(WARPS * 32)
     for (int i = 0; i < VC; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
-    const float sl = s.scale * LOG2E;                     // scores in units of log 2
-    // (a row may see no key of a chunk in front of its own: the maxima start finite, so that exp2(-inf - m) is 0)
-    float m0 = s.sink ? 0.0f : -1e30f, m1 = m0, l0 = 0.0f, l1 = 0.0f;
+    float sl0 = s.scale * LOG2E, sl1 = sl0, v_up = 1.0f;  // scores in units of log 2
+    if (HALF) {
+        float down, up;
+        attn_range(s.k_top, g, lane, down, up);
+        sl0 *= up * __ldcg(s.q_up + (int64_t)(row0 + c0 / s.rep) * s.H + g * s.rep + c0 % s.rep);
+        sl1 *= up * __ldcg(s.q_up + (int64_t)(row0 + c1 / s.rep) * s.H + g * s.rep + c1 % s.rep);
+        attn_range(s.v_top, g, lane, down, v_up);
+    }
+    // (a row may see no key of a chunk in front of its own: the maxima start finite, so that exp2(-inf - m) is 0; f16 holds probabilities
+    // of the row's own maximum only)
+    float m0 = s.sink && !HALF ? 0.0f : -1e30f, m1 = m0, l0 = 0.0f, l1 = 0.0f;
     fetch(0, kmin);
     int buf = 0;
     for (int j0 = kmin; j0 < kmax; j0 += AP_KEYS, buf ^= 1) {
@@ -397,7 +414,7 @@ __global__ void __launch_bounds__(WARPS * 32)
 #pragma unroll
             for (int j = 0; j < 4; j++) sc[n][j] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < AP_KEYS / 16; n++) scores16<DC>(qf, nk, kt, kstride, n * 16, lane, sc[2 * n], sc[2 * n + 1]);
+        for (int n = 0; n < AP_KEYS / 16; n++) scores16<DC, HALF>(qf, nk, kt, kstride, n * 16, lane, sc[2 * n], sc[2 * n + 1]);
         float b0 = -INFINITY, b1 = -INFINITY;
         const bool edge = j0 + AP_KEYS - 1 > pos0 + rr0 / s.rep || j0 < low_last;   // some row of the tile does not see all of these keys
 #pragma unroll
@@ -405,8 +422,8 @@ __global__ void __launch_bounds__(WARPS * 32)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int key = j0 + n * 8 + 2 * t + j;
-                sc[n][j] = (!edge || (key <= lim0 && key >= low0)) ? fmaf(bias0, (float)(key - lim0), sc[n][j] * sl) : -INFINITY;
-                sc[n][2 + j] = (!edge || (key <= lim1 && key >= low1)) ? fmaf(bias1, (float)(key - lim1), sc[n][2 + j] * sl) : -INFINITY;
+                sc[n][j] = (!edge || (key <= lim0 && key >= low0)) ? fmaf(bias0, (float)(key - lim0), sc[n][j] * sl0) : -INFINITY;
+                sc[n][2 + j] = (!edge || (key <= lim1 && key >= low1)) ? fmaf(bias1, (float)(key - lim1), sc[n][2 + j] * sl1) : -INFINITY;
                 b0 = fmaxf(b0, sc[n][j]);
                 b1 = fmaxf(b1, sc[n][2 + j]);
             }
@@ -440,8 +457,8 @@ __global__ void __launch_bounds__(WARPS * 32)
                 l0 += p[j] + p[4 + j];
                 l1 += p[2 + j] + p[6 + j];
             }
-            const uint32_t pf[4] = {pg_pack_bf16(p[0], p[1]), pg_pack_bf16(p[2], p[3]), pg_pack_bf16(p[4], p[5]), pg_pack_bf16(p[6], p[7])};
-            values16<VC>(o, nv, pf, vt, vstride, n * 16, lane);
+            const uint32_t pf[4] = {attn_pack<HALF>(p[0], p[1]), attn_pack<HALF>(p[2], p[3]), attn_pack<HALF>(p[4], p[5]), attn_pack<HALF>(p[6], p[7])};
+            values16<VC, HALF>(o, nv, pf, vt, vstride, n * 16, lane);
         }
         __syncthreads();
     }
@@ -454,16 +471,17 @@ __global__ void __launch_bounds__(WARPS * 32)
         l0 += exp2f(-m0);
         l1 += exp2f(-m1);
     }
-    const float i0 = __fdiv_rn(1.0f, l0), i1 = __fdiv_rn(1.0f, l1);
+    const float i0 = __fdiv_rn(1.0f, l0) * v_up, i1 = __fdiv_rn(1.0f, l1) * v_up;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int rr = h ? my1 : my0;
         if (rr >= total) continue;
         bf16 *dst = out + (int64_t)(row0 + rr / s.rep) * ldo + (int64_t)(g * s.rep + rr % s.rep) * s.V;
-        const float inv = h ? i1 : i0;
+        float inv = h ? i1 : i0;
 #pragma unroll
         for (int i = 0; i < VC; i++) {
             const int c = i * 8 + 2 * t;
+            if (HALF && i % 4 == 0 && c < s.V) inv = attn_sees_bad(s, g, c, h ? lim1 : lim0) ? __uint_as_float(0x7fc00000u) : h ? i1 : i0;
             if (c < s.V) pg_put(dst + c, o[i][2 * h] * inv);
             if (c + 1 < s.V) pg_put(dst + c + 1, o[i][2 * h + 1] * inv);
         }
@@ -767,6 +785,8 @@ AttnShape pgk_attention_shape(const pg_attention *p)
     s.slopes = p->d_slopes;
     s.eps = p->eps, s.scale = p->scale, s.coef = p->temp_coef, s.every = p->temp_every;
     s.qn = p->d_q_norm, s.kn = p->d_k_norm;
+    s.q_up = s.k_top = s.v_top = nullptr;
+    s.v_bad = nullptr;
     return s;
 }
 
@@ -781,15 +801,15 @@ int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s)
     return (int)std::min<int64_t>(S, AS_SLICES);
 }
 
-template <int DC, int VC>
+template <int DC, int VC, bool HALF>
 int32_t run_prompt(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, const bf16 *q, const bf16 *kc, const bf16 *vc, bf16 *out, int64_t ldo)
 {
     constexpr int WARPS = DC > 8 || VC > 16 ? 4 : 8;
     const int smem = 2 * AP_KEYS * ((s.dp + s.vp) * 2 + 32);
     static std::atomic<uint64_t> set{0};
-    PG_CUDA(pg_max_smem_once(attn_prompt_kernel<DC, VC, WARPS>, 2 * AP_KEYS * ((DC * 16 + VC * 8) * 2 + 32), ctx->device, set));
+    PG_CUDA(pg_max_smem_once(attn_prompt_kernel<DC, VC, WARPS, HALF>, 2 * AP_KEYS * ((DC * 16 + VC * 8) * 2 + 32), ctx->device, set));
     const int64_t tiles = ((int64_t)bt->max_len * s.rep + WARPS * 16 - 1) / (WARPS * 16);
-    return launch_pdl(ctx, attn_prompt_kernel<DC, VC, WARPS>, dim3((unsigned)tiles, (unsigned)s.G, (unsigned)bt->seqs), dim3(WARPS * 32), (size_t)smem, s, *bt,
+    return launch_pdl(ctx, attn_prompt_kernel<DC, VC, WARPS, HALF>, dim3((unsigned)tiles, (unsigned)s.G, (unsigned)bt->seqs), dim3(WARPS * 32), (size_t)smem, s, *bt,
                       q, kc, vc, out, ldo);
 }
 
@@ -823,9 +843,14 @@ int32_t pgk_attention_f32(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, c
 
 int32_t pgk_attention_prompt(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, const bf16 *q, const bf16 *kc, const bf16 *vc, bf16 *out, int64_t ldo)
 {
-    if (s.dp <= 64 && s.vp <= 64) return run_prompt<4, 8>(ctx, s, bt, q, kc, vc, out, ldo);
-    if (s.dp <= 128 && s.vp <= 128) return run_prompt<8, 16>(ctx, s, bt, q, kc, vc, out, ldo);
-    return run_prompt<16, 32>(ctx, s, bt, q, kc, vc, out, ldo);
+    if (s.q_up) {
+        if (s.dp <= 64 && s.vp <= 64) return run_prompt<4, 8, true>(ctx, s, bt, q, kc, vc, out, ldo);
+        if (s.dp <= 128 && s.vp <= 128) return run_prompt<8, 16, true>(ctx, s, bt, q, kc, vc, out, ldo);
+        return run_prompt<16, 32, true>(ctx, s, bt, q, kc, vc, out, ldo);
+    }
+    if (s.dp <= 64 && s.vp <= 64) return run_prompt<4, 8, false>(ctx, s, bt, q, kc, vc, out, ldo);
+    if (s.dp <= 128 && s.vp <= 128) return run_prompt<8, 16, false>(ctx, s, bt, q, kc, vc, out, ldo);
+    return run_prompt<16, 32, false>(ctx, s, bt, q, kc, vc, out, ldo);
 }
 
 extern "C" {

@@ -3,6 +3,7 @@
 
 #include <math.h>
 
+#include "pg_four.cuh"
 #include "pg_lm.cuh"
 
 struct AttnShape {
@@ -13,7 +14,13 @@ struct AttnShape {
     float eps, scale, coef, every;
     const float *qn, *kn;                // null: no norm
     const float *slopes;                 // [H], null: no distance bias
+    // queries, keys and values in f16 over powers of two (null: in bf16): what a query is multiplied by [rows][H], and the largest
+    // magnitudes of a head's keys and values, TOPS of them each
+    const float *q_up, *k_top, *v_top;
+    // [G][V up to 32 / 32][chunks of a slot]: the first row of a chunk whose values in 32 columns are not numbers, which are zeros where the values lie
+    const int *v_bad;
 };
+constexpr int ATTN_TOPS = 32;
 
 #ifdef __CUDACC__
 // A chunked layer keeps whole chunks only, position p in row p mod cap: the rows of a chunk lie next to each other.
@@ -42,6 +49,27 @@ __device__ __forceinline__ void attn_head_norm(const float *src, const float *__
         const int c = i * 32 + lane;
         if (c < dp) pg_put(dst + c, c < D ? x[i] * inv * (w ? __ldg(w + c) : 1.0f) * mul : 0.0f);
     }
+}
+
+// The powers of two of a head's keys or values, by a whole warp (they are within 2^15 times the first).
+__device__ __forceinline__ void attn_range(const float *tops, int g, int lane, float &down, float &up)
+{
+    float top = __ldcg(tops + g * ATTN_TOPS + lane);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    four_range(top, down, up);
+}
+// does a row that ends with position `pos` see values that are not numbers in the 32 columns from c on?
+__device__ __forceinline__ bool attn_sees_bad(const AttnShape &s, int g, int c, int pos)
+{
+    const int row = attn_row(s, pos), chunks = s.chunk ? s.cap / s.chunk : 1;
+    return __ldcg(s.v_bad + (g * ((s.V + 31) / 32) + c / 32) * chunks + (s.chunk ? row / s.chunk : 0)) <= row;
+}
+// operands of matrix instructions, two of them in a word
+template <bool HALF>
+__device__ __forceinline__ uint32_t attn_pack(float lo, float hi)
+{
+    return HALF ? four_pack_f16(lo, hi) : pg_pack_bf16(lo, hi);
 }
 #endif
 

@@ -12,8 +12,8 @@
 //                               Keys as f16 integers (exact) times the query as f16 over a power of two, sums of 32 columns scaled in f32; values as
 //                               bf16 integers (exact) times bf16(probability * scale).  One token per sequence (FUSED): the CTA with the newest
 //                               position quantises and appends it.  The last CTA of a (sequence, rows) to finish merges the slices.
-//   longer portions             attn4_append_kernel, then per sequence attn4_unfold_kernel (the values as bf16, one rounding) and the kernels that
-//                               prompts over a bf16 cache run through.
+//   longer portions             attn4_append_kernel, then per sequence attn4_unfold_kernel and the kernels that prompts over a bf16 cache run through, on
+//                               f16: keys and values over a power of two of their head, which is exact, queries over one of their own.
 #include <algorithm>
 
 #include "pg_async.cuh"
@@ -87,14 +87,16 @@ __device__ __forceinline__ void load_row(const float *src, const float *__restri
         if (32 * i + lane < width) x[i] *= inv * __ldg(w + 32 * i + lane);
 }
 
-// ---- append: a CTA per token, a warp per key or value head; with q: the queries too, as the prompt kernels read them ----------
+// ---- append: a CTA per token, a warp per key or value head; with q: the queries too, for pg_attention4_prompt ----------------------
+// A lane has four columns of every 128: 32 columns are those of eight lanes, so that the largest magnitudes of all groups are found together.
+// The next row is on its way while one is worked on.  2000 tokens of 32 + 8 + 8 heads of 128: 23 us
+// (49 MB of rows at 2.1 TB/s; instructions bound it, 160 to a row, three quarters of them the quants' and the queries' conversions).
 constexpr int AP_WARPS = 8;
-__global__ void __launch_bounds__(AP_WARPS * 32)
-    attn4_append_kernel(const AttnShape s, const Four f, const pg_batch bt, const float *__restrict__ proj, int64_t ldp, bf16 *__restrict__ q, unsigned char *kc,
-                        unsigned char *vc, int32_t *status)
+template <int NV, bool WIDE>                              // blocks of 128 columns; rows of 16-byte words
+__global__ void __launch_bounds__(AP_WARPS * 32, NV == 1 ? 6 : 4)
+    attn4_append_kernel(const AttnShape s, const Four f, const pg_batch bt, const float *__restrict__ proj, int64_t ldp, __half *__restrict__ q, float *__restrict__ q_up,
+                        unsigned char *kc, unsigned char *vc, int32_t *status)
 {
-    __shared__ uint8_t quants[AP_WARPS][256];
-    __shared__ bf16 scales[AP_WARPS][8];
     pg_pdl_begin();
     const int m = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int pos = __ldcg(bt.d_pos + m);
@@ -104,53 +106,233 @@ __global__ void __launch_bounds__(AP_WARPS * 32)
         return;
     }
     const float *row = proj + (int64_t)m * ldp;
-    const int at = attn_row(s, pos);
-    for (int i = warp; i < 2 * s.G; i += AP_WARPS) {
-        const bool key = i < s.G;
-        const int g = key ? i : i - s.G;
-        float x[8];
-        load_row(key ? row + (int64_t)(s.H + g) * s.D : row + (int64_t)(s.H + s.G) * s.D + (int64_t)g * s.V, key ? s.kn : nullptr, key ? s.D : s.V, s.eps, x, lane);
-        quantise_row(x, key ? f.gk : f.gv, quants[warp], scales[warp], lane);
-        if (key)
-            put_key(kc + (slot * s.G + g) * f.kh + (int64_t)(at >> 4) * f.kb, quants[warp], scales[warp], at & 15, f.gk, lane);
-        else
-            put_value(vc + (slot * s.G + g) * f.vh + (int64_t)(at >> 4) * f.vb, quants[warp], scales[warp], at & 15, f.gv, lane);
-        __syncwarp();
-    }
-    if (q) {
-        const float mul = attn_temperature(s, pos);
-        for (int h = warp; h < s.H; h += AP_WARPS) attn_head_norm(row + (int64_t)h * s.D, s.qn, s.D, s.dp, s.eps, mul, q + ((int64_t)m * s.H + h) * s.dp, lane);
+    const int at = attn_row(s, pos), items = q ? 2 * s.G + s.H : 2 * s.G;
+    // item i: key heads, value heads, queries
+    auto load = [&](int i, float4 (&x)[NV]) {
+        const bool value = i >= s.G && i < 2 * s.G;
+        const int width = value ? s.V : s.D;
+        const float *src = row + (i < s.G ? (int64_t)(s.H + i) * s.D : value ? (int64_t)(s.H + s.G) * s.D + (int64_t)(i - s.G) * s.V : (int64_t)(i - 2 * s.G) * s.D);
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            const int c = 128 * v + 4 * lane;
+            x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i >= items) continue;
+            if (WIDE) {
+                if (c < width) x[v] = __ldcg(reinterpret_cast<const float4 *>(src + c));
+            } else {
+                if (c < width) x[v].x = __ldcg(src + c);
+                if (c + 1 < width) x[v].y = __ldcg(src + c + 1);
+                if (c + 2 < width) x[v].z = __ldcg(src + c + 2);
+                if (c + 3 < width) x[v].w = __ldcg(src + c + 3);
+            }
+        }
+    };
+    float4 ahead[NV];
+    load(warp, ahead);
+    const float mul = attn_temperature(s, pos);
+    for (int i = warp; i < items; i += AP_WARPS) {
+        float x[NV][4];
+#pragma unroll
+        for (int v = 0; v < NV; v++) x[v][0] = ahead[v].x, x[v][1] = ahead[v].y, x[v][2] = ahead[v].z, x[v][3] = ahead[v].w;
+        load(i + AP_WARPS, ahead);
+        const bool key = i < s.G, query = i >= 2 * s.G;
+        const float *w = key ? s.kn : query ? s.qn : nullptr;
+        if (w) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; v++) ss += x[v][0] * x[v][0] + x[v][1] * x[v][1] + x[v][2] * x[v][2] + x[v][3] * x[v][3];
+            const float inv = __fdiv_rn(1.0f, sqrtf(__fdiv_rn(pg_warp_sum(ss), (float)s.D) + s.eps));
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int c = 128 * v + 4 * lane + e;
+                    if (c < s.D) x[v][e] *= inv * __ldg(w + c);
+                }
+        }
+        if (query) {
+            // f16 over a power of two of the row's own
+            float top = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[v][e] *= mul;
+                    top = fmaxf(top, fabsf(x[v][e]));
+                }
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+            float down, up;
+            four_range(top, down, up);
+            const int64_t to = (int64_t)m * s.H + i - 2 * s.G;
+            if (lane == 0) q_up[to] = up;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int c = 128 * v + 4 * lane;
+                if (c < s.dp)
+                    *reinterpret_cast<uint2 *>(q + to * s.dp + c) = make_uint2(four_pack_f16(x[v][0] * down, x[v][1] * down), four_pack_f16(x[v][2] * down, x[v][3] * down));
+            }
+            continue;
+        }
+        const int groups = key ? f.gk : f.gv;
+        unsigned char *tile = key ? kc + (slot * s.G + i) * f.kh + (int64_t)(at >> 4) * f.kb : vc + (slot * s.G + i - s.G) * f.vh + (int64_t)(at >> 4) * f.vb;
+        const int p = at & 15;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            // (magnitudes order as integers; not-a-numbers are the largest)
+            uint32_t most = 0;
+            float mine = x[v][0];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t mag = __float_as_uint(fabsf(x[v][e]));
+                if (mag > most) most = mag, mine = x[v][e];
+            }
+            const uint32_t own = most;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const uint32_t has = __ballot_sync(0xffffffffu, own == most) >> (lane & 24) & 255u;
+            const float scale = four_scale(__shfl_sync(0xffffffffu, mine, (lane & 24) + __ffs(has) - 1));
+            uint32_t n[4], all = 0;
+            four_quants(x[v], scale, n);
+#pragma unroll
+            for (int e = 0; e < 4; e++) all |= n[e] << (8 * e);
+            const uint32_t across = __shfl_xor_sync(0xffffffffu, all, 2);   // eight columns on (or back)
+            const int g = 4 * v + (lane >> 3), half = lane >> 2 & 1;
+            if (g < groups) {
+                if (key) {
+                    unsigned char *to = tile + g * 256 + (((p & 7) * 4 + (lane & 3)) * 2 + half) * 4 + (p >> 3);
+                    to[0] = (unsigned char)(n[0] | n[2] << 4);
+                    to[2] = (unsigned char)(n[1] | n[3] << 4);
+                } else {
+                    // columns r = 4 (lane & 1) + e of the first and the second eight in a byte: the lanes of the first write e = 0, 1
+                    const bool second = lane >> 1 & 1;
+                    const uint32_t both = second ? across | all << 4 : all | across << 4;
+                    const int e = second ? 2 : 0, r = 4 * (lane & 1) + e;
+                    unsigned char *to = tile + g * 256 + ((r * 4 + ((p & 7) >> 1)) * 2 + half) * 4 + 2 * (p & 1) + (p >> 3);
+                    to[0] = (unsigned char)(both >> (8 * e));
+                    to[32] = (unsigned char)(both >> (8 * e + 8));
+                }
+                if ((lane & 7) == 0) *reinterpret_cast<bf16 *>(tile + groups * 256 + (((p >> 1) * groups + g) * 2 + (p & 1)) * 2) = __float2bfloat16_rn(scale);
+            }
+        }
     }
 }
 
-// ---- unfold: grid (tiles of 16 positions, heads); values of a slot's rows [0, rows) as TA, zeros up to row `padded` -----------------
-template <typename TA, bool VALUES>
-__global__ void __launch_bounds__(128) attn4_unfold_kernel(const unsigned char *__restrict__ cache, int groups, int tile_bytes, int64_t head_bytes, int rows, int padded,
-                                                           int width, int64_t head_stride, TA *__restrict__ out)
+// ---- a cache as numbers -------------------------------------------------------------------------------------------------
+// quant of a tile: position p of 16, column c
+template <bool VALUES>
+__device__ __forceinline__ int quant_of(const unsigned char *tile, int p, int c)
+{
+    const int g = c >> 5, s = c >> 4 & 1;
+    if (VALUES) return tile[g * 256 + (((c & 7) * 4 + ((p & 7) >> 1)) * 2 + s) * 4 + 2 * (p & 1) + (p >> 3)] >> (4 * (c >> 3 & 1)) & 15;
+    return tile[g * 256 + (((p & 7) * 4 + (c >> 2 & 3)) * 2 + s) * 4 + 2 * (c & 1) + (p >> 3)] >> (4 * (c >> 1 & 1)) & 15;
+}
+__device__ __forceinline__ float scale_of(const unsigned char *tile, int groups, int p, int g)
+{
+    return __bfloat162float(*reinterpret_cast<const bf16 *>(tile + groups * 256 + (((p >> 1) * groups + g) * 2 + (p & 1)) * 2));
+}
+
+// grid (tiles, parts): f32 [parts][rows][32 groups]
+template <bool VALUES>
+__global__ void __launch_bounds__(128) attn4_read_kernel(const unsigned char *__restrict__ cache, int groups, int tile_bytes, int64_t head_bytes, int rows, float *__restrict__ out)
+{
+    pg_pdl_begin();
+    const unsigned char *tile = cache + (int64_t)blockIdx.y * head_bytes + (int64_t)blockIdx.x * tile_bytes;
+    const int first = (int)blockIdx.x * 16, width = groups * 32;
+    float *dst = out + ((int64_t)blockIdx.y * rows + first) * width;
+    for (int i = threadIdx.x; i < min(16, rows - first) * width; i += 128) {
+        const int p = i / width, c = i - p * width;
+        dst[i] = scale_of(tile, groups, p, c >> 5) * (float)(quant_of<VALUES>(tile, p, c) - 8);
+    }
+}
+
+// grid (ATTN_TOPS, G, keys and values): no value of a head's rows [0, rows) is larger than the largest of its tops.  (Scales that are not numbers
+// do not count: what lies beside them keeps its digits.)  Marks no row's values as bad.
+__global__ void __launch_bounds__(128) attn4_tops_kernel(const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc, const Four f, int rows, int bad,
+                                                         float *__restrict__ k_top, float *__restrict__ v_top, int *__restrict__ v_bad)
+{
+    __shared__ float tops[4];
+    pg_pdl_begin();
+    const bool values = blockIdx.z == 1;
+    const int groups = values ? f.gv : f.gk, bytes = values ? f.vb : f.kb, part = blockIdx.x, words = groups * 8, tiles = (rows + 15) / 16;
+    const unsigned char *head = values ? vc + blockIdx.y * f.vh : kc + blockIdx.y * f.kh;
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < (tiles - part + ATTN_TOPS - 1) / ATTN_TOPS * words; i += 128) {
+        const int tile = part + i / words * ATTN_TOPS, at = i % words, p = tile * 16 + at / groups * 2;
+        if (tile >= tiles) break;
+        const uint32_t two = __ldcg(reinterpret_cast<const uint32_t *>(head + (int64_t)tile * bytes + groups * 256) + at);
+        const float s0 = fabsf(pg_bf16_lo(two)), s1 = fabsf(pg_bf16_hi(two));
+        if (p < rows && isfinite(s0)) top = fmaxf(top, s0);
+        if (p + 1 < rows && isfinite(s1)) top = fmaxf(top, s1);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) (values ? v_top : k_top)[blockIdx.y * ATTN_TOPS + part] = 8.0f * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    if (values)
+        for (int i = part * 128 + threadIdx.x; i < bad; i += ATTN_TOPS * 128) v_bad[blockIdx.y * (int64_t)bad + i] = 0x7fffffff;
+}
+
+// grid (tiles of 16 positions, G, keys and values): rows [0, rows) of a slot in f16 over the head's power of two, zeros up to row `padded`.  A scale of
+// eight bits times a quant has eleven, so that f16 holds it as it is, down to 2^-29 of the head's largest.
+// 3000 positions of 8 heads of 128: 9.3 us, 12.3 MB written; the pass over the scales in front of it 4.5 us.
+__global__ void __launch_bounds__(128)
+    attn4_unfold_kernel(const AttnShape s, const Four f, const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc, int rows, int padded,
+                        __half *__restrict__ k, __half *__restrict__ v, int *__restrict__ v_bad)
 {
     __shared__ __align__(16) unsigned char tile[8 * 288];
+    __shared__ __align__(16) __half numbers[16][256 + 8];
     pg_pdl_begin();
-    const uint4 *src = reinterpret_cast<const uint4 *>(cache + (int64_t)blockIdx.y * head_bytes + (int64_t)blockIdx.x * tile_bytes);
-    for (int i = threadIdx.x; i < tile_bytes / 16; i += 128) reinterpret_cast<uint4 *>(tile)[i] = __ldcg(src + i);
+    const bool values = blockIdx.z == 1;
+    const int groups = values ? f.gv : f.gk, bytes = values ? f.vb : f.kb, width = values ? s.vp : s.dp, lane = threadIdx.x & 31;
+    const uint4 *src = reinterpret_cast<const uint4 *>((values ? vc + blockIdx.y * f.vh : kc + blockIdx.y * f.kh) + (int64_t)blockIdx.x * bytes);
+    for (int i = threadIdx.x; i < bytes / 16; i += 128) reinterpret_cast<uint4 *>(tile)[i] = __ldcg(src + i);
+    float down, up;
+    attn_range(values ? s.v_top : s.k_top, blockIdx.y, lane, down, up);
     __syncthreads();
-    const bf16 *scales = reinterpret_cast<const bf16 *>(tile + groups * 256);
-    const int fours = width / 4, first = (int)blockIdx.x * 16, left = min(16, padded - first);
-    TA *dst = out + (int64_t)blockIdx.y * head_stride + (int64_t)blockIdx.x * 16 * width;
-    for (int i = threadIdx.x; i < left * fours; i += 128) {
-        const int p = i / fours, c = (i - p * fours) * 4, g = c >> 5, s = c >> 4 & 1;
-        const float scale = __bfloat162float(scales[((p >> 1) * groups + g) * 2 + (p & 1)]);
+    const int first = (int)blockIdx.x * 16, left = min(16, padded - first);
+    const int r = lane >> 2, t = lane & 3;
+    for (int g = threadIdx.x >> 5; g < groups; g += 4) {
+        const uint2 two = *reinterpret_cast<const uint2 *>(tile + g * 256 + lane * 8);
+        const uint32_t w[2] = {two.x, two.y};
+        if (values) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            int q;
-            if (VALUES) {
-                const int col = (c + e) & 15, r = col & 7, n = col >> 3, i8 = p >> 3, t = (p & 7) >> 1, h = p & 1;
-                q = tile[g * 256 + ((r * 4 + t) * 2 + s) * 4 + 2 * h + i8] >> (4 * n) & 15;
-            } else {
-                const int t = (c & 15) >> 2, n = p >> 3, r = p & 7;
-                q = tile[g * 256 + ((r * 4 + t) * 2 + s) * 4 + 2 * (e & 1) + n] >> (4 * (e >> 1)) & 15;
+            for (int b = 0; b < 4; b++) {                 // byte 2 h + i
+                const int p = 8 * (b & 1) + 2 * t + (b >> 1);
+                float scale = scale_of(tile, groups, p, g);
+                if (!isfinite(scale)) {
+                    // a row that sees them has to say so, the others must not
+                    const int row = first + p, chunks = s.chunk ? s.cap / s.chunk : 1;
+                    if (r == 0 && row < rows) atomicMin(v_bad + (blockIdx.y * groups + g) * chunks + (s.chunk ? row / s.chunk : 0), row);
+                    scale = 0.0f;
+                }
+                scale = first + p < rows ? scale * down : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++) numbers[p][32 * g + 16 * e + 8 * n + r] = __float2half_rn(scale * (float)((int)(w[e] >> (8 * b + 4 * n) & 15u) - 8));
             }
-            pg_put(dst + (int64_t)p * width + c + e, first + p < rows ? scale * (float)(q - 8) : 0.0f);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const int p = 8 * n + r;
+                const float scale = first + p < rows ? scale_of(tile, groups, p, g) * down : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float x[4];                           // column 2 i + h: byte 2 h + n, half i
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] = first + p < rows ? scale * (float)((int)(w[e] >> (16 * (c & 1) + 8 * n + 4 * (c >> 1)) & 15u) - 8) : 0.0f;
+                    *reinterpret_cast<uint2 *>(&numbers[p][32 * g + 16 * e + 4 * t]) = make_uint2(four_pack_f16(x[0], x[1]), four_pack_f16(x[2], x[3]));
+                }
+            }
         }
+    }
+    __syncthreads();
+    __half *dst = (values ? v : k) + ((int64_t)blockIdx.y * s.cap + first) * width;
+    const int eights = width / 8;
+    for (int i = threadIdx.x; i < left * eights; i += 128) {
+        const int p = i / eights, c = (i - p * eights) * 8;
+        *reinterpret_cast<uint4 *>(dst + (int64_t)p * width + c) = *reinterpret_cast<const uint4 *>(&numbers[p][c]);
     }
 }
 
@@ -615,7 +797,9 @@ PG_API int64_t pg_attention4_tickets(pg_ctx *ctx) { return ctx ? (int64_t)2 * ct
 
 PG_API int64_t pg_attention4_unfold_bytes(const pg_attention *p)
 {
-    return p && p->kv_heads > 0 && p->cap > 0 ? (int64_t)p->kv_heads * p->cap * (pg_up(p->dim, 16) + pg_up(p->vdim, 16)) * 2 : 0;
+    if (!p || p->kv_heads <= 0 || p->cap <= 0 || p->chunk < 0) return 0;
+    const int64_t chunks = p->chunk ? std::max(1, p->cap / p->chunk) : 1;
+    return (int64_t)p->kv_heads * ((int64_t)p->cap * (pg_up(p->dim, 16) + pg_up(p->vdim, 16)) * 2 + 2 * ATTN_TOPS * 4 + pg_up(p->vdim, 32) / 32 * chunks * 4);
 }
 
 PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t few, int64_t short_rows, int64_t short_len, const float *d_proj,
@@ -634,8 +818,12 @@ PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_ba
     unsigned char *kc = (unsigned char *)d_kcache, *vc = (unsigned char *)d_vcache;
     const bool fused = batch->max_len == 1 && few >= 1;
     if (!fused) {
-        const int32_t ra = launch_pdl(ctx, attn4_append_kernel, dim3((unsigned)batch->rows), dim3(AP_WARPS * 32), 0, s, f, *batch, d_proj, ldp,
-                                      short_rows < batch->rows ? (bf16 *)p->d_q : (bf16 *)nullptr, kc, vc, ctx->d_status);
+        __half *q = short_rows < batch->rows ? (__half *)p->d_q : nullptr;
+        float *q_up = (float *)((__half *)p->d_q + (int64_t)batch->rows * s.H * s.dp);
+        const bool wide = s.D % 4 == 0 && s.V % 4 == 0 && ldp % 4 == 0 && ((uintptr_t)d_proj & 15) == 0;
+        auto append = s.D <= 128 && s.V <= 128 ? (wide ? attn4_append_kernel<1, true> : attn4_append_kernel<1, false>)
+                                               : (wide ? attn4_append_kernel<2, true> : attn4_append_kernel<2, false>);
+        const int32_t ra = launch_pdl(ctx, append, dim3((unsigned)batch->rows), dim3(AP_WARPS * 32), 0, s, f, *batch, d_proj, ldp, q, q_up, kc, vc, ctx->d_status);
         if (ra != PG_OK || short_rows == 0) return ra;
     }
     const int64_t cols = (fused ? 1 : short_len) * s.rep;
@@ -668,20 +856,23 @@ PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg
     PG_ENTER(ctx);
     const int32_t rc = check(p, batch, d_kcache, d_vcache, d_out, dtype, ldo);
     if (rc != PG_OK) return rc;
-    const AttnShape s = pgk_attention_shape(p);
+    AttnShape s = pgk_attention_shape(p);
     const Four f = four_of(s);
+    PG_REQUIRE(((uintptr_t)p->d_q & 15) == 0, "attention4: queries on no 16-byte boundary");
     PG_REQUIRE(d_work && ((uintptr_t)d_work & 127) == 0, "attention4: no workspace, or not on a 128-byte boundary");
     PG_REQUIRE(seq >= 0 && seq < batch->seqs && len > 0 && len <= batch->max_len && positions >= len && positions <= s.limit && slot >= 0 && slot < p->slots,
                "attention4: sequence %lld with %lld tokens and %lld positions in slot %lld", (long long)seq, (long long)len, (long long)positions, (long long)slot);
     // the slot's rows that hold something, in the order that they have there
     const int rows = (int)std::min<int64_t>(positions, s.cap), padded = (int)std::min<int64_t>(rows + 128, s.cap);   // (a tile of keys may end behind them)
-    bf16 *k = (bf16 *)d_work, *v = k + (int64_t)s.G * s.cap * s.dp;
-    const dim3 grid((unsigned)((padded + 15) / 16), (unsigned)s.G);
-    int32_t ru = launch_pdl(ctx, attn4_unfold_kernel<bf16, false>, grid, dim3(128), 0, (const unsigned char *)d_kcache + slot * s.G * f.kh, f.gk, f.kb, f.kh, rows, padded,
-                            s.dp, (int64_t)s.cap * s.dp, k);
+    __half *k = (__half *)d_work, *v = k + (int64_t)s.G * s.cap * s.dp;
+    float *k_top = (float *)(v + (int64_t)s.G * s.cap * s.vp), *v_top = k_top + s.G * ATTN_TOPS;
+    int *v_bad = (int *)(v_top + s.G * ATTN_TOPS);
+    const int bad = f.gv * (s.chunk ? s.cap / s.chunk : 1);
+    s.q_up = (const float *)((const __half *)p->d_q + (int64_t)batch->rows * s.H * s.dp), s.k_top = k_top, s.v_top = v_top, s.v_bad = v_bad;
+    const unsigned char *kc = (const unsigned char *)d_kcache + slot * s.G * f.kh, *vc = (const unsigned char *)d_vcache + slot * s.G * f.vh;
+    int32_t ru = launch_pdl(ctx, attn4_tops_kernel, dim3(ATTN_TOPS, (unsigned)s.G, 2), dim3(128), 0, kc, vc, f, rows, bad, k_top, v_top, v_bad);
     if (ru == PG_OK)
-        ru = launch_pdl(ctx, attn4_unfold_kernel<bf16, true>, grid, dim3(128), 0, (const unsigned char *)d_vcache + slot * s.G * f.vh, f.gv, f.vb, f.vh, rows, padded,
-                        s.vp, (int64_t)s.cap * s.vp, v);
+        ru = launch_pdl(ctx, attn4_unfold_kernel, dim3((unsigned)((padded + 15) / 16), (unsigned)s.G, 2), dim3(128), 0, s, f, kc, vc, rows, padded, k, v, v_bad);
     if (ru != PG_OK) return ru;
     // the sequence as a batch of its own, its cache in slot 0 (the last ticket is always zero)
     pg_batch one = *batch;
@@ -690,8 +881,9 @@ PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg
     one.d_seq_row0 += seq;
     one.d_seq_slot = p->d_tickets + 2 * ctx->sm_count;
     bf16 *out = (bf16 *)d_out;
-    if (pgk_attention_prompt_tc_supports(s, &one, 1, ldo, out)) return pgk_attention_prompt_tc(ctx, s, &one, 1, (const bf16 *)p->d_q, k, v, out, ldo);
-    return pgk_attention_prompt(ctx, s, &one, (const bf16 *)p->d_q, k, v, out, ldo);
+    const bf16 *q = (const bf16 *)p->d_q, *kh = (const bf16 *)k, *vh = (const bf16 *)v;   // (f16, which s says)
+    if (pgk_attention_prompt_tc_supports(s, &one, 1, ldo, out)) return pgk_attention_prompt_tc(ctx, s, &one, 1, q, kh, vh, out, ldo);
+    return pgk_attention_prompt(ctx, s, &one, q, kh, vh, out, ldo);
 }
 
 PG_API int32_t pg_cache4_read(pg_ctx *ctx, const void *d_cache, int32_t values, int32_t width, int64_t cap, int64_t parts, int64_t rows, float *d_out)
@@ -702,11 +894,8 @@ PG_API int32_t pg_cache4_read(pg_ctx *ctx, const void *d_cache, int32_t values, 
     const int w = (int)pg_up(width, 32), tile = (int)pg_cache4_tile_bytes(w);
     const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)parts);
     const int64_t head = pg_up(cap, 16) / 16 * tile;
-    if (values)
-        return launch_whole(ctx, attn4_unfold_kernel<float, true>, grid, dim3(128), 0, (const unsigned char *)d_cache, w / 32, tile, head, (int)rows, (int)rows, w, rows * w,
-                            d_out);
-    return launch_whole(ctx, attn4_unfold_kernel<float, false>, grid, dim3(128), 0, (const unsigned char *)d_cache, w / 32, tile, head, (int)rows, (int)rows, w, rows * w,
-                            d_out);
+    auto kern = values ? attn4_read_kernel<true> : attn4_read_kernel<false>;
+    return launch_whole(ctx, kern, grid, dim3(128), 0, (const unsigned char *)d_cache, w / 32, tile, head, (int)rows, d_out);
 }
 
 }  // extern "C"

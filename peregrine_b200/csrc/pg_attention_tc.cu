@@ -45,7 +45,8 @@ struct SplitArgs {
 };
 
 // BIAS: a distance bias and / or chunks; SPLIT: AttnSplitKeys
-template <int DK, int DV, bool BIAS, bool SPLIT>
+// HALF: f16 queries, keys, values and probabilities in bf16's place (AttnShape)
+template <int DK, int DV, bool BIAS, bool SPLIT, bool HALF>
 __global__ void __launch_bounds__(AT_THREADS, 1)
     attn_prompt_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                           const __grid_constant__ CUtensorMap map_s, const AttnShape s, const pg_batch bt, const SplitArgs sp, bf16 *__restrict__ out,
@@ -144,7 +145,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         // ---------------------------------------------------------------- MMA issuer (the whole warp; one lane's products count)
         if (most > 0) {
             const uint32_t on = pg_elect();
-            constexpr uint32_t idesc_s = make_idesc(TQ, TKEYS), idesc_o = make_idesc(TQ, DV) | IDESC_B_MN_MAJOR;
+            constexpr uint32_t types = HALF ? (1u << 7) | (1u << 10) : 0u;   // (the bits of bf16 operands)
+            constexpr uint32_t idesc_s = make_idesc(TQ, TKEYS) & ~types, idesc_o = (make_idesc(TQ, DV) & ~types) | IDESC_B_MN_MAJOR;
             int at = 0, phase = 0;
             auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, pg_mbar_wait(bar, parity, abort_flag, status, limit_ns)); };
             auto wait_full = [&]() { return wait(bar_full + 8 * at, phase); };
@@ -213,7 +215,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         const int rr = rr0 + t * TQ + q * 32 + lane, rc = min(rr, total - 1);
         const int lim = pos0 + rc / s.rep;              // last key of this row
         const uint32_t ts = tmem + ((uint32_t)(q * 32) << 16) + t * 128, to = ts + 256;
-        const float sl = s.scale * LOG2E, sx = BIAS ? 1.0f : sl;   // (with a bias the scores are scaled before the maximum)
+        float sl = s.scale * LOG2E, v_up = 1.0f;
+        if (HALF) {
+            float down, up;
+            attn_range(s.k_top, g, lane, down, up);
+            attn_range(s.v_top, g, lane, down, v_up);
+            if (total > 0) sl *= up * __ldcg(s.q_up + (int64_t)(row0 + rc / s.rep) * s.H + g * s.rep + rc % s.rep);
+        }
+        const float sx = BIAS ? 1.0f : sl;              // (with a bias the scores are scaled before the maximum)
         const float bias = BIAS && s.slopes ? __ldg(s.slopes + g * s.rep + rc % s.rep) * LOG2E : 0.0f;
         float m = 0.0f, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;
@@ -250,7 +259,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 for (int i = 0; i < 32; i++) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[c][i]));
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sx;
             if (j == 0) {
-                m = fmaxf(top, s.sink ? 0.0f : -1e30f); // (finite also where the row sees nothing of the first tile)
+                // finite also where the row sees nothing of the first tile; f16 holds probabilities of the row's own maximum only
+                m = fmaxf(top, s.sink && !HALF ? 0.0f : -1e30f);
             } else {
                 const bool behind = top > m + 8.0f;
                 if (__any_sync(0xffffffffu, behind)) {
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     const float a = pg_ex2(fmaf(__uint_as_float(v[c][e]), sx, -m)), b = pg_ex2(fmaf(__uint_as_float(v[c][e + 1]), sx, -m));
                     l0 += a;
                     l1 += b;
-                    p[i] = pg_pack_bf16(a, b);
+                    p[i] = attn_pack<HALF>(a, b);
                 }
                 tmem_st32(ts + h * 32, p);
             }
@@ -294,7 +304,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             tc_fence_after();
             float l = l0 + l1;
             if (s.sink) l += pg_ex2(-m);
-            const float inv = __fdiv_rn(1.0f, l);
+            const float inv = __fdiv_rn(1.0f, l) * v_up;
             const int head_at = (g * s.rep + rc % s.rep) * s.V;
             bf16 *dst = out + (int64_t)(row0 + rc / s.rep) * ldo + head_at;
             const float *gate = SPLIT ? sp.gate + (int64_t)(row0 + rc / s.rep) * sp.ldg + head_at : nullptr;
@@ -304,9 +314,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 uint32_t o[32];
                 tmem_ld32(to + c, o);
                 if (!ok || rr >= total) continue;
+                const float by = HALF && c < s.V && attn_sees_bad(s, g, c, lim) ? __uint_as_float(0x7fc00000u) : inv;
 #pragma unroll
                 for (int i = 0; i < 32; i++) {
-                    float y = __uint_as_float(o[i]) * inv;
+                    float y = __uint_as_float(o[i]) * by;
                     if (SPLIT && c + i < s.V) y *= pg_sigmoid(__ldcg(gate + c + i));
                     o[i] = __float_as_uint(y);
                 }
@@ -346,12 +357,12 @@ int32_t map3(CUtensorMap *map, const bf16 *p, int64_t cols, int64_t rows, int64_
     return pg_encode_bf16(map, p, 3, dims, strides, box);
 }
 
-template <int DK, int DV, bool BIAS, bool SPLIT>
+template <int DK, int DV, bool BIAS, bool SPLIT, bool HALF>
 int32_t launch(pg_ctx *ctx, const CUtensorMap (&maps)[4], const AttnShape &s, const pg_batch *bt, const SplitArgs &sp, int64_t len, int64_t seqs, bf16 *out,
                int64_t ldo)
 {
     using C = AtCfg<DK, DV>;
-    auto kern = attn_prompt_tc_kernel<DK, DV, BIAS, SPLIT>;
+    auto kern = attn_prompt_tc_kernel<DK, DV, BIAS, SPLIT, HALF>;
     static std::atomic<uint64_t> set{0};
     PG_CUDA(pg_max_smem_once(kern, C::SMEM, ctx->device, set));
     const int64_t tiles = (len * s.rep + 2 * TQ - 1) / (2 * TQ);
@@ -370,8 +381,12 @@ int32_t run(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, int64_t slots, 
     if (rc != PG_OK) return rc;
     maps[3] = maps[2];
     const SplitArgs none = {};
-    if (s.slopes || s.chunk) return launch<DK, DV, true, false>(ctx, maps, s, bt, none, bt->max_len, bt->seqs, out, ldo);
-    return launch<DK, DV, false, false>(ctx, maps, s, bt, none, bt->max_len, bt->seqs, out, ldo);
+    const bool bias = s.slopes || s.chunk;
+    if (s.q_up)
+        return bias ? launch<DK, DV, true, false, true>(ctx, maps, s, bt, none, bt->max_len, bt->seqs, out, ldo)
+                    : launch<DK, DV, false, false, true>(ctx, maps, s, bt, none, bt->max_len, bt->seqs, out, ldo);
+    return bias ? launch<DK, DV, true, false, false>(ctx, maps, s, bt, none, bt->max_len, bt->seqs, out, ldo)
+                : launch<DK, DV, false, false, false>(ctx, maps, s, bt, none, bt->max_len, bt->seqs, out, ldo);
 }
 
 template <int DK, int DV>
@@ -385,7 +400,7 @@ int32_t run_split(pg_ctx *ctx, const AttnShape &s, const pg_batch *bt, const Att
     if (rc == PG_OK) rc = map3(&maps[3], k.shared, k.sd, k.positions, k.lds, 1, k.positions * k.lds, TKEYS, 1);
     if (rc != PG_OK) return rc;
     const SplitArgs sp = {k.seq, (k.kd + 63) / 64, k.gate, k.ldg};
-    return launch<DK, DV, false, true>(ctx, maps, s, bt, sp, k.len, 1, out, ldo);
+    return launch<DK, DV, false, true, false>(ctx, maps, s, bt, sp, k.len, 1, out, ldo);
 }
 
 }  // namespace

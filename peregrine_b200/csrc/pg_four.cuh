@@ -31,11 +31,28 @@ size_t pgk_linear4_tc_workspace(const pg_ctx *ctx);
 
 #ifdef __CUDACC__
 // scale and quant of a value, with the group's value of largest magnitude
-__device__ __forceinline__ float four_scale(float top) { return isfinite(top) ? __bfloat162float(__float2bfloat16_rn(__fdiv_rn(top, -8.0f))) : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ float four_scale(float top) { return isfinite(top) ? __bfloat162float(__float2bfloat16_rn(top * -0.125f)) : __uint_as_float(0x7fc00000u); }
 __device__ __forceinline__ uint32_t four_quant(float w, float scale)
 {
     if (!(scale != 0.0f) || !isfinite(scale)) return 8u;   // (a zero scale stands for zeros whatever the quants)
     return (uint32_t)min(15, max(0, __float2int_rn(__fdiv_rn(w, scale)) + 8));
+}
+// The same for four values, with a product in place of the quotients: that is off by 2^-18 at most where the scale is in the middle of its range
+// (reciprocal 2 units in the last place, product half a one, quotients of up to 8), so what it rounds to is the quotient's integer unless it lies
+// within 2^-17 of a half.
+__device__ __forceinline__ void four_quants(const float (&w)[4], float scale, uint32_t (&q)[4])
+{
+    const float inv = __fdividef(1.0f, scale), mag = fabsf(scale);
+    bool plain = mag >= 1e-30f && mag <= 1e30f;            // (false for not-a-number)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float x = w[e] * inv, n = rintf(x);
+        plain = plain && fabsf(fabsf(x - n) - 0.5f) > 0x1p-17f;
+        q[e] = (uint32_t)min(15, (int)n + 8);              // (the largest is -8 steps of the scale; bf16's rounding of that adds less than a half)
+    }
+    if (plain) return;
+#pragma unroll
+    for (int e = 0; e < 4; e++) q[e] = four_quant(w[e], scale);
 }
 
 // ---- quants -> f16 pairs: bits 0-3 / 4-7 of both halves of a word, as q - 8 and 16 (q - 8), exact.  1024 + q and 1024 + 16 q are f16 numbers

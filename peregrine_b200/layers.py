@@ -298,7 +298,7 @@ class Attention4Plan:
         # sequences of up to so many tokens in a step read the cache as it is: four blocks of 16 (token, head) rows
         self.few = 1 if chunk else max(1, 64 * kv_heads // heads)
         t = d.torch
-        self.q_cols = heads * up(dim, 16)
+        self.q_cols = heads * (up(dim, 16) + 2)   # (and a f32 factor of every query)
         d.buffer("attn.q", self.q_cols)
         d.buffer("attn4.part", 1, max(1, d.lib.pg_attention4_part_floats(d.gpu.handle, C.byref(self.c))), t.float32)
         d.buffer("attn4.tickets", 1, d.lib.pg_attention4_tickets(d.gpu.handle), t.int32)

@@ -102,15 +102,16 @@ class Case:
     def held(self):
         return self.plan.values(self.kc, self.cap, False).double().cpu().numpy(), self.plan.values(self.vc, self.cap, True).double().cpu().numpy()
 
-    def want(self, entries, proj):
-        """The formula over what the cache holds now, and the bounds of its outputs."""
+    def want(self, entries, proj, half=False):
+        """The formula over what the cache holds now, and the bounds of its outputs.  half: longer portions as they are computed, in f16: queries and
+        probabilities are off by half a step, 2^-11, keys and values not at all; a probability below 2^-14 of its row's largest by 2^-25 of that."""
         K, Vv = self.held()
         kw, H, G, D, V = self.kw, self.H, self.G, self.D, self.V
         chunk, sink = kw.get("chunk", 0), kw.get("sink", False)
         out, bound = np.zeros((len(proj), H, V)), np.zeros((len(proj), H, V))
         at = 0
         for slot, pos0, n in entries:
-            few = n <= self.plan.few
+            few = n <= self.plan.few or half
             for i in range(n):
                 pos = pos0 + i
                 q = proj[at, :H * D].astype(np.float64).reshape(H, D)
@@ -136,7 +137,9 @@ class Case:
                     out[at, h] = p @ v / l
                     A = p @ np.abs(v) / l
                     e = math.expm1(2 * ds)
-                    b = A * (e + (2.0 ** -8 if few else 2 * 2.0 ** -8) * (1 + e) + 2.0 ** -17)
+                    b = A * (e + (2.0 ** -11 if half else 2.0 ** -8 if few else 2 * 2.0 ** -8) * (1 + e) + 2.0 ** -17)
+                    if half:
+                        b = b + 2.0 ** -24 * np.abs(v).sum(0) * (1 + e)
                     bound[at, h] = b + 2.0 ** -8 * (np.abs(out[at, h]) + b)
                 at += 1
         return out.reshape(len(proj), -1), bound.reshape(len(proj), -1)
@@ -244,6 +247,50 @@ def test_longer_portions(lm, H, G, D, V):
     # longer and shorter ones and single tokens in one step
     c.run_and_check([(3, 499, 1), (1, 33, max(n, 130)), (2, 100, 1)])
     c.run_and_check([(2, 101, n), (0, max(n, 150), min(2, c.plan.few))])
+
+
+@pytest.mark.parametrize("H,G,D,V", SHAPES)
+@pytest.mark.parametrize("sink", [False, True])
+def test_longer_portions_keep_their_digits(lm, H, G, D, V, sink):
+    """Scores of a wide range, keys and values of positions (and a head's from another's) that are thousands of times larger than the rest."""
+    c = Case(lm, H * D + V + 1, H, G, D, V, 300, 2, 400, sink=sink)
+    before = c.rows(60)
+    before[17, H * D:] *= 3000.0
+    before[40] *= 1e-3
+    c.append(1, 0, before)
+    n = max(c.plan.few + 1, 140)
+    proj = c.rows(2 * n)
+    proj[:, :H * D] *= 4.0
+    proj[:, H * D:H * D + D] *= 1e-6
+    proj[5], proj[7] = 0.0, proj[7] * 1e-12
+    entries = [(1, 60, n), (0, 0, n)]
+    got = c.step(entries, proj)
+    want, bound = c.want(entries, proj, half=True)
+    got = got.reshape(want.shape)
+    assert np.isfinite(got).all()
+    worst = np.abs(got - want) / np.maximum(bound, 1e-300)
+    assert worst.max() <= 1, f"{worst.max():.3g} times the bound at {np.unravel_index(worst.argmax(), worst.shape)}"
+
+
+@pytest.mark.parametrize("kw,D,V", [({}, 64, 96), ({}, 160, 64), ({"chunk": 50, "positions": 300}, 64, 96), ({"chunk": 40, "positions": 240}, 64, 256)])
+def test_longer_portions_beside_what_is_not_finite(lm, kw, D, V):
+    """Values (32 columns) and keys that are not numbers are seen by the rows that see their positions, and by no others."""
+    H, G, n = 4, 2, 170
+    cap = kw["chunk"] * -(-300 // kw["chunk"]) if kw else 300
+    c = Case(lm, 12, H, G, D, V, cap, 2, 400, **kw)
+    c.append(1, 0, c.rows(20))
+    proj = c.rows(n)
+    for at, what in ((30, np.inf), (90, np.nan), (133, -np.inf)):
+        proj[at, (H + G) * D + 40] = what                                 # head 0's value, columns 32 .. 63
+    proj[120, H * D + D + 3] = np.nan                                     # head 1's key
+    got = c.step([(1, 20, n)], proj).reshape(n, H, V)
+    bad = np.isnan(got)
+    pos, chunk = 20 + np.arange(n), kw.get("chunk", 1 << 30)
+    sees = lambda at: (pos >= 20 + at) & (pos // chunk == (20 + at) // chunk)
+    value = sees(30) | sees(90) | sees(133)
+    assert (bad[:, :2, 32:64] == value[:, None, None]).all()
+    assert not bad[:, :2, :32].any() and not bad[:, :2, 64:].any()
+    assert (bad[:, 2:] == sees(120)[:, None, None]).all()
 
 
 @pytest.mark.parametrize("kw", [{"sink": True}, {"slopes": True}, {"norms": True}, {"temp": (0.3, 40.0)}, {"sink": True, "slopes": True, "norms": True, "temp": (0.1, 7.0)}])
