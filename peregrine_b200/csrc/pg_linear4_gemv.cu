@@ -45,13 +45,16 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     const uint32_t cell_full = pg_smem(tail) + V4_WARPS * V4_SLOTS_MAX * 8 + (uint32_t)slot_idx * (V4_CELLS * 16), cell_free = cell_full + V4_CELLS * 8;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + V4_WARPS * V4_SLOTS_MAX * 8 + V4_WARPS * V4_CELLS * 16);
     const uint32_t ring = pg_smem(smem) + (uint32_t)(warp * v4_ring(NT));
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < V4_WARPS * V4_SLOTS_MAX; i++) pg_mbar_init(pg_smem(tail) + 8 * i, 1);
-        for (int i = 0; i < groups * V4_CELLS * 2; i++)
-            pg_mbar_init(pg_smem(tail) + V4_WARPS * V4_SLOTS_MAX * 8 + 8 * i, i / V4_CELLS % 2 ? 1 : max(1, kw - 1));   // the parts are there; they have been added
-        *abort_flag = 0;
+    if (threadIdx.x == 0) *abort_flag = 0;
+    if (threadIdx.x < V4_WARPS * V4_SLOTS_MAX) {
+        pg_mbar_init(pg_smem(tail) + 8 * threadIdx.x, 1);
+        pg_mbar_fence();
+    } else if (threadIdx.x < V4_WARPS * V4_SLOTS_MAX + groups * V4_CELLS * 2) {
+        const int i = threadIdx.x - V4_WARPS * V4_SLOTS_MAX;   // the parts are there; they have been added
+        pg_mbar_init(pg_smem(tail) + 8 * threadIdx.x, i / V4_CELLS % 2 ? 1 : max(1, kw - 1));
         pg_mbar_fence();
     }
+    static_assert(V4_WARPS * (V4_SLOTS_MAX + V4_CELLS * 2) <= V4_THREADS, "a thread per barrier");
     __syncthreads();
 
     const int ka0 = my_part * KH, k0 = ka0 + kpart * KW;
