@@ -336,20 +336,36 @@ __global__ void __launch_bounds__(128)
     }
 }
 
+// D[16 x 8] = C + A[16 x 16] B[16 x 8], f16 operands; C has one number for rows r and one for rows r + 8
+__device__ __forceinline__ void mma_from(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // ---- few tokens: grid (slices, G * blocks of 16 rows, seqs) --------------------------------------------------------------------
 constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // most fills in flight of a warp; tiles of a fill
 
 // part [(seq, block)][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row
-template <int GK, int GV, bool HI, bool FUSED>
+// EXACT: GK and GV are the groups of the layer, else at least as many
+template <int GK, int GV, bool HI, bool FUSED, bool EXACT>
 __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
     attn4_few_kernel(const AttnShape s, const Four f, const pg_batch bt, int few, int stages, const float *__restrict__ proj, int64_t ldp, unsigned char *kc, unsigned char *vc,
                      float *part, int32_t *tickets, bf16 *__restrict__ out, int64_t ldo, int32_t *status, unsigned long long limit_ns)
 {
-    constexpr int NT = HI ? 2 : 1;
+    constexpr int NT = HI ? 2 : 1, JT = HI ? 1 : 2;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t bars[A4_WARPS * A4_STAGES];
     __shared__ float weight[16][A4_SLICES];
     __shared__ float denom[16], back[16];
+    __shared__ __align__(16) float offset[16][8];
     __shared__ int last_in;
     __shared__ volatile int abort_flag;
     __shared__ uint8_t new_q[2][256];
@@ -357,7 +373,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int split = blockIdx.x, S = gridDim.x, g = blockIdx.y % s.G, block = blockIdx.y / s.G, seq = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-    const int gk = f.gk, gv = f.gv, stage = A4_FILL * (f.kb + f.vb), vs = gv * 32;
+    const int gk = EXACT ? GK : f.gk, gv = EXACT ? GV : f.gv, kbytes = gk * 288, vbytes = gv * 288, stage = A4_FILL * (kbytes + vbytes), vs = gv * 32;
     const uint32_t ring = pg_smem(smem) + (uint32_t)(warp * stages) * stage, bar = pg_smem(bars) + (uint32_t)warp * A4_STAGES * 8;
     const int qs = gk * 32 + 8;                                       // f16 elements between the rows of queries
     __half *qrow = reinterpret_cast<__half *>(smem + A4_WARPS * stages * stage);
@@ -393,9 +409,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
         if (lane == 0) {
             const uint32_t at = ring + (uint32_t)(to) * stage, on = bar + (uint32_t)(to) * 8;
             const int tile = (t0 >> 4) + A4_FILL * (warp + A4_WARPS * i), n = min(A4_FILL, tiles - tile);
-            pg_mbar_expect(on, (uint32_t)(n * (f.kb + f.vb)));
-            pg_bulk_load(at, kb + (int64_t)tile * f.kb, (uint32_t)(n * f.kb), on);
-            pg_bulk_load(at + A4_FILL * f.kb, vb + (int64_t)tile * f.vb, (uint32_t)(n * f.vb), on);
+            pg_mbar_expect(on, (uint32_t)(n * (kbytes + vbytes)));
+            pg_bulk_load(at, kb + (int64_t)tile * kbytes, (uint32_t)(n * kbytes), on);
+            pg_bulk_load(at + A4_FILL * kbytes, vb + (int64_t)tile * vbytes, (uint32_t)(n * vbytes), on);
         }
     };
     for (int i = 0; i < stages && i < mine; i++) fetch(i, i);
@@ -419,12 +435,18 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
             four_range(top, down, up);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (i < gk) qrow[c * qs + 32 * i + lane] = __float2half_rn(x[i] * down);
+                if (i < gk) {
+                    const __half v = __float2half_rn(x[i] * down);
+                    qrow[c * qs + 32 * i + lane] = v;
+                    const float sum = pg_warp_sum(__half2float(v));
+                    if (lane == 0) offset[c][i] = sum * -0x1p-21f;   // (the keys' quants are 8 too large)
+                }
             if (lane == 0) back[c] = up * sl;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (i < gk) qrow[c * qs + 32 * i + lane] = __float2half_rn(0.0f);
+            if (lane < 8) offset[c][lane] = 0.0f;
             if (lane == 0) back[c] = 0.0f;
         }
     }
@@ -441,9 +463,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
         // appended for later steps; this step takes it from shared memory (below)
         const int at = x1 - 1;
         if (warp == A4_WARPS - 2)
-            put_key(kb + (int64_t)(at >> 4) * f.kb, new_q[0], new_s[0], at & 15, gk, lane);
+            put_key(kb + (int64_t)(at >> 4) * kbytes, new_q[0], new_s[0], at & 15, gk, lane);
         else
-            put_value(vb + (int64_t)(at >> 4) * f.vb, new_q[1], new_s[1], at & 15, gv, lane);
+            put_value(vb + (int64_t)(at >> 4) * vbytes, new_q[1], new_s[1], at & 15, gv, lane);
     }
     uint32_t qf[GK][2][HI ? 4 : 2];
 #pragma unroll
@@ -465,17 +487,18 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
             }
         }
     }
-    float o[GV][2][NT][4];
+    float o[GV][2][NT][4], l[NT][4];
 #pragma unroll
-    for (int i = 0; i < GV; i++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 2; e++)
+        for (int j = 0; j < 4; j++) {
+            l[n][j] = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[i][e][n][j] = 0.0f;
+            for (int i = 0; i < GV; i++) o[i][0][n][j] = o[i][1][n][j] = 0.0f;
+        }
+    constexpr uint32_t ONES = 0x3f803f80u;                // two bf16 ones
     // of the lane's rows r (and r + 8): factor of the scores, last row of the cache seen, slope
-    float fac[NT], m[NT], l[NT], bias[NT];
+    float fac[NT], m[NT], bias[NT];
     int seen[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -483,7 +506,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
         fac[n] = back[c];
         seen[n] = x0 + pos0 + idx / s.rep - low;
         bias[n] = s.slopes ? __ldg(s.slopes + g * s.rep + idx % s.rep) * LOG2E : 0.0f;
-        m[n] = -1e30f, l[n] = 0.0f;                       // (finite: exp2(-inf - m) is 0 where a row sees nothing of a slice)
+        m[n] = -1e30f;                                    // (finite: exp2(-inf - m) is 0 where a row sees nothing of a slice)
     }
     const int sees_all = x0 + pos0 + block * 16 / s.rep - low;        // of the block's first row: every row sees that far
     bool ok = true;
@@ -497,110 +520,128 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
         if (newest && j0 + 32 >= x1) {
             // the copies brought what the cache held at the newest position: put the new one in its place
             const int row = x1 - 1 - j0;
-            put_key(at + (row >> 4) * f.kb, new_q[0], new_s[0], row & 15, gk, lane);
-            put_value(at + A4_FILL * f.kb + (row >> 4) * f.vb, new_q[1], new_s[1], row & 15, gv, lane);
+            put_key(at + (row >> 4) * kbytes, new_q[0], new_s[0], row & 15, gk, lane);
+            put_value(at + A4_FILL * kbytes + (row >> 4) * vbytes, new_q[1], new_s[1], row & 15, gv, lane);
             __syncwarp();
         }
         const bool edge = j0 < x0 || j0 + 31 > sees_all || j0 + 31 >= t1;   // some row does not see all of these
 #pragma unroll
-        for (int h = 0; h < A4_FILL; h++) {
-            const int jt = j0 + 16 * h;
-            if (jt >= t1) break;                                      // (uniform)
-            const uint32_t kt = pg_smem(at) + (uint32_t)(h * f.kb), vt = pg_smem(at) + (uint32_t)(A4_FILL * f.kb + h * f.vb);
-            // scores of keys 8 n + 2 t and 8 n + 2 t + 1 with rows r and r + 8
-            float sc[2][4] = {};
+        for (int part = 0; part < A4_FILL; part += JT) {  // as many tiles at once as registers allow
+            const int jp = j0 + 16 * part;
+            if (jp >= t1) break;                              // (uniform)
+                // scores of keys 16 h + 8 n + 2 t and 16 h + 8 n + 2 t + 1 with rows r and r + 8.  A quant as the low bits of an f16 number is that number of
+            // its smallest steps, 2^-24; the sums start at what 8 of them in every column make.
+            float sc[JT][2][2 * NT];
 #pragma unroll
-            for (int x = 0; x < GK; x++) {
-                if (x >= gk) break;
-                float d[2][4] = {};
-                uint32_t w[2];
-                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(kt + x * 256 + lane * 8));
+            for (int h = 0; h < JT; h++) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t w8 = w[e] >> 8;
-                    four_mma_f16(d[0], qf[x][e][0], HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, qf[x][e][1], HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u, four_f16_lo(w[e]), four_f16_hi(w[e]));
-                    four_mma_f16(d[1], qf[x][e][0], HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, qf[x][e][1], HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u, four_f16_lo(w8), four_f16_hi(w8));
-                }
+                for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    uint32_t two;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(kt + (uint32_t)(gk * 256 + ((4 * n + t) * gk + x) * 4)));
-                    const float s0 = pg_bf16_lo(two), s1 = pg_bf16_hi(two);
-                    sc[n][0] = fmaf(s0, d[n][0], sc[n][0]), sc[n][1] = fmaf(s1, d[n][1], sc[n][1]);
-                    if (HI) sc[n][2] = fmaf(s0, d[n][2], sc[n][2]), sc[n][3] = fmaf(s1, d[n][3], sc[n][3]);
+                    for (int j = 0; j < 2 * NT; j++) sc[h][n][j] = 0.0f;
+                const uint32_t kt = pg_smem(at) + (uint32_t)((part + h) * kbytes);
+#pragma unroll
+                for (int x = 0; x < GK; x++) {
+                    if (x >= gk) break;
+                    const float c0 = offset[r][x], c1 = HI ? offset[r + 8][x] : 0.0f;
+                    float d[2][4];
+                    uint32_t w[2];
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(kt + x * 256 + lane * 8));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t w8 = w[e] >> 8, q0 = qf[x][e][0], q1 = HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, q2 = qf[x][e][1], q3 = HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u;
+                        if (e == 0) {
+                            mma_from(d[0], c0, c1, q0, q1, q2, q3, w[e] & FOUR_LO, w[e] & FOUR_HI);
+                            mma_from(d[1], c0, c1, q0, q1, q2, q3, w8 & FOUR_LO, w8 & FOUR_HI);
+                        } else {
+                            four_mma_f16(d[0], q0, q1, q2, q3, w[e] & FOUR_LO, w[e] & FOUR_HI);
+                            four_mma_f16(d[1], q0, q1, q2, q3, w8 & FOUR_LO, w8 & FOUR_HI);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        uint32_t both;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(kt + (uint32_t)(gk * 256 + ((4 * n + t) * gk + x) * 4)));
+                        const float s0 = pg_bf16_lo(both), s1 = pg_bf16_hi(both);
+                        sc[h][n][0] = fmaf(s0, d[n][0], sc[h][n][0]), sc[h][n][1] = fmaf(s1, d[n][1], sc[h][n][1]);
+                        if (HI) sc[h][n][2 * NT - 2] = fmaf(s0, d[n][2], sc[h][n][2 * NT - 2]), sc[h][n][2 * NT - 1] = fmaf(s1, d[n][3], sc[h][n][2 * NT - 1]);
+                    }
                 }
             }
             // to units of log 2, bias, mask
             float top[NT];
 #pragma unroll
-            for (int n = 0; n < NT; n++) top[n] = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int x = jt + 8 * n + 2 * t + j;
-#pragma unroll
-                    for (int u = 0; u < NT; u++) {
-                        float v = fmaf(bias[u], (float)(x - seen[u]), sc[n][2 * u + j] * fac[u]);
-                        if (edge && (x < x0 || x >= t1 || x > seen[u])) v = -INFINITY;
-                        sc[n][2 * u + j] = v;
-                        top[u] = fmaxf(top[u], v);
-                    }
-                }
-            float corr[NT];
-#pragma unroll
             for (int u = 0; u < NT; u++) {
-                top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
-                top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-                const float next = fmaxf(m[u], top[u]);
-                corr[u] = pg_ex2(m[u] - next);
-                m[u] = next;
-                float ps = 0.0f;
+                top[u] = -INFINITY;
+                const float b0 = s.slopes ? bias[u] * (float)(jp + 2 * t - seen[u]) : 0.0f;
 #pragma unroll
-                for (int n = 0; n < 2; n++)
+                for (int h = 0; h < JT; h++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        sc[n][2 * u + j] = pg_ex2(sc[n][2 * u + j] - next);
-                        ps += sc[n][2 * u + j];
-                    }
-                l[u] = fmaf(l[u], corr[u], ps);
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            float v = sc[h][n][2 * u + j] * 0x1p24f;
+                            v = s.slopes ? fmaf(v, fac[u], fmaf(bias[u], (float)(16 * h + 8 * n + j), b0)) : v * fac[u];
+                            if (edge) {
+                                const int x = jp + 16 * h + 8 * n + 2 * t + j;
+                                if (x < x0 || x >= t1 || x > seen[u]) v = -INFINITY;
+                            }
+                            sc[h][n][2 * u + j] = v;
+                            top[u] = fmaxf(top[u], v);
+                        }
             }
-            if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[NT - 1] != 1.0f)) {
-                // sums lie by row as columns: 2 t and 2 t + 1 of every eight
+            // the maximum is replaced where it falls behind by more than 2^8, which is rare behind the first keys
+            if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[NT - 1] > m[NT - 1] + 8.0f)) {
 #pragma unroll
                 for (int u = 0; u < NT; u++) {
-                    const float c0 = __shfl_sync(0xffffffffu, corr[u], 8 * t), c1 = __shfl_sync(0xffffffffu, corr[u], 8 * t + 4);
+                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+                    const float next = fmaxf(m[u], top[u]), corr = pg_ex2(m[u] - next);
+                    m[u] = next;
+                    // sums lie by row as columns: 2 t and 2 t + 1 of every eight
+                    const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+                    auto less = [&](float (&v)[4]) { v[0] *= c0, v[1] *= c1, v[2] *= c0, v[3] *= c1; };
+                    less(l[u]);
 #pragma unroll
-                    for (int x = 0; x < GV; x++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) o[x][e][u][0] *= c0, o[x][e][u][1] *= c1, o[x][e][u][2] *= c0, o[x][e][u][3] *= c1;
+                    for (int x = 0; x < GV; x++) less(o[x][0][u]), less(o[x][1][u]);
                 }
             }
+            // probabilities, rounded to bf16: their sums are those of the rounded ones, so that a row's weights still add up to one
+            uint32_t p[JT][NT][2];
 #pragma unroll
-            for (int x = 0; x < GV; x++) {
-                if (x >= gv) break;
-                // probabilities times the scales of keys 2 t, 2 t + 1 and 8 + 2 t, 8 + 2 t + 1
-                uint32_t b[NT][2];
+            for (int h = 0; h < JT; h++)
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    uint32_t two;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(two) : "r"(vt + (uint32_t)(gv * 256 + ((4 * n + t) * gv + x) * 4)));
-                    const float s0 = pg_bf16_lo(two), s1 = pg_bf16_hi(two);
+                for (int u = 0; u < NT; u++) {
 #pragma unroll
-                    for (int u = 0; u < NT; u++) {
-                        float p0 = sc[n][2 * u] * s0, p1 = sc[n][2 * u + 1] * s1;
-                        // (what a row does not see may hold anything)
-                        if (edge) p0 = sc[n][2 * u] == 0.0f ? 0.0f : p0, p1 = sc[n][2 * u + 1] == 0.0f ? 0.0f : p1;
-                        b[u][n] = pg_pack_bf16(p0, p1);
-                    }
+                    for (int n = 0; n < 2; n++) p[h][u][n] = pg_pack_bf16(pg_ex2(sc[h][n][2 * u] - m[u]), pg_ex2(sc[h][n][2 * u + 1] - m[u]));
+                    pg_mma_bf16(l[u], ONES, ONES, ONES, ONES, p[h][u][0], p[h][u][1]);
                 }
-                uint32_t w[2];
-                asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(vt + x * 256 + lane * 8));
+            // O^T += V^T P'^T, P' a probability times its value's scale
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t a0 = four_bf16_lo(w[e]), a1 = four_bf16_lo(w[e] >> 4), a2 = four_bf16_lo(w[e] >> 8), a3 = four_bf16_lo(w[e] >> 12);
+            for (int h = 0; h < JT; h++) {
+                const uint32_t vt = pg_smem(at) + (uint32_t)(A4_FILL * kbytes + (part + h) * vbytes);
 #pragma unroll
-                    for (int u = 0; u < NT; u++) pg_mma_bf16(o[x][e][u], a0, a1, a2, a3, b[u][0], b[u][1]);
+                for (int x = 0; x < GV; x++) {
+                    if (x >= gv) break;
+                    uint32_t b[NT][2];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        uint32_t both;                        // the scales of keys 8 n + 2 t and 8 n + 2 t + 1
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(vt + (uint32_t)(gv * 256 + ((4 * n + t) * gv + x) * 4)));
+#pragma unroll
+                        for (int u = 0; u < NT; u++) {
+                            b[u][n] = mul_bf16(p[h][u][n], both);
+                            // (what a row does not see may hold anything)
+                            if (edge) b[u][n] &= ((p[h][u][n] & 0xffffu) ? 0xffffu : 0u) | ((p[h][u][n] >> 16) ? 0xffff0000u : 0u);
+                        }
+                    }
+                    uint32_t w[2];
+                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(vt + x * 256 + lane * 8));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t a0 = four_bf16_lo(w[e]), a1 = four_bf16_lo(w[e] >> 4), a2 = four_bf16_lo(w[e] >> 8), a3 = four_bf16_lo(w[e] >> 12);
+#pragma unroll
+                        for (int u = 0; u < NT; u++) pg_mma_bf16(o[x][e][u], a0, a1, a2, a3, b[u][0], b[u][1]);
+                    }
                 }
             }
         }
@@ -614,11 +655,6 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
         while (pg_globaltimer_ns() - w0 < 2000000ull) {
         }
     }
-#pragma unroll
-    for (int u = 0; u < NT; u++) {
-        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-    }
     __syncthreads();                                      // the rings are free
     // warps meet in shared memory: [warp][16][vs + 4]
     const int ms = vs + 4;
@@ -627,15 +663,17 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
     for (int x = 0; x < GV; x++) {
         if (x >= gv) break;
 #pragma unroll
-        for (int e = 0; e < 2; e++)
+        for (int u = 0; u < NT; u++) {
 #pragma unroll
-            for (int u = 0; u < NT; u++)
+            for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) w0[(8 * u + 2 * t + (j & 1)) * ms + 32 * x + 16 * e + r + 8 * (j >> 1)] = o[x][e][u][j];
+        }
     }
-    if (t == 0) {
 #pragma unroll
-        for (int u = 0; u < NT; u++) w0[(r + 8 * u) * ms + vs] = m[u], w0[(r + 8 * u) * ms + vs + 1] = l[u];
+    for (int u = 0; u < NT; u++) {
+        if (t == 0) w0[(r + 8 * u) * ms + vs] = m[u];
+        if (r == 0) w0[(8 * u + 2 * t) * ms + vs + 1] = l[u][0], w0[(8 * u + 2 * t + 1) * ms + vs + 1] = l[u][1];
     }
     __syncthreads();
     const int64_t unit = (int64_t)seq * gridDim.y + blockIdx.y;
@@ -747,11 +785,11 @@ int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s)
     return (int)std::max<int64_t>(1, std::min<int64_t>(S, A4_SLICES));
 }
 
-template <int GK, int GV, bool HI, bool FUSED>
+template <int GK, int GV, bool HI, bool FUSED, bool EXACT>
 int32_t run_few(pg_ctx *ctx, const AttnShape &s, const Four &f, const pg_batch *bt, int few, int blocks, const float *proj, int64_t ldp, unsigned char *kc,
                 unsigned char *vc, float *part, int32_t *tickets, bf16 *out, int64_t ldo)
 {
-    auto kern = attn4_few_kernel<GK, GV, HI, FUSED>;
+    auto kern = attn4_few_kernel<GK, GV, HI, FUSED, EXACT>;
     // (two CTAs to an SM where the widths allow)
     const int fill = A4_WARPS * A4_FILL * (f.kb + f.vb), stages = 3 * fill <= 100 * 1024 ? 3 : 2, rings = stages * fill;
     const int smem = std::max(rings + 16 * (f.gk * 32 + 8) * 2, A4_WARPS * 16 * (f.gv * 32 + 4) * 4);
@@ -833,19 +871,22 @@ PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_ba
     float *part = p->d_part;
     int32_t *tickets = p->d_tickets;
     bf16 *out = (bf16 *)d_out;
-#define PG_A4(GK, GV, HI)                                                                                                                                     \
+#define PG_A4(GK, GV, HI, EXACT)                                                                                                                              \
     do {                                                                                                                                                      \
-        if (fused) return run_few<GK, GV, HI, true>(ctx, s, f, batch, (int)few, blocks, d_proj, ldp, kc, vc, part, tickets, out, ldo);                        \
-        return run_few<GK, GV, HI, false>(ctx, s, f, batch, (int)few, blocks, d_proj, ldp, kc, vc, part, tickets, out, ldo);                                  \
+        if (fused) return run_few<GK, GV, HI, true, EXACT>(ctx, s, f, batch, (int)few, blocks, d_proj, ldp, kc, vc, part, tickets, out, ldo);                 \
+        return run_few<GK, GV, HI, false, EXACT>(ctx, s, f, batch, (int)few, blocks, d_proj, ldp, kc, vc, part, tickets, out, ldo);                           \
     } while (0)
-#define PG_A4_HI(GK, GV)             \
-    do {                             \
-        if (hi) PG_A4(GK, GV, true); \
-        PG_A4(GK, GV, false);        \
+#define PG_A4_HI(GK, GV, EXACT)             \
+    do {                                    \
+        if (hi) PG_A4(GK, GV, true, EXACT); \
+        PG_A4(GK, GV, false, EXACT);        \
     } while (0)
-    if (f.gk <= 2 && f.gv <= 2) PG_A4_HI(2, 2);
-    if (f.gk <= 4 && f.gv <= 4) PG_A4_HI(4, 4);
-    PG_A4_HI(8, 8);
+    // (loops of a known length without a way out are half again as fast; the usual widths have them)
+    if (f.gk == 2 && f.gv == 2) PG_A4_HI(2, 2, true);
+    if (f.gk == 4 && f.gv == 4) PG_A4_HI(4, 4, true);
+    if (f.gk <= 2 && f.gv <= 2) PG_A4_HI(2, 2, false);
+    if (f.gk <= 4 && f.gv <= 4) PG_A4_HI(4, 4, false);
+    PG_A4_HI(8, 8, false);
 #undef PG_A4
 #undef PG_A4_HI
 }
