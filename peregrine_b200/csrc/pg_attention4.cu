@@ -15,6 +15,7 @@
 //   longer portions             attn4_append_kernel, then per sequence attn4_unfold_kernel and the kernels that prompts over a bf16 cache run through, on
 //                               f16: keys and values over a power of two of their head, which is exact, queries over one of their own.
 #include <algorithm>
+#include <type_traits>
 
 #include "pg_async.cuh"
 #include "pg_attention.cuh"
@@ -336,12 +337,12 @@ __global__ void __launch_bounds__(128)
     }
 }
 
-// D[16 x 8] = C + A[16 x 16] B[16 x 8], f16 operands; C has one number for rows r and one for rows r + 8
-__device__ __forceinline__ void mma_from(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+// D[16 x 8] = C + A[16 x 16] B[16 x 8], f16 operands
+__device__ __forceinline__ void mma_from(float (&d)[4], const float4 &c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 __device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b)
 {
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
     __shared__ __align__(8) uint64_t bars[A4_WARPS * A4_STAGES];
     __shared__ float weight[16][A4_SLICES];
     __shared__ float denom[16], back[16];
-    __shared__ __align__(16) float offset[16][8];
+    __shared__ __align__(16) float4 offset[8][8];         // of rows r, r, r + 8, r + 8
     __shared__ int last_in;
     __shared__ volatile int abort_flag;
     __shared__ uint8_t new_q[2][256];
@@ -439,14 +440,14 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
                     const __half v = __float2half_rn(x[i] * down);
                     qrow[c * qs + 32 * i + lane] = v;
                     const float sum = pg_warp_sum(__half2float(v));
-                    if (lane == 0) offset[c][i] = sum * -0x1p-21f;   // (the keys' quants are 8 too large)
+                    if (lane < 2) reinterpret_cast<float *>(&offset[c & 7][i])[c / 8 * 2 + lane] = sum * -0x1p-21f;   // (the keys' quants are 8 too large)
                 }
             if (lane == 0) back[c] = up * sl;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (i < gk) qrow[c * qs + 32 * i + lane] = __float2half_rn(0.0f);
-            if (lane < 8) offset[c][lane] = 0.0f;
+            if (lane < 16) reinterpret_cast<float *>(&offset[c & 7][lane >> 1])[c / 8 * 2 + (lane & 1)] = 0.0f;
             if (lane == 0) back[c] = 0.0f;
         }
     }
@@ -524,127 +525,134 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
             put_value(at + A4_FILL * kbytes + (row >> 4) * vbytes, new_q[1], new_s[1], row & 15, gv, lane);
             __syncwarp();
         }
-        const bool edge = j0 < x0 || j0 + 31 > sees_all || j0 + 31 >= t1;   // some row does not see all of these
+        // (the masks have a version of their own: taking them out of the way of all other keys is a fifth of the instructions)
+        auto tiles_of = [&](auto masked) {
+            constexpr bool edge = decltype(masked)::value;
 #pragma unroll
-        for (int part = 0; part < A4_FILL; part += JT) {  // as many tiles at once as registers allow
-            const int jp = j0 + 16 * part;
-            if (jp >= t1) break;                              // (uniform)
+            for (int part = 0; part < A4_FILL; part += JT) {  // as many tiles at once as registers allow
+                const int jp = j0 + 16 * part;
+                if (jp >= t1) break;                          // (uniform)
                 // scores of keys 16 h + 8 n + 2 t and 16 h + 8 n + 2 t + 1 with rows r and r + 8.  A quant as the low bits of an f16 number is that number of
-            // its smallest steps, 2^-24; the sums start at what 8 of them in every column make.
-            float sc[JT][2][2 * NT];
+                // its smallest steps, 2^-24; the sums start at what 8 of them in every column make.
+                float sc[JT][2][2 * NT];
 #pragma unroll
-            for (int h = 0; h < JT; h++) {
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int j = 0; j < 2 * NT; j++) sc[h][n][j] = 0.0f;
-                const uint32_t kt = pg_smem(at) + (uint32_t)((part + h) * kbytes);
-#pragma unroll
-                for (int x = 0; x < GK; x++) {
-                    if (x >= gk) break;
-                    const float c0 = offset[r][x], c1 = HI ? offset[r + 8][x] : 0.0f;
-                    float d[2][4];
-                    uint32_t w[2];
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(kt + x * 256 + lane * 8));
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const uint32_t w8 = w[e] >> 8, q0 = qf[x][e][0], q1 = HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, q2 = qf[x][e][1], q3 = HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u;
-                        if (e == 0) {
-                            mma_from(d[0], c0, c1, q0, q1, q2, q3, w[e] & FOUR_LO, w[e] & FOUR_HI);
-                            mma_from(d[1], c0, c1, q0, q1, q2, q3, w8 & FOUR_LO, w8 & FOUR_HI);
-                        } else {
-                            four_mma_f16(d[0], q0, q1, q2, q3, w[e] & FOUR_LO, w[e] & FOUR_HI);
-                            four_mma_f16(d[1], q0, q1, q2, q3, w8 & FOUR_LO, w8 & FOUR_HI);
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        uint32_t both;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(kt + (uint32_t)(gk * 256 + ((4 * n + t) * gk + x) * 4)));
-                        const float s0 = pg_bf16_lo(both), s1 = pg_bf16_hi(both);
-                        sc[h][n][0] = fmaf(s0, d[n][0], sc[h][n][0]), sc[h][n][1] = fmaf(s1, d[n][1], sc[h][n][1]);
-                        if (HI) sc[h][n][2 * NT - 2] = fmaf(s0, d[n][2], sc[h][n][2 * NT - 2]), sc[h][n][2 * NT - 1] = fmaf(s1, d[n][3], sc[h][n][2 * NT - 1]);
-                    }
-                }
-            }
-            // to units of log 2, bias, mask
-            float top[NT];
-#pragma unroll
-            for (int u = 0; u < NT; u++) {
-                top[u] = -INFINITY;
-                const float b0 = s.slopes ? bias[u] * (float)(jp + 2 * t - seen[u]) : 0.0f;
-#pragma unroll
-                for (int h = 0; h < JT; h++)
+                for (int h = 0; h < JT; h++) {
 #pragma unroll
                     for (int n = 0; n < 2; n++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            float v = sc[h][n][2 * u + j] * 0x1p24f;
-                            v = s.slopes ? fmaf(v, fac[u], fmaf(bias[u], (float)(16 * h + 8 * n + j), b0)) : v * fac[u];
-                            if (edge) {
-                                const int x = jp + 16 * h + 8 * n + 2 * t + j;
-                                if (x < x0 || x >= t1 || x > seen[u]) v = -INFINITY;
+                        for (int j = 0; j < 2 * NT; j++) sc[h][n][j] = 0.0f;
+                    const uint32_t kt = pg_smem(at) + (uint32_t)((part + h) * kbytes);
+#pragma unroll
+                    for (int x = 0; x < GK; x++) {
+                        if (x >= gk) break;
+                        const float4 c4 = offset[r][x];
+                        float d[2][4];
+                        uint32_t w[2];
+                        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(kt + x * 256 + lane * 8));
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const uint32_t w8 = w[e] >> 8, q0 = qf[x][e][0], q1 = HI ? qf[x][e][2 % (HI ? 4 : 2)] : 0u, q2 = qf[x][e][1], q3 = HI ? qf[x][e][3 % (HI ? 4 : 2)] : 0u;
+                            if (e == 0) {
+                                mma_from(d[0], c4, q0, q1, q2, q3, w[e] & FOUR_LO, w[e] & FOUR_HI);
+                                mma_from(d[1], c4, q0, q1, q2, q3, w8 & FOUR_LO, w8 & FOUR_HI);
+                            } else {
+                                four_mma_f16(d[0], q0, q1, q2, q3, w[e] & FOUR_LO, w[e] & FOUR_HI);
+                                four_mma_f16(d[1], q0, q1, q2, q3, w8 & FOUR_LO, w8 & FOUR_HI);
                             }
-                            sc[h][n][2 * u + j] = v;
-                            top[u] = fmaxf(top[u], v);
                         }
-            }
-            // the maximum is replaced where it falls behind by more than 2^8, which is rare behind the first keys
-            if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[NT - 1] > m[NT - 1] + 8.0f)) {
 #pragma unroll
-                for (int u = 0; u < NT; u++) {
-                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
-                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-                    const float next = fmaxf(m[u], top[u]), corr = pg_ex2(m[u] - next);
-                    m[u] = next;
-                    // sums lie by row as columns: 2 t and 2 t + 1 of every eight
-                    const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
-                    auto less = [&](float (&v)[4]) { v[0] *= c0, v[1] *= c1, v[2] *= c0, v[3] *= c1; };
-                    less(l[u]);
-#pragma unroll
-                    for (int x = 0; x < GV; x++) less(o[x][0][u]), less(o[x][1][u]);
-                }
-            }
-            // probabilities, rounded to bf16: their sums are those of the rounded ones, so that a row's weights still add up to one
-            uint32_t p[JT][NT][2];
-#pragma unroll
-            for (int h = 0; h < JT; h++)
-#pragma unroll
-                for (int u = 0; u < NT; u++) {
-#pragma unroll
-                    for (int n = 0; n < 2; n++) p[h][u][n] = pg_pack_bf16(pg_ex2(sc[h][n][2 * u] - m[u]), pg_ex2(sc[h][n][2 * u + 1] - m[u]));
-                    pg_mma_bf16(l[u], ONES, ONES, ONES, ONES, p[h][u][0], p[h][u][1]);
-                }
-            // O^T += V^T P'^T, P' a probability times its value's scale
-#pragma unroll
-            for (int h = 0; h < JT; h++) {
-                const uint32_t vt = pg_smem(at) + (uint32_t)(A4_FILL * kbytes + (part + h) * vbytes);
-#pragma unroll
-                for (int x = 0; x < GV; x++) {
-                    if (x >= gv) break;
-                    uint32_t b[NT][2];
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        uint32_t both;                        // the scales of keys 8 n + 2 t and 8 n + 2 t + 1
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(vt + (uint32_t)(gv * 256 + ((4 * n + t) * gv + x) * 4)));
-#pragma unroll
-                        for (int u = 0; u < NT; u++) {
-                            b[u][n] = mul_bf16(p[h][u][n], both);
-                            // (what a row does not see may hold anything)
-                            if (edge) b[u][n] &= ((p[h][u][n] & 0xffffu) ? 0xffffu : 0u) | ((p[h][u][n] >> 16) ? 0xffff0000u : 0u);
+                        for (int n = 0; n < 2; n++) {
+                            uint32_t both;
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(kt + (uint32_t)(gk * 256 + ((4 * n + t) * gk + x) * 4)));
+                            const float s0 = pg_bf16_lo(both), s1 = pg_bf16_hi(both);
+                            sc[h][n][0] = fmaf(s0, d[n][0], sc[h][n][0]), sc[h][n][1] = fmaf(s1, d[n][1], sc[h][n][1]);
+                            if (HI) sc[h][n][2 * NT - 2] = fmaf(s0, d[n][2], sc[h][n][2 * NT - 2]), sc[h][n][2 * NT - 1] = fmaf(s1, d[n][3], sc[h][n][2 * NT - 1]);
                         }
                     }
-                    uint32_t w[2];
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(vt + x * 256 + lane * 8));
+                }
+                // to units of log 2, bias, mask
+                float top[NT];
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const uint32_t a0 = four_bf16_lo(w[e]), a1 = four_bf16_lo(w[e] >> 4), a2 = four_bf16_lo(w[e] >> 8), a3 = four_bf16_lo(w[e] >> 12);
+                for (int u = 0; u < NT; u++) {
+                    top[u] = -INFINITY;
+                    const float b0 = s.slopes ? bias[u] * (float)(jp + 2 * t - seen[u]) : 0.0f;
 #pragma unroll
-                        for (int u = 0; u < NT; u++) pg_mma_bf16(o[x][e][u], a0, a1, a2, a3, b[u][0], b[u][1]);
+                    for (int h = 0; h < JT; h++)
+#pragma unroll
+                        for (int n = 0; n < 2; n++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                float v = sc[h][n][2 * u + j] * 0x1p24f;
+                                v = s.slopes ? fmaf(v, fac[u], fmaf(bias[u], (float)(16 * h + 8 * n + j), b0)) : v * fac[u];
+                                if (edge) {
+                                    const int x = jp + 16 * h + 8 * n + 2 * t + j;
+                                    if (x < x0 || x >= t1 || x > seen[u]) v = -INFINITY;
+                                }
+                                sc[h][n][2 * u + j] = v;
+                                top[u] = fmaxf(top[u], v);
+                            }
+                }
+                // the maximum is replaced where it falls behind by more than 2^8, which is rare behind the first keys
+                if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[NT - 1] > m[NT - 1] + 8.0f)) {
+#pragma unroll
+                    for (int u = 0; u < NT; u++) {
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+                        const float next = fmaxf(m[u], top[u]), corr = pg_ex2(m[u] - next);
+                        m[u] = next;
+                        // sums lie by row as columns: 2 t and 2 t + 1 of every eight
+                        const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+                        auto less = [&](float (&v)[4]) { v[0] *= c0, v[1] *= c1, v[2] *= c0, v[3] *= c1; };
+                        less(l[u]);
+#pragma unroll
+                        for (int x = 0; x < GV; x++) less(o[x][0][u]), less(o[x][1][u]);
+                    }
+                }
+                // probabilities, rounded to bf16: their sums are those of the rounded ones, so that a row's weights still add up to one
+                uint32_t p[JT][NT][2];
+#pragma unroll
+                for (int h = 0; h < JT; h++)
+#pragma unroll
+                    for (int u = 0; u < NT; u++) {
+#pragma unroll
+                        for (int n = 0; n < 2; n++) p[h][u][n] = pg_pack_bf16(pg_ex2(sc[h][n][2 * u] - m[u]), pg_ex2(sc[h][n][2 * u + 1] - m[u]));
+                        pg_mma_bf16(l[u], ONES, ONES, ONES, ONES, p[h][u][0], p[h][u][1]);
+                    }
+                // O^T += V^T P'^T, P' a probability times its value's scale
+#pragma unroll
+                for (int h = 0; h < JT; h++) {
+                    const uint32_t vt = pg_smem(at) + (uint32_t)(A4_FILL * kbytes + (part + h) * vbytes);
+#pragma unroll
+                    for (int x = 0; x < GV; x++) {
+                        if (x >= gv) break;
+                        uint32_t b[NT][2];
+#pragma unroll
+                        for (int n = 0; n < 2; n++) {
+                            uint32_t both;                        // the scales of keys 8 n + 2 t and 8 n + 2 t + 1
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(vt + (uint32_t)(gv * 256 + ((4 * n + t) * gv + x) * 4)));
+#pragma unroll
+                            for (int u = 0; u < NT; u++) {
+                                b[u][n] = mul_bf16(p[h][u][n], both);
+                                // (what a row does not see may hold anything)
+                                if (edge) b[u][n] &= ((p[h][u][n] & 0xffffu) ? 0xffffu : 0u) | ((p[h][u][n] >> 16) ? 0xffff0000u : 0u);
+                            }
+                        }
+                        uint32_t w[2];
+                        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(vt + x * 256 + lane * 8));
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const uint32_t a0 = four_bf16_lo(w[e]), a1 = four_bf16_lo(w[e] >> 4), a2 = four_bf16_lo(w[e] >> 8), a3 = four_bf16_lo(w[e] >> 12);
+#pragma unroll
+                            for (int u = 0; u < NT; u++) pg_mma_bf16(o[x][e][u], a0, a1, a2, a3, b[u][0], b[u][1]);
+                        }
                     }
                 }
             }
-        }
+        };
+        if (j0 < x0 || j0 + 31 > sees_all || j0 + 31 >= t1)   // some row does not see all of these
+            tiles_of(std::true_type{});
+        else
+            tiles_of(std::false_type{});
         __syncwarp();                                     // every lane is done with the stage before it is filled again
         if (i + stages < mine) fetch(i + stages, at_stage);
         if (++at_stage == stages) at_stage = 0, phase ^= 1;
