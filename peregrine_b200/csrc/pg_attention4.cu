@@ -351,6 +351,22 @@ __device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b)
     return r;
 }
 
+// the scales of a pair of positions, all groups'
+template <int N, bool EXACT>
+__device__ __forceinline__ void load_scales(uint32_t (&v)[N], uint32_t at, int groups)
+{
+    if (EXACT && N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]) : "r"(at + i * 4));
+    } else if (EXACT && N == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < groups) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(at + i * 4));
+    }
+}
+
 // ---- few tokens: grid (slices, G * blocks of 16 rows, seqs) --------------------------------------------------------------------
 constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // most fills in flight of a warp; tiles of a fill
 
@@ -542,6 +558,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
 #pragma unroll
                         for (int j = 0; j < 2 * NT; j++) sc[h][n][j] = 0.0f;
                     const uint32_t kt = pg_smem(at) + (uint32_t)((part + h) * kbytes);
+                    uint32_t ks[2][GK];                   // of keys 8 n + 2 t and 8 n + 2 t + 1
+#pragma unroll
+                    for (int n = 0; n < 2; n++) load_scales<GK, EXACT>(ks[n], kt + (uint32_t)((gk * 64 + (4 * n + t) * gk) * 4), gk);
 #pragma unroll
                     for (int x = 0; x < GK; x++) {
                         if (x >= gk) break;
@@ -562,9 +581,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
                         }
 #pragma unroll
                         for (int n = 0; n < 2; n++) {
-                            uint32_t both;
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(kt + (uint32_t)(gk * 256 + ((4 * n + t) * gk + x) * 4)));
-                            const float s0 = pg_bf16_lo(both), s1 = pg_bf16_hi(both);
+                            const float s0 = pg_bf16_lo(ks[n][x]), s1 = pg_bf16_hi(ks[n][x]);
                             sc[h][n][0] = fmaf(s0, d[n][0], sc[h][n][0]), sc[h][n][1] = fmaf(s1, d[n][1], sc[h][n][1]);
                             if (HI) sc[h][n][2 * NT - 2] = fmaf(s0, d[n][2], sc[h][n][2 * NT - 2]), sc[h][n][2 * NT - 1] = fmaf(s1, d[n][3], sc[h][n][2 * NT - 1]);
                         }
@@ -622,17 +639,18 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
 #pragma unroll
                 for (int h = 0; h < JT; h++) {
                     const uint32_t vt = pg_smem(at) + (uint32_t)(A4_FILL * kbytes + (part + h) * vbytes);
+                    uint32_t scales[2][GV];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) load_scales<GV, EXACT>(scales[n], vt + (uint32_t)((gv * 64 + (4 * n + t) * gv) * 4), gv);
 #pragma unroll
                     for (int x = 0; x < GV; x++) {
                         if (x >= gv) break;
                         uint32_t b[NT][2];
 #pragma unroll
                         for (int n = 0; n < 2; n++) {
-                            uint32_t both;                        // the scales of keys 8 n + 2 t and 8 n + 2 t + 1
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(vt + (uint32_t)(gv * 256 + ((4 * n + t) * gv + x) * 4)));
 #pragma unroll
                             for (int u = 0; u < NT; u++) {
-                                b[u][n] = mul_bf16(p[h][u][n], both);
+                                b[u][n] = mul_bf16(p[h][u][n], scales[n][x]);
                                 // (what a row does not see may hold anything)
                                 if (edge) b[u][n] &= ((p[h][u][n] & 0xffffu) ? 0xffffu : 0u) | ((p[h][u][n] >> 16) ? 0xffff0000u : 0u);
                             }
