@@ -1,0 +1,213 @@
+"""Models with weights and caches of 4 bits, on the GPU against the oracles with the same roundings.
+
+Weights are rounded when a model is built, by a formula that this file repeats, so that the oracle with the rounded weights differs from the model
+only by the rounding of bf16 steps: the tolerances of the models' own tests.  A cache rounds what a step computes, and a key or value that a bf16 step
+has off by 2^-8 of itself now and then falls on the other side of a half: one in 30 by a step of an eighth of its group's largest, 2 % of that in
+the mean.  Half of the layers are attention layers and their outputs are averages, so logits are off by up to twice what a bf16 step alone does."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from oracle import bubotar_oracle as bo
+from oracle import sonalorn_oracle as so
+from tests import _bubotar as tb
+from tests import _sonalorn as ts
+from tests.test_linear4_gpu import quantised
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TOL = 4e-2      # the median error of logits that a model's bf16 steps are allowed
+
+LAYER_MATRICES = ("q", "k", "v", "g", "b", "a", "o", "dkv", "in", "gate", "up", "down")
+
+
+@pytest.fixture(scope="module")
+def lm():
+    from peregrine_b200.runtime import GpuContext
+
+    return GpuContext(component="lm")
+
+
+def rng(seed):
+    return np.random.Generator(np.random.PCG64(seed))
+
+
+def four_bits(w, group):
+    pad = -w.shape[1] % group
+    return quantised(np.pad(w.astype(np.float32), ((0, 0), (0, pad))), group)[:, :w.shape[1]]
+
+
+def rounded(W):
+    """Weights as a model of 4 bits holds them."""
+    return {k: four_bits(v, 64) if k.startswith("l") and v.ndim == 2 and k.split(".")[-1] in LAYER_MATRICES else v for k, v in W.items()}
+
+
+def rounded_cache(attention):
+    """An oracle's attention over keys and values as a cache of 4 bits holds them."""
+    rows = lambda x: four_bits(x.reshape(-1, x.shape[2]), 32).reshape(x.shape).astype(x.dtype)
+    return lambda q, k, v, *rest: attention(q, rows(k), rows(v), *rest)
+
+
+def make_engine(lm, t, cfg, W, slots=3, portion=0, step_rows=400, **bits):
+    from peregrine_b200.bubotar import BubotarConfig, BubotarModel
+    from peregrine_b200.engine import Engine
+    from peregrine_b200.sonalorn import SonalornConfig, SonalornModel
+
+    conf, model = (SonalornConfig, SonalornModel) if t is ts else (BubotarConfig, BubotarModel)
+    more = {} if t is ts else {"capacity": 400}
+    raw = {k: t.to_bits(v) for k, v in W.items()}
+    return Engine(model(conf.from_dict(cfg), raw, lm, dtype="bfloat16", slots=slots, step_rows=step_rows, max_wanted=16, **more, **bits), portion=portion)
+
+
+def logit_error(got, want):
+    e = np.asarray(got, np.float64) - want
+    e -= e.mean(-1, keepdims=True)
+    return np.sqrt((e ** 2).mean(-1)) / np.sqrt((want ** 2).mean())
+
+
+def run(e, tokens, cuts):
+    at, got = 0, []
+    for n in cuts:
+        got.append(e.step([("r", tokens[at:at + n], list(range(n)))]))
+        at += n
+    e.end("r")
+    return np.concatenate(got)
+
+
+def attention_heavy(t):
+    """Attention and feed-forward layers at widths that prompts run through the tcgen05 kernels with, experts among them."""
+    if t is tb:
+        return tb.config(120, 128, [tb.layer("attention", tb.attention(4, 2, 64, 128, 0.12, 48), tb.dense(136, 2.0)),
+                                    tb.layer("attention", tb.attention(8, 1, 96, 40, 0.1, 500), tb.dense(72, 1.4))], logit_scale=3.0)
+    return ts.config(83, 128, [ts.layer("attention", ts.attention(4, 1, 64, 64, 0.2, (0.4, 50)), ts.dense(72)),
+                               ts.layer("attention", ts.attention(16, 4, 128, 64, 0.1), ts.moe(200, 1.2, 12, 3, 3, (3, 2)))], max_positions=500)
+
+
+@pytest.mark.parametrize("t,make", [(ts, ts.small_config), (ts, ts.other_config), (tb, tb.small_config), (tb, tb.even_config), (ts, lambda: attention_heavy(ts))])
+def test_weights(lm, t, make):
+    cfg = make()
+    W = t.weights(cfg, 11)
+    oracle = (so if t is ts else bo).Model(cfg, rounded(W))
+    e = make_engine(lm, t, cfg, W, weight_bits=4)
+    g = rng(12)
+    for T in (1, 2, 37, 150):
+        tokens = g.integers(0, cfg["vocab"], T).tolist()
+        want = oracle.forward(tokens, oracle.start())
+        for cuts in ([T], [1] * T, [T - T // 3] + [1] * (T // 3)):
+            err = logit_error(run(e, tokens, cuts), want)
+            # (a bf16 router can choose differently at a close call: single positions may be further off)
+            assert np.median(err) < TOL and err.max() < 12 * TOL, (T, cuts[:3], np.median(err), err.max())
+    held = lambda e: sum(L["mixer"].bytes() + (L["ff"].bytes(150) if L.get("ff") else 0) for L in e.model.layers)
+    small = held(e)
+    e.close()
+    e = make_engine(lm, t, cfg, W)
+    assert small < 0.8 * held(e)      # (a latent's and a scan's low-rank matrices stay as they are)
+    e.close()
+
+
+@pytest.mark.parametrize("t", [ts, tb])
+def test_caches(lm, t, monkeypatch):
+    cfg = attention_heavy(t)
+    W = t.weights(cfg, 21)
+    mod = so if t is ts else bo
+    e = make_engine(lm, t, cfg, W, cache_bits=4)
+    tokens = rng(22).integers(0, cfg["vocab"], 300).tolist()
+    plain = mod.Model(cfg, W).forward(tokens, mod.Model(cfg, W).start())
+    monkeypatch.setattr(mod, "attention", rounded_cache(mod.attention))
+    oracle = mod.Model(cfg, W)
+    want = oracle.forward(tokens, oracle.start())
+    first = None
+    for cuts in ([300], [200] + [1] * 100, [10, 5, 16, 1, 1, 130, 1, 136], [1] * 300):
+        got = run(e, tokens, cuts)
+        err = logit_error(got, want)
+        assert np.median(err) < 2 * TOL, (cuts[:3], np.median(err))
+        assert np.median(err) < np.median(logit_error(got, plain)), "the cache's rounding is not the one expected"
+        first = got if first is None else first
+        assert np.median(logit_error(got, first.astype(np.float64))) < 2 * TOL
+    # 9 bits for every 2 columns and position in place of 32
+    small = e.model.pool.bytes
+    e.close()
+    e = make_engine(lm, t, cfg, W)
+    assert small < 0.4 * e.model.pool.bytes
+    e.close()
+
+
+@pytest.mark.parametrize("t", [ts, tb])
+def test_together_in_mixed_and_recorded_steps(lm, t, monkeypatch):
+    """Weights and caches of 4 bits: unequal requests in one step, slots used again, greedy decoding through the scheduler as recorded graphs."""
+    cfg = attention_heavy(t)
+    W = t.weights(cfg, 31)
+    W["head"] = t.bf16_values(W["head"] * 2)
+    mod = so if t is ts else bo
+    monkeypatch.setattr(mod, "attention", rounded_cache(mod.attention))
+    oracle = mod.Model(cfg, rounded(W))
+    g = rng(32)
+    prompts = {k: g.integers(0, cfg["vocab"], n).tolist() for k, n in {"a": 310, "b": 8, "c": 180}.items()}
+    cuts = {"a": [140, 1, 60, 1, 108], "b": [2, 1, 2, 1, 2], "c": [33, 1, 130, 1, 15]}
+    e = make_engine(lm, t, cfg, W, weight_bits=4, cache_bits=4)
+    for again in range(2):
+        at, out = dict.fromkeys(prompts, 0), {k: [] for k in prompts}
+        for i in range(5):
+            entries = [(k, x[at[k]:at[k] + cuts[k][i]], list(range(cuts[k][i]))) for k, x in prompts.items()]
+            rows = e.step(entries)
+            for k, x, want in entries:
+                out[k].append(rows[:len(want)])
+                rows = rows[len(want):]
+                at[k] += len(x)
+        for k, x in prompts.items():
+            assert np.median(logit_error(np.concatenate(out[k]), oracle.forward(x, oracle.start()))) < 2 * TOL, k
+            e.end(k)
+    e.close()
+    e = make_engine(lm, t, cfg, W, weight_bits=4, cache_bits=4, portion=70, step_rows=80)
+    prompts = [g.integers(0, cfg["vocab"], n).tolist() for n in (1, 33, 5, 18, 64, 150)]
+    got = e.generate(prompts, 12)
+    assert got == e.generate(prompts, 12)
+    for x, y in zip(prompts, got):
+        logits = oracle.forward(x + y[:-1], oracle.start())[len(x) - 1:]
+        lead = logits.max(-1) - logits[np.arange(len(y)), y]
+        assert (lead < 8 * TOL * np.sqrt((logits ** 2).mean())).all()
+    e.close()
+
+
+def test_wider_layers(lm, monkeypatch):
+    """Sizes at which the kernels take their other forms: K over several blocks, 128-wide heads, many experts."""
+    cfg = ts.config(300, 640, [ts.layer("delta", ts.delta(8, 4, 128, 128, 4), ts.dense(4300)),
+                               ts.layer("attention", ts.attention(16, 2, 128, 64, 0.09, (0.4, 32)), ts.moe(200, 1.2, 40, 8, 6, (8, 4)))], max_positions=260)
+    W = ts.weights(cfg, 41)
+    monkeypatch.setattr(so, "attention", rounded_cache(so.attention))
+    oracle = so.Model(cfg, rounded(W), np.float32)
+    tokens = rng(42).integers(0, 300, 200).tolist()
+    want = oracle.forward(tokens, oracle.start()).astype(np.float64)
+    e = make_engine(lm, ts, cfg, W, weight_bits=4, cache_bits=4)
+    for cuts in ([150] + [1] * 50, [17, 3, 160, 20]):
+        assert np.median(logit_error(run(e, tokens, cuts), want)) < 2 * TOL
+    e.close()
+
+
+def test_refusals(lm):
+    cfg = attention_heavy(ts)
+    W = {k: ts.to_bits(v) for k, v in ts.weights(cfg, 51).items()}
+    from peregrine_b200.sonalorn import SonalornConfig, SonalornModel
+
+    for kw in ({"weight_bits": 4}, {"cache_bits": 4}):
+        with pytest.raises(ValueError, match="bfloat16"):
+            SonalornModel(SonalornConfig.from_dict(cfg), W, lm, dtype="float32", **kw)
+    for kw in ({"weight_bits": 8}, {"cache_bits": 5}):
+        with pytest.raises(ValueError, match="16, or 4|bits"):
+            SonalornModel(SonalornConfig.from_dict(cfg), W, lm, **kw)
+
+
+def test_command_line(lm, tmp_path):
+    cfg = attention_heavy(ts)
+    W = ts.weights(cfg, 61)
+    ts.save(str(tmp_path / "model"), cfg, W)
+    e = make_engine(lm, ts, cfg, W, slots=2, step_rows=2048, weight_bits=4, cache_bits=4)
+    want = e.generate([[1, 2, 3, 4, 5], [80, 7]], 5)
+    e.close()
+    r = subprocess.run([sys.executable, "-m", "peregrine_b200", "generate", "--model", str(tmp_path / "model"), "--max-new", "5", "--prompt", "1,2,3,4,5",
+                        "--prompt", "80,7", "--weight-bits", "4", "--cache-bits", "4"], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert [[int(x) for x in line.split(",")] for line in r.stdout.split()] == want
