@@ -70,24 +70,24 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     const uint32_t fill_bytes = (uint32_t)(klen / 64 * record);
     const int64_t row_bytes = (int64_t)(K / 64) * record;
 
-    // row of the weights' layout: tile of an expert
-    auto base_of = [&](int64_t it) -> int64_t {
-        if (!ROUTED) return it;
-        const int blk = (int)(it / tiles);
-        return (int64_t)__ldcg(rt.block_expert + blk) * tiles + (it - (int64_t)blk * tiles);
-    };
+    // a tile of the weights' layout; with a route the tiles of a block's expert follow one another, and the expert is looked up where a block begins
+    const int blk0 = ROUTED ? (int)(first / tiles) : 0, tile0 = ROUTED ? (int)(first - (int64_t)blk0 * tiles) : 0;
+    auto expert_of = [&](int blk) -> int64_t { return blk < nblk ? __ldcg(rt.block_expert + blk) : 0; };
+    const int64_t base0 = !ROUTED ? first : mine > 0 ? expert_of(blk0) * tiles + tile0 : 0;
     // fills follow one another through the slots; without a route they lie a constant distance apart
-    int fill_slot = 0, filled = 0;
-    const unsigned char *next = w + first * row_bytes + k0 / 64 * record;
+    int fill_slot = 0, fill_blk = blk0, fill_tile = tile0;
+    const unsigned char *next = w + base0 * row_bytes + k0 / 64 * record;
     auto issue = [&]() {
         if (lane == 0) {
             const uint32_t bar = my_bar + (uint32_t)fill_slot * 8;
-            if (ROUTED) next = w + base_of(first + filled) * row_bytes + k0 / 64 * record;
             pg_mbar_expect(bar, fill_bytes);
             pg_bulk_load(ring + (uint32_t)fill_slot * fill_bytes, next, fill_bytes, bar);
         }
-        if (!ROUTED) next += step * row_bytes;
-        filled++;
+        next += step * row_bytes;
+        if (ROUTED && ++fill_tile == tiles) {
+            fill_tile = 0;
+            next = w + expert_of(++fill_blk) * tiles * row_bytes + k0 / 64 * record;
+        }
         if (++fill_slot == slots) fill_slot = 0;
     };
     for (int f = 0; f < slots; f++)
@@ -98,9 +98,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     // quants beside it come 16 times too large)
     uint32_t x[NT][KWM / 8];
     float back[NT][2];                                    // what the sums of columns 2 t and 2 t + 1 are multiplied by
-    int have = -1;
     auto bring = [&](int blk) {
-        have = blk;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             int64_t at = r + 8 * j;
@@ -139,14 +137,24 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
         }
     };
 
+    // bit 2 j + i: there is a row 8 j + 2 t + i
+    auto rows_of = [&](int blk) {
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * NT; j++) {
+            const int m = 8 * (j >> 1) + 2 * t + (j & 1);
+            in |= (uint32_t)(ROUTED ? __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + m) >= 0 : m < M) << j;
+        }
+        return in;
+    };
     // outputs of a tile; lane: weight rows r and r + 8, rows 2 t and 2 t + 1 of the activations
-    auto finish = [&](const float (&acc)[NT][4], int blk, int tile) {
+    auto finish = [&](const float (&acc)[NT][4], int blk, int tile, uint32_t in) {
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int m = (ROUTED ? blk * PG_ROUTE_SMALL : 0) + 8 * j + 2 * t + i;
-                if (ROUTED ? (__ldcg(rt.row_pair + m) < 0) : (m >= M)) continue;
+                const int64_t m = (ROUTED ? blk * PG_ROUTE_SMALL : 0) + 8 * j + 2 * t + i;
+                if (!(in >> (2 * j + i) & 1u)) continue;
                 const float v0 = acc[j][i], v1 = acc[j][2 + i];
                 if (ACT != PG_ACT_NONE) {
                     pg_put(y + m * ldy + tile * 8 + r, pg_glu<ACT>(v0, v1, limit));
@@ -162,18 +170,23 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     int slot = 0, cell = 0;
     uint32_t phase = 0, cell_phase = 0;
     if (!ROUTED && mine > 0 && klen > 0) bring(0);
+    int blk = blk0 - 1, tile = ROUTED ? tiles - 1 : (int)(first - step);
+    uint32_t in = ROUTED ? 0 : rows_of(0);
+    const float *fac = wrow + (base0 - step) * 16 + r;    // the factors of rows r and r + 8 of the tile
     for (int j = 0; j < mine; j++) {
         float acc[NT][4] = {};
         const int64_t it = first + j * step;
-        const int blk = ROUTED ? (int)(it / tiles) : 0, tile = (int)(it - (int64_t)blk * tiles);
+        tile += (int)step, fac += step * 16;
+        if (ROUTED && (tile == tiles || j == 0)) {        // another block, another expert
+            blk++, tile = j == 0 ? tile0 : 0;
+            if (j > 0) fac = wrow + expert_of(blk) * tiles * 16 + r;
+            in = rows_of(blk);
+            if (klen > 0) bring(blk);
+            second = NT == 2 && __shfl_sync(0xffffffffu, (int)(in >> 2 & 1u), 0);   // (a block's rows are filled from the first on)
+        }
         const int turn = (j + slot_idx) & (kw - 1);       // the warp that adds the parts up
         if (klen > 0) {
-            const float *fac = wrow + base_of(it) * 16 + r;
             const float f0 = __ldg(fac), f1 = __ldg(fac + 8);
-            if (ROUTED && blk != have) {
-                bring(blk);
-                second = NT == 2 && __shfl_sync(0xffffffffu, __ldcg(rt.row_pair + blk * PG_ROUTE_SMALL + 8), 0) >= 0;   // (a block's rows are filled from the first on)
-            }
             ok = ok && pg_mbar_wait_warp(my_bar + (uint32_t)slot * 8, phase, abort_flag, status, limit_ns);
             if (ok) {
                 const uint32_t slot_at = ring + (uint32_t)slot * fill_bytes;
@@ -262,7 +275,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
 #pragma unroll
                 for (int n = 0; n < NT; n++) dst[n] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
             } else {
-                finish(acc, blk, tile);
+                finish(acc, blk, tile, in);
             }
         }
     }
@@ -301,7 +314,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
                         acc[n][0] += v.x, acc[n][1] += v.y, acc[n][2] += v.z, acc[n][3] += v.w;
                     }
                 }
-                finish(acc, blk, (int)(it - (int64_t)blk * tiles));
+                finish(acc, blk, (int)(it - (int64_t)blk * tiles), rows_of(blk));
             }
         }
     }
@@ -363,7 +376,7 @@ int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int6
                          const PgRouted *routed, int64_t max_blocks)
 {
     const int64_t items = lin->tiles * (routed ? max_blocks : 1);
-    const int nt = m > 8 || routed ? 2 : 1;
+    const int nt = m > 8 ? 2 : 1;   // (an expert has a row of a token at most)
     const Parts p = parts_of(lin, items, ctx->sm_count, nt);
     PG_REQUIRE(p.KW <= v4_kw_max(nt) && p.sp <= 16, "linear4: K too long");
     if (p.sp > 1) {
@@ -382,7 +395,8 @@ int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int6
     } while (0)
 #define PG_V4_ACT(ACT, TY)                  \
     do {                                    \
-        if (routed) PG_V4(ACT, 2, true, TY); \
+        if (routed && nt == 2) PG_V4(ACT, 2, true, TY); \
+        if (routed) PG_V4(ACT, 1, true, TY); \
         if (nt == 2) PG_V4(ACT, 2, false, TY); \
         PG_V4(ACT, 1, false, TY);           \
     } while (0)
