@@ -12,6 +12,7 @@
 //
 // Every mbarrier wait is bounded; a warp that gave up goes on through the remaining barriers without computing.
 #include <algorithm>
+#include <type_traits>
 
 #include "pg_async.cuh"
 #include "pg_four.cuh"
@@ -191,41 +192,49 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
             if (ok) {
                 const uint32_t slot_at = ring + (uint32_t)slot * fill_bytes;
                 uint32_t at = slot_at + 16u * (uint32_t)(4 * r + (t ^ (r >> 1 & 3))), s_at = slot_at + 512u + (uint32_t)r * 4;
-                float sum[NT][4];
+                // (without a way out between the records their loads and products overlap)
+                auto records = [&](auto full) {
+                    constexpr bool whole = decltype(full)::value;
+                    float sum[NT][4];
 #pragma unroll
-                for (int b = 0; b < KWM / 64; b++) {
-                    if (b * 64 >= klen) break;
-                    const uint4 q4 = pg_lds128(at);
-                    const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+                    for (int b = 0; b < KWM / 64; b++) {
+                        if (!whole && b * 64 >= klen) break;
+                        const uint4 q4 = pg_lds128(at);
+                        const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                        for (int h = 0; h < 2; h++) {
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const uint32_t w0 = u ? q[h] >> 8 : q[h], w1 = u ? q[2 + h] >> 8 : q[2 + h];
-                            const uint32_t a0 = four_f16_lo(w0), a1 = four_f16_lo(w1), a2 = four_f16_hi(w0), a3 = four_f16_hi(w1);
-                            const int i = 8 * b + 4 * h + 2 * u;
-                            if ((2 * b + h) % G32 == 0 && u == 0) {
-                                four_mma_f16_first(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);
-                                if (NT == 2 && (!ROUTED || second)) four_mma_f16_first(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][i], x[NT - 1][i + 1]);
-                            } else {
-                                four_mma_f16(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);
-                                if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][i], x[NT - 1][i + 1]);
+                            for (int u = 0; u < 2; u++) {
+                                const uint32_t w0 = u ? q[h] >> 8 : q[h], w1 = u ? q[2 + h] >> 8 : q[2 + h];
+                                const uint32_t a0 = four_f16_lo(w0), a1 = four_f16_lo(w1), a2 = four_f16_hi(w0), a3 = four_f16_hi(w1);
+                                const int i = 8 * b + 4 * h + 2 * u;
+                                if ((2 * b + h) % G32 == 0 && u == 0) {
+                                    four_mma_f16_first(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);
+                                    if (NT == 2 && (!ROUTED || second)) four_mma_f16_first(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][i], x[NT - 1][i + 1]);
+                                } else {
+                                    four_mma_f16(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);
+                                    if (NT == 2 && (!ROUTED || second)) four_mma_f16(sum[NT - 1], a0, a1, a2, a3, x[NT - 1][i], x[NT - 1][i + 1]);
+                                }
+                            }
+                            if ((2 * b + h + 1) % G32 == 0) { // the group ends behind this half of the record
+                                uint32_t both;                // the scales of rows r and r + 8
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(s_at + (G32 == 1 ? h * 32 : 0)));
+                                const float2 sc = __half22float2(*reinterpret_cast<const __half2 *>(&both));
+#pragma unroll
+                                for (int n = 0; n < NT; n++) {
+                                    if (n == 1 && ROUTED && !second) break;
+                                    acc[n][0] = fmaf(sc.x, sum[n][0], acc[n][0]), acc[n][1] = fmaf(sc.x, sum[n][1], acc[n][1]);
+                                    acc[n][2] = fmaf(sc.y, sum[n][2], acc[n][2]), acc[n][3] = fmaf(sc.y, sum[n][3], acc[n][3]);
+                                }
                             }
                         }
-                        if ((2 * b + h + 1) % G32 == 0) { // the group ends behind this half of the record
-                            uint32_t both;                // the scales of rows r and r + 8
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(both) : "r"(s_at + (G32 == 1 ? h * 32 : 0)));
-                            const float2 sc = __half22float2(*reinterpret_cast<const __half2 *>(&both));
-#pragma unroll
-                            for (int n = 0; n < NT; n++) {
-                                if (n == 1 && ROUTED && !second) break;
-                                acc[n][0] = fmaf(sc.x, sum[n][0], acc[n][0]), acc[n][1] = fmaf(sc.x, sum[n][1], acc[n][1]);
-                                acc[n][2] = fmaf(sc.y, sum[n][2], acc[n][2]), acc[n][3] = fmaf(sc.y, sum[n][3], acc[n][3]);
-                            }
-                        }
+                        at += record, s_at += record;
                     }
-                    at += record, s_at += record;
-                }
+                };
+                if (klen == KWM)
+                    records(std::true_type{});
+                else
+                    records(std::false_type{});
                 __syncwarp();                             // every lane has read the slot
                 if (j + slots < total) issue();
                 if (++slot == slots) slot = 0, phase ^= 1;
