@@ -53,7 +53,8 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b)
 
 // ---- rows of a as f16 over a power of two: a CTA per row of a.  With a route: to the rows of the token's pairs, or (by_token == 0) per pair; rows
 // without a pair keep what is there, and nobody reads their outputs -----------------------------------------------------------------
-constexpr int RW_T = 128, RW_KEEP = 4;
+constexpr int RW_KEEP = 4;
+template <int RW_T>
 __global__ void __launch_bounds__(RW_T)
     linear4_rows_kernel(const bf16 *__restrict__ a, int64_t lda, int k, const PgRouted rt, const int32_t *pair_row, uint4 *__restrict__ out, float *__restrict__ back)
 {
@@ -126,12 +127,12 @@ struct Piece {
 
 // A warp's sums of weight rows n0 + lane with rows m0 .. of a (`left` of them exist) -> outputs
 template <int COLS, int ACT, bool ALL, typename TY>
-__device__ __forceinline__ void put_rows(const float (&v)[COLS], float fac, const float *xback, int m0, int left, bool in, TY *dst, int64_t ldy, int lane)
+__device__ __forceinline__ void put_rows(const float (&v)[COLS], float fac, const float (&xback)[COLS / 16], int left, bool in, TY *dst, int64_t ldy)
 {
 #pragma unroll
     for (int c = 0; c < COLS; c += 16) {
         if (!ALL && c >= left) break;                      // uniform over the warp
-        const float xb = ALL || (lane & 15) < left - c ? __ldcg(xback + m0 + c + (lane & 15)) : 0.0f;
+        const float xb = xback[c / 16];
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const float o = v[c + j] * fac * __shfl_sync(0xffffffffu, xb, j);
@@ -141,15 +142,16 @@ __device__ __forceinline__ void put_rows(const float (&v)[COLS], float fac, cons
     }
 }
 template <int COLS, int ACT, typename TY>
-__device__ __forceinline__ void put(const float (&v)[COLS], float fac, const float *xback, int m0, int left, int n0, int N, float limit, TY *y, int64_t ldy, int lane)
+__device__ __forceinline__ void put(const float (&v)[COLS], float fac, const float (&xback)[COLS / 16], int m0, int left, int n0, int N, float limit, TY *y, int64_t ldy,
+                                    int lane)
 {
     const bool in = n0 + lane < N;
     if constexpr (ACT == PG_ACT_NONE) {
         TY *dst = y + (int64_t)m0 * ldy + n0 + lane;
         if (left >= COLS)
-            put_rows<COLS, ACT, true>(v, fac, xback, m0, left, in, dst, ldy, lane);
+            put_rows<COLS, ACT, true>(v, fac, xback, left, in, dst, ldy);
         else
-            put_rows<COLS, ACT, false>(v, fac, xback, m0, left, in, dst, ldy, lane);
+            put_rows<COLS, ACT, false>(v, fac, xback, left, in, dst, ldy);
     } else {
         // lanes l and l ^ 8 have a gate and its up: the gate's lane takes the even rows, the other the odd ones
         const bool up = lane & 8;
@@ -157,7 +159,7 @@ __device__ __forceinline__ void put(const float (&v)[COLS], float fac, const flo
 #pragma unroll
         for (int c = 0; c < COLS; c += 16) {
             if (c >= left) break;                          // uniform over the warp
-            const float xb = (lane & 15) < left - c ? __ldcg(xback + m0 + c + (lane & 15)) : 0.0f;
+            const float xb = xback[c / 16];
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
                 const float v0 = v[c + j] * fac * __shfl_sync(0xffffffffu, xb, j), v1 = v[c + j + 1] * fac * __shfl_sync(0xffffffffu, xb, j + 1);
@@ -454,6 +456,9 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
             for (int64_t at = at0; ok && next(at, p);) {
                 const int m0 = p.tile % tiles_m * BN + half * COLS, n0 = (p.tile / tiles_m * CG + rank) * BM + q * 32;
                 const float fac = n0 + lane < wtiles * 16 ? __ldg(wrow + (int64_t)(w_tile(p.tile) + q * 2) * 16 + lane) : 0.0f;
+                float xb[COLS / 16];                           // of rows m0 + 16 c + (lane & 15)
+#pragma unroll
+                for (int c = 0; c < COLS / 16; c++) xb[c] = m0 + 16 * c + (lane & 15) < rows ? __ldcg(xback + m0 + 16 * c + (lane & 15)) : 0.0f;
                 float sum[COLS];
                 for (int left = p.k1 - p.k0, first = 1; left > 0; left -= CHUNK, first = 0) {
                     if (!(ok = pg_mbar_wait_warp(bar_tfull + 8 * acc, acc_phase, abort_flag, status, limit_ns))) break;
@@ -473,7 +478,7 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
                 if (n0 >= N || m0 >= rows) {
                     // (nothing of the warp's piece lies inside y)
                 } else if (p.k1 - p.k0 == kblocks) {
-                    put<COLS, ACT>(sum, fac, xback, m0, rows - m0, n0, N, limit, y, ldy, lane);
+                    put<COLS, ACT>(sum, fac, xb, m0, rows - m0, n0, N, limit, y, ldy, lane);
                 } else {
                     // the tile's pairs: a pair's piece is the first of its stretch unless that starts at the tile's beginning or in front of it
                     const int64_t b0 = (int64_t)p.tile * kblocks;
@@ -498,18 +503,27 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
                             float a[16];
 #pragma unroll
                             for (int j = 0; j < 16; j++) a[j] = 0.0f;
-                            for (int pair = lo; pair <= hi; pair++) {
-                                const float *from = slab_of(pair) + c * 32;
-                                float b[16];
+                            // (as many pairs' sums on their way at once as registers allow)
+                            constexpr int AHEAD = COLS == 64 ? 3 : COLS == 32 ? 2 : 4;
+                            for (int pair = lo; pair <= hi; pair += AHEAD) {
+                                float b[AHEAD][16];
 #pragma unroll
-                                for (int j = 0; j < 16; j++) b[j] = __ldcg(from + j * 32);
+                                for (int u = 0; u < AHEAD; u++) {
+                                    const float *from = slab_of(min(pair + u, hi)) + c * 32;
 #pragma unroll
-                                for (int j = 0; j < 16; j++) a[j] += b[j];
+                                    for (int j = 0; j < 16; j++) b[u][j] = __ldcg(from + j * 32);
+                                }
+#pragma unroll
+                                for (int u = 0; u < AHEAD; u++)
+                                    if (pair + u <= hi) {
+#pragma unroll
+                                        for (int j = 0; j < 16; j++) a[j] += b[u][j];
+                                    }
                             }
 #pragma unroll
                             for (int j = 0; j < 16; j++) sum[c + j] = a[j];
                         }
-                        put<COLS, ACT>(sum, fac, xback, m0, rows - m0, n0, N, limit, y, ldy, lane);
+                        put<COLS, ACT>(sum, fac, xb, m0, rows - m0, n0, N, limit, y, ldy, lane);
                     }
                 }
             }
@@ -595,7 +609,9 @@ int32_t pgk_linear4_tc(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int64_
     int32_t rc = pg_scratch_reserve_recording(ctx, xbytes + (size_t)m * sizeof(float));
     if (rc != PG_OK) return rc;
     float *back = reinterpret_cast<float *>((unsigned char *)ctx->scratch + xbytes);
-    rc = launch_pdl(ctx, linear4_rows_kernel, dim3((unsigned)(route ? rt.by_token ? route->m : pairs : m)), dim3(RW_T), 0, a, lda, (int)lin->k, rt,
+    // (a row's loads all on their way at once: up to 4096 columns with 128 threads, up to 16384 with 512)
+    const bool wide = lin->k > 128 * RW_KEEP * 8;
+    rc = launch_pdl(ctx, wide ? linear4_rows_kernel<512> : linear4_rows_kernel<128>, dim3((unsigned)(route ? rt.by_token ? route->m : pairs : m)), dim3(wide ? 512 : 128), 0, a, lda, (int)lin->k, rt,
                     route ? (const int32_t *)route->pair_row : (const int32_t *)nullptr, (uint4 *)ctx->scratch, back);
     if (rc != PG_OK) return rc;
     if (act == PG_ACT_GELU_TANH_GLU) return dispatch<PG_ACT_GELU_TANH_GLU, bf16>(ctx, lin, ctx->scratch, back, m, limit, (bf16 *)y, ldy, rt, pairs);
