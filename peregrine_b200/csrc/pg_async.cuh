@@ -76,6 +76,12 @@ __device__ __forceinline__ void pg_mbar_arrive_warp(uint32_t bar, int lane)
     __syncwarp();
     asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"(lane) : "memory");
 }
+// the same, `count` arrivals
+__device__ __forceinline__ void pg_mbar_arrive_warp_n(uint32_t bar, int lane, uint32_t count)
+{
+    __syncwarp();
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0], %2;\n\t}" ::"r"(bar), "r"(lane), "r"(count) : "memory");
+}
 __device__ __forceinline__ void pg_bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
 {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),

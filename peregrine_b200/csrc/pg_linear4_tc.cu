@@ -31,8 +31,8 @@ struct Cfg {
     static constexpr int TEAMS = BN > 64 ? 2 : 3;         // of unpacking warps, four warps each; they take the blocks in turn
     static constexpr int SLOTS = 2 * TEAMS;               // blocks in flight: activations in shared memory, unpacked weights in TMEM (64 columns each)
     static constexpr int OUT = W_UNPACK + 4 * TEAMS, THREADS = (OUT + 8) * 32;
-    static constexpr int DEPTH = 14;                      // blocks in the weights' ring
-    static constexpr int RING = DEPTH * W_BLOCK;
+    static constexpr int DEPTH = 7;                       // entries of the weights' ring, two blocks each
+    static constexpr int RING = DEPTH * 2 * W_BLOCK;
     static constexpr int XT = BN / CG * 128;              // 64 columns of a block of the activations, a CTA's half
     static constexpr int A_COL = 2 * BN;                  // behind the two accumulators
     static constexpr size_t SMEM = (size_t)SLOTS * 2 * XT + RING + 1024 + (2 * SLOTS + 5 + 2 * DEPTH) * 8;
@@ -236,17 +236,20 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
         }
         for (int i = 0; i < DEPTH; i++) {
             pg_mbar_init(bar_w + 8 * i, 1);
-            pg_mbar_init(bar_read + 8 * i, 4);             // the warps of a team
+            pg_mbar_init(bar_read + 8 * i, 8);             // the warps of a team, for each of two blocks
         }
         *abort_flag = 0;
         pg_mbar_fence();
     }
-    __syncwarp();
+    __syncthreads();
     if (warp == W_MMA) tmem_alloc<CG>(pg_smem(tmem_slot), 512);
     tc_fence_before();
-    pg_group_sync<CG>();
+    // (the warps that bring weights need neither the other CTA nor TMEM: they wait at their end)
+    const bool early = warp >= W_WEIGHTS && warp < W_UNPACK;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (!early) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const uint32_t tmem = early ? 0u : __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const bool routed = rt.blocks != nullptr;
     if (routed) asm volatile("griddepcontrol.wait;" ::: "memory");   // the list of tiles comes from the preceding kernels
     constexpr int PER_BLOCK = PG_ROUTE_BLOCK / BN;
@@ -306,29 +309,30 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
                 }
             }
         } else if (warp >= W_WEIGHTS) {
-            // ------------------------------------------------------------ weights: every second block, a 16-row tile's two records by a lane each
-            // (Copied by the warps that unpack them, a lane's two copies took 450 cycles of a block's 2700; tensor copies of the tile, issued by one
-            // thread, 385 to 520 per 64 k.)
+            // ------------------------------------------------------------ weights: every second entry, a 16-row tile's four records by a lane each
+            // (A copy's issue takes its lane some 200 cycles whatever its size, and a warp's lanes follow one another.  An entry per block: 2048 rows of
+            // 28672 x 4096 449 us instead of 430.  Copied by the warps that unpack, a lane's two copies took 450 cycles of a block's 2700.)
             int64_t at = at0;
             Piece p = {0, 0, 0};
-            int kb = warp - W_WEIGHTS;
-            uint32_t entry = (uint32_t)kb, phase = 1;
+            int e = warp - W_WEIGHTS;                      // the warp's next entry of the piece
+            uint32_t entry = (uint32_t)e, phase = 1;
             bool ok = true;
             while (ok) {
                 bool more = true;
-                while (kb >= p.k1 && more) {
-                    kb -= p.k1;
-                    if ((more = next(at, p))) kb += p.k0;
+                for (int n; more && e >= (n = (p.k1 - p.k0 + 1) / 2);) {
+                    e -= n;
+                    more = next(at, p);
                 }
                 if (!more) break;
                 // (rows behind the last weights repeat the last ones, whose sums are dropped)
                 const unsigned char *from = w + (int64_t)min(w_tile(p.tile) + (lane & 7), alltiles - 1) * (K / 64) * record;
-                for (; kb < p.k1; kb += 2) {
+                for (; p.k0 + 2 * e < p.k1; e += 2) {
                     if (!(ok = pg_mbar_wait_warp(bar_read + 8 * entry, phase, abort_flag, status, limit_ns))) break;
-                    const uint32_t bytes = (uint32_t)(odd && kb == kblocks - 1 ? record : 2 * record), bar = bar_w + 8 * entry;
+                    const int kb = p.k0 + 2 * e, end = min(kb + 2, p.k1);
+                    const uint32_t bytes = (uint32_t)((2 * (end - kb) - (odd && end == kblocks ? 1 : 0)) * record), bar = bar_w + 8 * entry;
                     if (lane == 0) pg_mbar_expect(bar, 8 * bytes);
                     __syncwarp();
-                    if (lane < 8) pg_bulk_load(base + SLOTS * 2 * C::XT + entry * W_BLOCK + (uint32_t)lane * 2 * record, from + (int64_t)(2 * kb) * record, bytes, bar);
+                    if (lane < 8) pg_bulk_load(base + SLOTS * 2 * C::XT + entry * (2 * W_BLOCK) + (uint32_t)lane * 4 * record, from + (int64_t)(2 * kb) * record, bytes, bar);
                     entry += 2;
                     if (entry >= (uint32_t)DEPTH) entry -= DEPTH, phase ^= 1;
                 }
@@ -339,6 +343,8 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
                 while (pg_globaltimer_ns() - t0 < 2000000ull) {
                 }
             }
+            __syncwarp();
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         } else if (warp == W_MMA && rank == 0) {
             // ------------------------------------------------------------ products (the whole warp; one lane's count)
             // This warp shares its scheduler with four that unpack and two that write: every instruction here counts, so one wait and one
@@ -379,9 +385,9 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
         // ---------------------------------------------------------------- quants -> f16 in TMEM: a thread per weight row
         if constexpr (C::SHARES) set_regs_less<C::R_UNPACK>();
         const int team = (warp - W_UNPACK) >> 2, quarter = warp & 3, ti = lane >> 4, rr = lane & 15;
-        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(quarter * 4 * record);
-        const uint32_t off = (uint32_t)(ti * 2 * record + (rr & 7) * 64 + (rr >> 3) * 8), swz = (uint32_t)(rr >> 1 & 3) << 4;
-        const uint32_t s_off = (uint32_t)(ti * 2 * record + 512 + (rr & 7) * 4 + (rr >> 3) * 2), s_step = record > 544 ? 32u : 0u;
+        const uint32_t ring = base + SLOTS * 2 * C::XT + (uint32_t)(quarter * 8 * record);
+        const uint32_t off = (uint32_t)(ti * 4 * record + (rr & 7) * 64 + (rr >> 3) * 8), swz = (uint32_t)(rr >> 1 & 3) << 4;
+        const uint32_t s_off = (uint32_t)(ti * 4 * record + 512 + (rr & 7) * 4 + (rr >> 3) * 2), s_step = record > 544 ? 32u : 0u;
         const uint32_t q_off[4] = {off + swz, off + (16u ^ swz), off + (32u ^ swz), off + (48u ^ swz)};
         const uint32_t a_at = tmem + ((uint32_t)(quarter * 32) << 16) + C::A_COL + team * 64, full = pg_leader<CG>(bar_full) + 8 * team, free_at = bar_free + 8 * team;
         uint32_t turn = 0;                                     // which of the team's two slots
@@ -389,12 +395,13 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
         int64_t read_at = at0;
         Piece now = {0, 0, 0};
         int rb = team;
-        uint32_t phase = 1, entry = (uint32_t)team, w_phase = 0;
+        uint32_t phase = 1, entries = 0;                       // entries: of the pieces in front of this one
         bool ok = true;
 #pragma unroll 1
         for (;; rb += TEAMS) {
             while (rb >= now.k1) {
                 rb -= now.k1;
+                entries += (uint32_t)(now.k1 - now.k0 + 1) >> 1;
                 if (!next(read_at, now)) {
                     rb = -1;
                     break;
@@ -403,8 +410,9 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
             }
             if (rb < 0) break;
             const int halves = odd && rb == kblocks - 1 ? 1 : 2;
-            if (!(ok = pg_mbar_wait_warp(bar_w + entry * 8, w_phase, abort_flag, status, limit_ns))) break;
-            uint32_t at = ring + entry * W_BLOCK, to_tmem = a_at + turn * (64 * TEAMS);
+            const uint32_t in = (uint32_t)(rb - now.k0), nth = entries + (in >> 1), entry = nth % DEPTH;
+            if (!(ok = pg_mbar_wait_warp(bar_w + entry * 8, nth / DEPTH & 1, abort_flag, status, limit_ns))) break;
+            uint32_t at = ring + entry * (2 * W_BLOCK) + (in & 1) * 2 * (uint32_t)record, to_tmem = a_at + turn * (64 * TEAMS);
 #pragma unroll 1
             for (int c = 0; c < halves; c++) {                 // 64 columns, then 32 at a time: word e of the row's four lanes
                 uint2 q[4];
@@ -434,12 +442,10 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
                 at += record, to_tmem += 32;
             }
             if (!ok) break;
-            pg_mbar_arrive_warp(bar_read + entry * 8, lane);
+            pg_mbar_arrive_warp_n(bar_read + entry * 8, lane, (in & 1) == 0 && rb + 1 == now.k1 ? 2u : 1u);
             tmem_wait_st();
             tc_fence_before();
             pg_arrive_leader_warp<CG>(full + turn * (8 * TEAMS), lane);
-            entry += TEAMS;
-            if (entry >= (uint32_t)DEPTH) entry -= DEPTH, w_phase ^= 1;
             phase ^= turn;
             turn ^= 1;
         }
