@@ -752,8 +752,15 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
     if (!last_in) return;
     __threadfence();
     if (threadIdx.x == 0) tickets[unit] = 0;
-    // a warp per row: the slices' weights; then all columns with their loads in flight together
+    // a warp per row: the slices' weights; then all columns, eight slices' loads in flight, the first eight's while the weights are found
     const float *parts = part + unit * S * 16 * ms;
+    float4 v[8];
+    auto load = [&](int x, int k0) {
+        const float *from = parts + (size_t)(x / vq) * ms + (x % vq) * 4;
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)min(k0 + k, used - 1) * 16 * ms));
+    };
+    if (threadIdx.x < count * vq) load(threadIdx.x, 0);
     for (int c = warp; c < count; c += A4_WARPS) {
         float2 ml[A4_SLICES / 32];
         float top = s.sink ? 0.0f : -INFINITY, sum = 0.0f;
@@ -777,12 +784,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
     __syncthreads();
     for (int x = threadIdx.x; x < count * vq; x += A4_WARPS * 32) {
         const int c = x / vq, col = (x - c * vq) * 4;
-        const float *from = parts + (size_t)c * ms + col;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < used; k0 += 8) {            // eight loads in flight; behind the last slice its weight is 0
-            float4 v[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)min(k0 + k, used - 1) * 16 * ms));
+        for (int k0 = 0; k0 < used; k0 += 8) {            // (behind the last slice its weight is 0)
+            if (x != (int)threadIdx.x || k0 > 0) load(x, k0);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const float by = k0 + k < used ? weight[c][k0 + k] : 0.0f;
@@ -807,7 +811,7 @@ Four four_of(const AttnShape &s)
 int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s)
 {
     const int64_t cap = s.chunk && s.chunk < s.cap ? s.chunk : s.cap;
-    const int64_t S = std::min<int64_t>(2 * (int64_t)ctx->sm_count / std::max<int64_t>(1, units), cap / 256);
+    const int64_t S = std::min<int64_t>(2 * (int64_t)ctx->sm_count / std::max<int64_t>(1, units), (cap + 255) / 256);
     return (int)std::max<int64_t>(1, std::min<int64_t>(S, A4_SLICES));
 }
 
