@@ -370,10 +370,14 @@ __device__ __forceinline__ void load_scales(uint32_t (&v)[N], uint32_t at, int g
 // ---- few tokens: grid (slices, G * blocks of 16 rows, seqs) --------------------------------------------------------------------
 constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // most fills in flight of a warp; tiles of a fill
 
+// CTAs to an SM.  More than eight rows of heads wider than 64: one with 255 registers a lane, as two with 128 spill (32 + 8 heads of 128, 16 x 4 tokens at
+// 4096: 36.7 us instead of 64).  Up to eight rows keep two: one is slower in long contexts (4 at 60000: 85 instead of 75), faster in short ones (2000: 8.3, 9.3).
+__host__ __device__ constexpr int a4_per_sm(int gk, int gv, bool hi) { return gk > 4 || gv > 4 || (hi && gk + gv > 4) ? 1 : 2; }
+
 // part [(seq, block)][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row
 // EXACT: GK and GV are the groups of the layer, else at least as many
 template <int GK, int GV, bool HI, bool FUSED, bool EXACT>
-__global__ void __launch_bounds__(A4_WARPS * 32, GK > 4 || GV > 4 ? 1 : 2)
+__global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
     attn4_few_kernel(const AttnShape s, const Four f, const pg_batch bt, int few, int stages, const float *__restrict__ proj, int64_t ldp, unsigned char *kc, unsigned char *vc,
                      float *part, int32_t *tickets, bf16 *__restrict__ out, int64_t ldo, int32_t *status, unsigned long long limit_ns)
 {
@@ -807,11 +811,11 @@ Four four_of(const AttnShape &s)
     return f;
 }
 
-// slices of the context: about two CTAs per SM, none shorter than 256 positions
-int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s)
+// slices of the context: as many CTAs as SMs take at once, none shorter than 256 positions
+int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s, int per_sm)
 {
     const int64_t cap = s.chunk && s.chunk < s.cap ? s.chunk : s.cap;
-    const int64_t S = std::min<int64_t>(2 * (int64_t)ctx->sm_count / std::max<int64_t>(1, units), (cap + 255) / 256);
+    const int64_t S = std::min<int64_t>(per_sm * (int64_t)ctx->sm_count / std::max<int64_t>(1, units), (cap + 255) / 256);
     return (int)std::max<int64_t>(1, std::min<int64_t>(S, A4_SLICES));
 }
 
@@ -825,7 +829,7 @@ int32_t run_few(pg_ctx *ctx, const AttnShape &s, const Four &f, const pg_batch *
     const int smem = std::max(rings + 16 * (f.gk * 32 + 8) * 2, A4_WARPS * 16 * (f.gv * 32 + 4) * 4);
     static std::atomic<uint64_t> set{0};
     PG_CUDA(pg_max_smem_once(kern, 220 * 1024, ctx->device, set));   // (widths of 256: 157 KB)
-    const int S = slices(ctx, (int64_t)bt->seqs * s.G * blocks, s);
+    const int S = slices(ctx, (int64_t)bt->seqs * s.G * blocks, s, a4_per_sm(GK, GV, HI));
     return launch_pdl(ctx, kern, dim3((unsigned)S, (unsigned)(s.G * blocks), (unsigned)bt->seqs), dim3(A4_WARPS * 32), (size_t)smem, s, f, *bt, few, stages, proj, ldp, kc,
                       vc, part, tickets, out, ldo, ctx->d_status, ctx->wait_limit_ns);
 }
