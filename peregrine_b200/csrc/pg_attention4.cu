@@ -344,12 +344,6 @@ __device__ __forceinline__ void mma_from(float (&d)[4], const float4 &c, uint32_
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
-__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
 
 // the scales of a pair of positions, all groups'
 template <int N, bool EXACT>
@@ -508,18 +502,15 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
             }
         }
     }
-    float o[GV][2][NT][4], l[NT][4];
+    float o[GV][2][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            l[n][j] = 0.0f;
+        for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int i = 0; i < GV; i++) o[i][0][n][j] = o[i][1][n][j] = 0.0f;
-        }
-    constexpr uint32_t ONES = 0x3f803f80u;                // two bf16 ones
     // of the lane's rows r (and r + 8): factor of the scores, last row of the cache seen, slope
-    float fac[NT], m[NT], bias[NT];
+    float fac[NT], m[NT], l[NT], bias[NT];
     int seen[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -527,7 +518,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
         fac[n] = back[c];
         seen[n] = x0 + pos0 + idx / s.rep - low;
         bias[n] = s.slopes ? __ldg(s.slopes + g * s.rep + idx % s.rep) * LOG2E : 0.0f;
-        m[n] = -1e30f;                                    // (finite: exp2(-inf - m) is 0 where a row sees nothing of a slice)
+        m[n] = -1e30f, l[n] = 0.0f;                       // (finite: exp2(-inf - m) is 0 where a row sees nothing of a slice)
     }
     const int sees_all = x0 + pos0 + block * 16 / s.rep - low;        // of the block's first row: every row sees that far
     bool ok = true;
@@ -624,21 +615,20 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
                         // sums lie by row as columns: 2 t and 2 t + 1 of every eight
                         const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
                         auto less = [&](float (&v)[4]) { v[0] *= c0, v[1] *= c1, v[2] *= c0, v[3] *= c1; };
-                        less(l[u]);
+                        l[u] *= corr;
 #pragma unroll
                         for (int x = 0; x < GV; x++) less(o[x][0][u]), less(o[x][1][u]);
                     }
                 }
-                // probabilities, rounded to bf16: their sums are those of the rounded ones, so that a row's weights still add up to one
-                uint32_t p[JT][NT][2];
 #pragma unroll
                 for (int h = 0; h < JT; h++)
 #pragma unroll
-                    for (int u = 0; u < NT; u++) {
+                    for (int n = 0; n < 2; n++)
 #pragma unroll
-                        for (int n = 0; n < 2; n++) p[h][u][n] = pg_pack_bf16(pg_ex2(sc[h][n][2 * u] - m[u]), pg_ex2(sc[h][n][2 * u + 1] - m[u]));
-                        pg_mma_bf16(l[u], ONES, ONES, ONES, ONES, p[h][u][0], p[h][u][1]);
-                    }
+                        for (int j = 0; j < 2 * NT; j++) {
+                            sc[h][n][j] = pg_ex2(sc[h][n][j] - m[j >> 1]);
+                            l[j >> 1] += sc[h][n][j];
+                        }
                 // O^T += V^T P'^T, P' a probability times its value's scale
 #pragma unroll
                 for (int h = 0; h < JT; h++) {
@@ -654,9 +644,10 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
                         for (int n = 0; n < 2; n++) {
 #pragma unroll
                             for (int u = 0; u < NT; u++) {
-                                b[u][n] = mul_bf16(p[h][u][n], scales[n][x]);
+                                float p0 = sc[h][n][2 * u] * pg_bf16_lo(scales[n][x]), p1 = sc[h][n][2 * u + 1] * pg_bf16_hi(scales[n][x]);
                                 // (what a row does not see may hold anything)
-                                if (edge) b[u][n] &= ((p[h][u][n] & 0xffffu) ? 0xffffu : 0u) | ((p[h][u][n] >> 16) ? 0xffff0000u : 0u);
+                                if (edge) p0 = sc[h][n][2 * u] == 0.0f ? 0.0f : p0, p1 = sc[h][n][2 * u + 1] == 0.0f ? 0.0f : p1;
+                                b[u][n] = pg_pack_bf16(p0, p1);
                             }
                         }
                         uint32_t w[2];
@@ -702,8 +693,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
     }
 #pragma unroll
     for (int u = 0; u < NT; u++) {
-        if (t == 0) w0[(r + 8 * u) * ms + vs] = m[u];
-        if (r == 0) w0[(8 * u + 2 * t) * ms + vs + 1] = l[u][0], w0[(8 * u + 2 * t + 1) * ms + vs + 1] = l[u][1];
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+        if (t == 0) w0[(r + 8 * u) * ms + vs] = m[u], w0[(r + 8 * u) * ms + vs + 1] = l[u];
     }
     __syncthreads();
     const int64_t unit = (int64_t)seq * gridDim.y + blockIdx.y;

@@ -2,8 +2,8 @@
 
 Bounds.  What the cache holds is read back, and the outputs are compared with attention over exactly that.  Few tokens: a query enters as f16
 (half a step, 2^-11 of a value), so a score is off by ds <= 2^-11 scale sum |q k| and what the f32 sums lose (2^-18 of the same); a probability
-is rounded to bf16 (2^-8), and divided by the sum of the rounded ones, which is off by no more, and its product with a value's scale is rounded
-again (2^-8).  With A = sum p |v| / l an output is off by A (2 ds + 3 * 2^-8) at most, and rounded once (2^-8 of itself).  Longer portions: queries, keys and values are bf16 each, so ds <= 2 * 2^-8 scale sum |q k|, and A (2 ds + 2 * 2^-8)."""
+times a value's scale is rounded to bf16 (2^-8).  With A = sum p |v| / l an output is off by A (2 ds + 2^-8) at most, and rounded once
+(2^-8 of itself).  Longer portions: queries, keys and values are bf16 each, so ds <= 2 * 2^-8 scale sum |q k|, and A (2 ds + 2 * 2^-8)."""
 import ctypes as C
 import math
 
@@ -137,7 +137,7 @@ class Case:
                     out[at, h] = p @ v / l
                     A = p @ np.abs(v) / l
                     e = math.expm1(2 * ds)
-                    b = A * (e + (2.0 ** -11 if half else 3 * 2.0 ** -8 if few else 2 * 2.0 ** -8) * (1 + e) + 2.0 ** -17)
+                    b = A * (e + (2.0 ** -11 if half else 2.0 ** -8 if few else 2 * 2.0 ** -8) * (1 + e) + 2.0 ** -17)
                     if half:
                         b = b + 2.0 ** -24 * np.abs(v).sum(0) * (1 + e)
                     bound[at, h] = b + 2.0 ** -8 * (np.abs(out[at, h]) + b)

