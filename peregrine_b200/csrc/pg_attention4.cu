@@ -9,9 +9,13 @@
 // O^T = V^T P^T, so that a lane's probabilities are the B operand as they come.  A byte belongs to one position: appending is byte stores.
 //
 //   few tokens of a sequence    attn4_few_kernel: streams the cache once, a block of 16 (token, head of the group) rows per CTA, the context in slices.
-//                               Keys as f16 integers (exact) times the query as f16 over a power of two, sums of 32 columns scaled in f32; values as
-//                               bf16 integers (exact) times bf16(probability * scale).  One token per sequence (FUSED): the CTA with the newest
-//                               position quantises and appends it.  The last CTA of a (sequence, rows) to finish merges the slices.
+//                               Keys as f16 (exact: a quant as the low bits of an f16 number) times the query as f16 over a power of two, sums of 32
+//                               columns scaled in f32; values as bf16 integers (exact) times bf16(probability * scale).  One token per sequence
+//                               (FUSED): the CTA with the newest position quantises and appends it.  The last CTA of a (sequence, rows) to finish
+//                               merges the slices.  What bounds it, 32 + 8 heads of 128: instructions, 300 to a tile of 16 positions and 128 + 128
+//                               columns, of which 64 take the quants apart (four bits at a time, the integer pipe at half rate); 4 contexts of 30000 to
+//                               60000 71 us, 3.1 TB/s of 6.5, 16 of 2048 to 4096 31 us.  One of 2000: 10 us, a launch and seven dependent trips to
+//                               memory (positions, tiles, slices' sums, tickets, the merge).
 //   longer portions             attn4_append_kernel, then per sequence attn4_unfold_kernel and the kernels that prompts over a bf16 cache run through, on
 //                               f16: keys and values over a power of two of their head, which is exact, queries over one of their own.
 #include <algorithm>
@@ -361,18 +365,18 @@ __device__ __forceinline__ void load_scales(uint32_t (&v)[N], uint32_t at, int g
     }
 }
 
-// ---- few tokens: grid (slices, G * blocks of 16 rows, seqs) --------------------------------------------------------------------
-constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // most fills in flight of a warp; tiles of a fill
+// ---- few tokens: grid (slices of all sequences, G * blocks of 16 rows) --------------------------------------------------------------------
+constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // most fills in flight of a warp; most slices of a context; tiles of a fill
 
 // CTAs to an SM.  More than eight rows of heads wider than 64: one with 255 registers a lane, as two with 128 spill (32 + 8 heads of 128, 16 x 4 tokens at
 // 4096: 36.7 us instead of 64).  Up to eight rows keep two: one is slower in long contexts (4 at 60000: 85 instead of 75), faster in short ones (2000: 8.3, 9.3).
 __host__ __device__ constexpr int a4_per_sm(int gk, int gv, bool hi) { return gk > 4 || gv > 4 || (hi && gk + gv > 4) ? 1 : 2; }
 
-// part [(seq, block)][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row
+// part [blocks of rows][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row
 // EXACT: GK and GV are the groups of the layer, else at least as many
 template <int GK, int GV, bool HI, bool FUSED, bool EXACT>
 __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
-    attn4_few_kernel(const AttnShape s, const Four f, const pg_batch bt, int few, int stages, const float *__restrict__ proj, int64_t ldp, unsigned char *kc, unsigned char *vc,
+    attn4_few_kernel(const AttnShape s, const Four f, const pg_batch bt, int few, int per, int stages, const float *__restrict__ proj, int64_t ldp, unsigned char *kc, unsigned char *vc,
                      float *part, int32_t *tickets, bf16 *__restrict__ out, int64_t ldo, int32_t *status, unsigned long long limit_ns)
 {
     constexpr int NT = HI ? 2 : 1, JT = HI ? 1 : 2;
@@ -385,8 +389,9 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
     __shared__ volatile int abort_flag;
     __shared__ uint8_t new_q[2][256];
     __shared__ bf16 new_s[2][8];
+    __shared__ volatile int kept[4];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int split = blockIdx.x, S = gridDim.x, g = blockIdx.y % s.G, block = blockIdx.y / s.G, seq = blockIdx.z;
+    const int S = gridDim.x, g = blockIdx.y % s.G, block = blockIdx.y / s.G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     const int gk = EXACT ? GK : f.gk, gv = EXACT ? GV : f.gv, kbytes = gk * 288, vbytes = gv * 288, stage = A4_FILL * (kbytes + vbytes), vs = gv * 32;
     const uint32_t ring = pg_smem(smem) + (uint32_t)(warp * stages) * stage, bar = pg_smem(bars) + (uint32_t)warp * A4_STAGES * 8;
@@ -400,21 +405,74 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
     }
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int row0 = __ldcg(bt.d_seq_row0 + seq), T = __ldcg(bt.d_seq_row0 + seq + 1) - row0;
-    const int count = min(16, T * s.rep - block * 16);               // rows: (token, head) = (block * 16 + c) / rep, % rep
-    if (T > few || count <= 0) return;
-    const int pos0 = __ldcg(bt.d_pos + row0), last = pos0 + T - 1;
-    const int64_t slot = __ldcg(bt.d_seq_slot + seq);
-    if (pos0 < 0 || last >= s.limit) {                                // outside the cache: record it, touch nothing (all CTAs of the sequence leave)
-        if (threadIdx.x == 0) atomicExch(status, (int32_t)PG_ERR_INVALID);
-        return;
+    // A sequence's part of this block: count rows (token, head) = (block * 16 + c) / rep, % rep; the cache's rows x0 .. x1 - 1 hold the positions
+    // low .. of them (in a chunked layer T is 1, and a chunk's rows lie together), a0 is the first row of the first fill.
+    struct Seq {
+        int row0 = 0, count = 0, pos0 = 0, low = 0, x0 = 0, x1 = 0, a0 = 0;
+    };
+    auto look = [&](int i, Seq &q) {
+        q.row0 = __ldcg(bt.d_seq_row0 + i);
+        const int T = __ldcg(bt.d_seq_row0 + i + 1) - q.row0;
+        q.count = min(16, T * s.rep - block * 16);
+        if (T > few || q.count <= 0) return false;
+        q.pos0 = __ldcg(bt.d_pos + q.row0);
+        if (q.pos0 < 0 || q.pos0 + T > s.limit) {                     // outside the cache: record it, touch nothing (all CTAs of the sequence leave)
+            atomicExch(status, (int32_t)PG_ERR_INVALID);
+            return false;
+        }
+        q.low = attn_low(s, q.pos0), q.x0 = attn_row(s, q.low), q.x1 = q.x0 + (q.pos0 + (block * 16 + q.count - 1) / s.rep) + 1 - q.low;
+        q.a0 = q.x0 & ~31;
+        return true;
+    };
+    // per > 0: so many slices to every context, in whole fills of all warps (256 rows).  per == 0, single tokens of 2 to 32 sequences: slices of one length,
+    // the shortest of which there are no more than CTAs, found by every warp for itself, a lane to a sequence.  (32 + 8 heads of 128, contexts of 16 sequences
+    // anywhere up to 4096: 27.2 us with equal numbers, 18.8 dealt out; all of 4096: 31.1 both.)
+    int seq, split, used, chunk;
+    int64_t slot = 0;
+    Seq me;
+    if (!FUSED || per) {
+        seq = blockIdx.x / per, split = blockIdx.x - seq * per;
+        slot = __ldcg(bt.d_seq_slot + seq);
+        if (!look(seq, me)) return;
+        chunk = ((me.x1 - me.a0 + per - 1) / per + 255) & ~255;
+        used = (me.x1 - me.a0 + chunk - 1) / chunk;
+        if (split >= used) return;
+    } else {
+        int own = 0;
+        if (lane < bt.seqs) {
+            slot = __ldcg(bt.d_seq_slot + lane);
+            own = look(lane, me) ? (me.x1 - me.a0 + 255) / 256 : 0;
+        }
+        const int all = __reduce_add_sync(0xffffffffu, own), most = __reduce_max_sync(0xffffffffu, own);
+        uint32_t lo = max(1, max((all + S - 1) / S, (most + A4_SLICES - 1) / A4_SLICES)), hi = max((int)lo, most);
+        for (uint32_t mid = lo; lo < hi; mid = (lo + hi) / 2) {       // (the shortest that could be is tried first)
+            if (__reduce_add_sync(0xffffffffu, (own + mid - 1) / mid) <= (uint32_t)S)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        chunk = (int)lo * 256;
+        // this CTA's sequence: the one whose slices hold the CTA's number
+        const int n = (own + lo - 1) / lo;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, upto > (int)blockIdx.x);
+        if (!past) return;
+        seq = __ffs(past) - 1;
+        used = __shfl_sync(0xffffffffu, n, seq);
+        split = (int)blockIdx.x - __shfl_sync(0xffffffffu, upto - n, seq);
+        slot = __shfl_sync(0xffffffffu, slot, seq);
+        me.row0 = __shfl_sync(0xffffffffu, me.row0, seq), me.count = __shfl_sync(0xffffffffu, me.count, seq);
+        me.pos0 = __shfl_sync(0xffffffffu, me.pos0, seq), me.low = __shfl_sync(0xffffffffu, me.low, seq);
+        me.x0 = __shfl_sync(0xffffffffu, me.x0, seq), me.x1 = __shfl_sync(0xffffffffu, me.x1, seq), me.a0 = __shfl_sync(0xffffffffu, me.a0, seq);
     }
-    // rows of the cache: x0 .. x1 - 1 hold the positions low .. of this block (in a chunked layer T is 1, and a chunk's rows lie together)
-    const int low = attn_low(s, pos0), x0 = attn_row(s, low), x1 = x0 + (pos0 + (block * 16 + count - 1) / s.rep) + 1 - low;
-    const int a0 = x0 & ~31;                                          // first row of the first fill
-    const int chunk = ((x1 - a0 + S - 1) / S + 255) & ~255;           // of a slice: a fill for every warp
-    const int t0 = a0 + split * chunk, t1 = min(x1, t0 + chunk), used = (x1 - a0 + chunk - 1) / chunk;
-    if (t0 >= t1) return;
+    const int row0 = me.row0, count = me.count, pos0 = me.pos0, low = me.low, x0 = me.x0, x1 = me.x1;
+    const int t0 = me.a0 + split * chunk, t1 = min(x1, t0 + chunk);
+    if (threadIdx.x == 0) kept[0] = split, kept[1] = used, kept[2] = row0, kept[3] = count;   // (for the end: registers are short in between)
     const bool newest = FUSED && t1 == x1;
     unsigned char *kb = kc + (slot * s.G + g) * f.kh, *vb = vc + (slot * s.G + g) * f.vh;
 
@@ -698,18 +756,20 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
         if (t == 0) w0[(r + 8 * u) * ms + vs] = m[u], w0[(r + 8 * u) * ms + vs + 1] = l[u];
     }
     __syncthreads();
-    const int64_t unit = (int64_t)seq * gridDim.y + blockIdx.y;
-    float *mine_part = part + (unit * S + split) * 16 * ms;
+    // (a sequence's slices are neighbours)
+    const int slices = kept[1], row_at = kept[2], rows = kept[3];
+    const int64_t first = (int64_t)blockIdx.y * S + blockIdx.x - kept[0];
+    float *mine_part = part + ((int64_t)blockIdx.y * S + blockIdx.x) * 16 * ms;
     const int vq = vs / 4;
     auto put = [&](int c, int col, const float4 &a, float by) {
         const int idx = block * 16 + c;
-        bf16 *dst = out + (int64_t)(row0 + idx / s.rep) * ldo + (int64_t)(g * s.rep + idx % s.rep) * s.V + col;
+        bf16 *dst = out + (int64_t)(row_at + idx / s.rep) * ldo + (int64_t)(g * s.rep + idx % s.rep) * s.V + col;
         const float y[4] = {a.x * by, a.y * by, a.z * by, a.w * by};
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (col + i < s.V) pg_put(dst + i, y[i]);
     };
-    for (int x = threadIdx.x; x < count * vq; x += A4_WARPS * 32) {
+    for (int x = threadIdx.x; x < rows * vq; x += A4_WARPS * 32) {
         const int c = x / vq, col = (x - c * vq) * 4;
         float top = -INFINITY;
 #pragma unroll
@@ -724,7 +784,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
             a.x = fmaf(by, v.x, a.x), a.y = fmaf(by, v.y, a.y), a.z = fmaf(by, v.z, a.z), a.w = fmaf(by, v.w, a.w);
             sum = fmaf(by, from[vs + 1], sum);
         }
-        if (used == 1) {
+        if (slices == 1) {
             float by = 1.0f;
             if (s.sink) {
                 const float mm = fmaxf(top, 0.0f);
@@ -737,33 +797,33 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
             if (col == 0) *reinterpret_cast<float2 *>(mine_part + (size_t)c * ms + vs) = make_float2(top, sum);
         }
     }
-    if (used == 1) return;
+    if (slices == 1) return;
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
-        last_in = atomicAdd(tickets + unit, 1) == used - 1;
+        last_in = atomicAdd(tickets + first, 1) == slices - 1;
     }
     __syncthreads();
     if (!last_in) return;
     __threadfence();
-    if (threadIdx.x == 0) tickets[unit] = 0;
+    if (threadIdx.x == 0) tickets[first] = 0;
     // a warp per row: the slices' weights; then all columns, eight slices' loads in flight, the first eight's while the weights are found
-    const float *parts = part + unit * S * 16 * ms;
+    const float *parts = part + first * 16 * ms;
     float4 v[8];
     auto load = [&](int x, int k0) {
         const float *from = parts + (size_t)(x / vq) * ms + (x % vq) * 4;
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)min(k0 + k, used - 1) * 16 * ms));
+        for (int k = 0; k < 8; k++) v[k] = __ldcg(reinterpret_cast<const float4 *>(from + (size_t)min(k0 + k, slices - 1) * 16 * ms));
     };
-    if (threadIdx.x < count * vq) load(threadIdx.x, 0);
-    for (int c = warp; c < count; c += A4_WARPS) {
+    if (threadIdx.x < rows * vq) load(threadIdx.x, 0);
+    for (int c = warp; c < rows; c += A4_WARPS) {
         float2 ml[A4_SLICES / 32];
         float top = s.sink ? 0.0f : -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < A4_SLICES / 32; i++) {
             const int k = i * 32 + lane;
-            ml[i] = k < used ? __ldcg(reinterpret_cast<const float2 *>(parts + ((size_t)k * 16 + c) * ms + vs)) : make_float2(-INFINITY, 0.0f);
+            ml[i] = k < slices ? __ldcg(reinterpret_cast<const float2 *>(parts + ((size_t)k * 16 + c) * ms + vs)) : make_float2(-INFINITY, 0.0f);
             top = fmaxf(top, ml[i].x);
         }
 #pragma unroll
@@ -778,14 +838,14 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
         if (lane == 0) denom[c] = __fdiv_rn(1.0f, sum);
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < count * vq; x += A4_WARPS * 32) {
+    for (int x = threadIdx.x; x < rows * vq; x += A4_WARPS * 32) {
         const int c = x / vq, col = (x - c * vq) * 4;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < used; k0 += 8) {            // (behind the last slice its weight is 0)
+        for (int k0 = 0; k0 < slices; k0 += 8) {            // (behind the last slice its weight is 0)
             if (x != (int)threadIdx.x || k0 > 0) load(x, k0);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float by = k0 + k < used ? weight[c][k0 + k] : 0.0f;
+                const float by = k0 + k < slices ? weight[c][k0 + k] : 0.0f;
                 a.x = fmaf(by, v[k].x, a.x), a.y = fmaf(by, v[k].y, a.y), a.z = fmaf(by, v[k].z, a.z), a.w = fmaf(by, v[k].w, a.w);
             }
         }
@@ -803,12 +863,18 @@ Four four_of(const AttnShape &s)
     return f;
 }
 
-// slices of the context: as many CTAs as SMs take at once, none shorter than 256 positions
-int slices(const pg_ctx *ctx, int64_t units, const AttnShape &s, int per_sm)
+// Slices of all sequences' contexts: as many CTAs as SMs take at once, none shorter than 256 rows.  per: of every context, 0 where they are dealt out
+int slices(const pg_ctx *ctx, int64_t seqs, int64_t rows, const AttnShape &s, int per_sm, bool single, int &per)
 {
     const int64_t cap = s.chunk && s.chunk < s.cap ? s.chunk : s.cap;
-    const int64_t S = std::min<int64_t>(per_sm * (int64_t)ctx->sm_count / std::max<int64_t>(1, units), (cap + 255) / 256);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(S, A4_SLICES));
+    const int64_t most = std::min<int64_t>((cap + 31 + 255) / 256, A4_SLICES), at_once = per_sm * (int64_t)ctx->sm_count / std::max<int64_t>(1, rows);   // (a chunk may begin inside a fill)
+    const int64_t all = std::min(at_once, seqs * most);
+    per = (int)std::max<int64_t>(1, all / std::max<int64_t>(1, seqs));
+    if (single && seqs > 1 && seqs <= 32 && all > seqs) {
+        per = 0;
+        return (int)all;
+    }
+    return (int)(seqs * per);
 }
 
 template <int GK, int GV, bool HI, bool FUSED, bool EXACT>
@@ -820,9 +886,10 @@ int32_t run_few(pg_ctx *ctx, const AttnShape &s, const Four &f, const pg_batch *
     const int fill = A4_WARPS * A4_FILL * (f.kb + f.vb), stages = 3 * fill <= 100 * 1024 ? 3 : 2, rings = stages * fill;
     const int smem = std::max(rings + 16 * (f.gk * 32 + 8) * 2, A4_WARPS * 16 * (f.gv * 32 + 4) * 4);
     static std::atomic<uint64_t> set{0};
-    PG_CUDA(pg_max_smem_once(kern, 220 * 1024, ctx->device, set));   // (widths of 256: 157 KB)
-    const int S = slices(ctx, (int64_t)bt->seqs * s.G * blocks, s, a4_per_sm(GK, GV, HI));
-    return launch_pdl(ctx, kern, dim3((unsigned)S, (unsigned)(s.G * blocks), (unsigned)bt->seqs), dim3(A4_WARPS * 32), (size_t)smem, s, f, *bt, few, stages, proj, ldp, kc,
+    PG_CUDA(pg_max_smem_once(kern, 200 * 1024, ctx->device, set));   // (widths of 256: 157 KB)
+    int per;
+    const int S = slices(ctx, bt->seqs, (int64_t)s.G * blocks, s, a4_per_sm(GK, GV, HI), FUSED, per);
+    return launch_pdl(ctx, kern, dim3((unsigned)S, (unsigned)(s.G * blocks)), dim3(A4_WARPS * 32), (size_t)smem, s, f, *bt, few, per, stages, proj, ldp, kc,
                       vc, part, tickets, out, ldo, ctx->d_status, ctx->wait_limit_ns);
 }
 
@@ -853,7 +920,7 @@ PG_API int64_t pg_cache4_bytes(int32_t width, int64_t positions)
 
 PG_API int64_t pg_attention4_part_floats(pg_ctx *ctx, const pg_attention *p)
 {
-    // (slices only where there are fewer units than two per SM)
+    // (slices only where there are no more CTAs than two per SM)
     return ctx && p && p->vdim > 0 ? (int64_t)2 * ctx->sm_count * 16 * (pg_up(p->vdim, 32) + 4) : 0;
 }
 

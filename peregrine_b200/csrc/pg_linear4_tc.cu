@@ -1,14 +1,17 @@
 // Product y = act(a W^T) with weights of 4 bits (csrc/pg_linear4.cu) and many rows, on the 5th-generation tensor cores.
 //
-//   * The weights are the M side: a pair of CTAs has 256 rows, each unpacks its 128 to f16 in TMEM, 128 k at a time (a thread per row, sixteen warps in
-//     four teams that take the blocks in turn); the activations are the N side, BN rows of f16 in shared memory by TMA, half in each CTA.
+//   * The weights are the M side: a pair of CTAs has 256 rows, each unpacks its 128 to f16 in TMEM, 128 k at a time (a thread per row, two or three
+//     teams of four warps that take the blocks in turn, two blocks of TMEM each); the activations are the N side, BN rows of f16 in shared memory by TMA, half in each CTA.
 //     scale * (q - 8) is an f16 number exactly (csrc/pg_linear4.cu), and linear4_rows_kernel writes the activations as f16 divided by a power of two
 //     per row, which holds bf16 numbers exactly down to 2^-29 of the row's largest: sums are those of the bf16 activations with the weights.
 //   * An accumulator sums up 512 k; eight warps add the accumulators up in f32 registers.  (The tensor cores cut sums off: 4096 k in one
 //     accumulator were 3.9e-6 off 64 bits, 512 at a time 6e-7.)  They write the outputs: lane = weight row, so a store is 32 columns of one row of y.
 //   * Where whole tiles would leave SMs idle, the tiles' blocks of 128 k are divided evenly over the pairs of CTAs; sums of a tile that several share
 //     go to slabs, and the last warp to finish adds them in a fixed order.
-//   * ROUTED: BN rows belong to one expert; pieces of a 128-row block without a row are left out.
+//   * With a route BN rows belong to one expert; pieces of a 128-row block without a row are left out.
+//   * What bounds it: up to some 100 rows the unpacking, 830 cycles for a block of 128 x 128 where its products at BN = 128 are 512 (its steps' latency: more
+//     teams were no faster), and what a call costs besides, some 10 us (rows_kernel 3, first weights 3.5, slabs and outputs 3, pair and TMEM 1.5).
+//     2048 rows of 28672 x 4096: 430 us, 1.12 PFLOP/s of 1.68, the power cap included.
 //
 // Every mbarrier wait is bounded (pg_async.cuh).
 #include <algorithm>

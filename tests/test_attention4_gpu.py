@@ -345,6 +345,45 @@ def test_slices(lm):
     assert not c.d.buffer("attn4.tickets", 1, 1, c.d.torch.int32).any()
 
 
+@pytest.mark.parametrize("H,G,D,V,kw", [(8, 2, 64, 64, {}), (16, 2, 128, 96, {"sink": True}), (4, 1, 64, 64, {"chunk": 1500, "positions": 6000})])
+def test_slices_of_unequal_contexts(lm, H, G, D, V, kw):
+    """Slices are dealt out over the sequences of a step: one long context among short ones, new ones, all equal, more sequences than a warp has lanes,
+    a longer portion and a sequence outside its cache among them."""
+    kw = dict(kw)
+    if kw.get("chunk"):
+        kw["slopes"] = (2.0 ** -np.arange(1, H + 1)).astype(np.float32)
+    cap = 6000
+    c = Case(lm, H + D, H, G, D, V, cap, 40, 256, **kw)
+    lens = [5800, 0, 1, 700, 256, 255, 31, 2600]
+    for s, n in enumerate(lens):
+        if n:
+            c.append(s, 0, c.rows(n))
+    at = list(lens) + [0] * 32
+    for slots in ([0], [7, 0], [1, 2], list(range(8)), [6, 5, 4, 3, 2, 1, 0], list(range(40)), [3, 0, 39, 38, 1]):
+        c.run_and_check([(s, at[s], 1) for s in slots], str(kw))
+        for s in slots:
+            at[s] += 1
+    if not kw.get("chunk"):
+        few = min(3, c.plan.few)
+        c.run_and_check([(0, at[0], few), (2, at[2], 1), (7, at[7], 1), (1, at[1], c.plan.few + 60)], "mixed")
+        at[0], at[2], at[7] = at[0] + few, at[2] + 1, at[7] + 1
+    # a sequence outside its cache is reported and the others are as ever
+    d = c.d
+    proj = c.rows(3)
+    got = None
+    x, out = d.torch.from_numpy(proj).to(d.dev), d.torch.full((3, (H * V + 7) // 8 * 8), 7.0, dtype=d.torch.bfloat16, device=d.dev)
+    entries = [(0, at[0], 1), (5, cap, 1), (7, at[7], 1)]
+    b = c.batch(entries)
+    d.torch.cuda.synchronize()
+    c.plan.run(b, x, c.kc, c.vc, out)
+    lm.sync()
+    assert lm.device_status() != 0
+    got = out.float().cpu().numpy()[:, :H * V]
+    want, bound = c.want([entries[0], entries[2]], proj[[0, 2]])
+    assert (np.abs(got[[0, 2]] - want) <= bound).all() and (got[1] == 7.0).all()
+    assert not d.buffer("attn4.tickets", 1, 1, d.torch.int32).any()
+
+
 def test_positions_outside_the_cache(lm):
     """Recorded as a status, nothing written; the next call is as good as ever."""
     c = Case(lm, 11, 4, 2, 64, 64, 64, 2, 64)
