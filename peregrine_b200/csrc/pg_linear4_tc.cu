@@ -581,16 +581,18 @@ int32_t dispatch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float 
         const int64_t rows = (pairs + lin->experts - 1) / lin->experts;
         bn = rows <= 12 ? 16 : rows <= 24 ? 32 : rows <= 48 ? 64 : 128;
     } else {
-        // cycles: of a block of 128 k, its products (4 BN) or the unpacking; of a pair's stretch, with what it costs to put shared tiles together
+        // cycles, from measurements: of a block of 128 k (its unpacking, products and sums), and of a pair's stretch what it costs to put shared tiles
+        // together.  (17 to 300 rows of five matrices from 4096 x 4096 to 28672 x 4096, BN 32, 64 and 128: at most 2 % from the best of the six.  Shared
+        // stretches against whole tiles: 100 rows 4096 x 14336 30.6 and 51.9 us, 200 rows 4096 x 4096 25.6 and 20.4.)
         double best = 1e30;
         const int64_t sm_pairs = ctx->sm_count / CG;
         for (int cand : {16, 32, 64, 128}) {
             const int64_t tiles = ((m + cand - 1) / cand) * ((lin->n + CG * BM - 1) / (CG * BM)), rounds = (tiles + sm_pairs - 1) / sm_pairs;
-            const double block = std::max(4.0 * cand, 500.0), whole = (double)rounds * kblocks * block;
+            const double block = cand <= 32 ? 550.0 : cand == 64 ? 600.0 : 800.0, whole = (double)rounds * kblocks * block;
             if (whole < best) best = whole, bn = cand, sh.blocks = 0;
             if (tiles > 1024) continue;
             const int64_t blocks = std::max<int64_t>(2, (tiles * kblocks + sm_pairs - 1) / sm_pairs);
-            const double time = blocks * block + 4000.0 + 16.0 * cand;
+            const double time = blocks * block + 6000.0 + 60.0 * cand;
             if (time < best) best = time, bn = cand, sh.blocks = (int)blocks;
         }
     }
