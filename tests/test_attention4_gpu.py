@@ -417,6 +417,88 @@ def test_rows_do_not_depend_on_their_company(lm):
     assert np.array_equal(c.step(entries, proj2)[2], a[2])
 
 
+@pytest.mark.parametrize("H,G,D,V", [(6, 2, 18, 10), (2, 1, 130, 7), (3, 1, 33, 250)])
+def test_odd_widths(lm, H, G, D, V):
+    """Rows that are no whole 16-byte words, widths of which the last 32 columns are partly there."""
+    c = Case(lm, D + V, H, G, D, V, 333, 3, 300)
+    c.append(1, 0, c.rows(33)), c.append(2, 0, c.rows(100))
+    c.run_and_check([(0, 0, 1), (1, 33, 1), (2, 100, 1)])
+    c.run_and_check([(0, 1, 3), (2, 101, 2)])
+    n = c.plan.few + 70
+    c.run_and_check([(2, 103, n), (1, 34, 1)])
+
+
+def test_a_recorded_longer_portion(lm):
+    """A portion of 150 tokens recorded once, replayed over other rows of the projection."""
+    c = Case(lm, 15, 8, 2, 64, 96, 700, 2, 400, sink=True)
+    t = c.d.torch
+    c.append(1, 0, c.rows(200))
+    entries = [(1, 200, 150), (0, 0, 2)]
+    b = c.batch(entries, fixed=True)
+    x, out = t.zeros(152, c.width, device=c.d.dev), t.zeros(152, c.H * c.V, dtype=t.bfloat16, device=c.d.dev)
+    t.cuda.synchronize()
+    with lm.record() as g:
+        c.plan.run(b, x, c.kc, c.vc, out)
+    for _ in range(3):
+        proj = c.rows(152)
+        x.copy_(t.from_numpy(proj).to(c.d.dev))
+        t.cuda.synchronize()
+        g.launch()
+        lm.sync()
+        want, bound = c.want(entries, proj)
+        assert (np.abs(out.float().cpu().numpy() - want) <= bound).all()
+    g.free()
+    assert lm.device_status() == 0
+
+
+def test_two_contexts_at_once(lm):
+    """Steps on two contexts' streams, each with its caches and workspaces."""
+    from peregrine_b200.runtime import GpuContext
+
+    other = GpuContext(component="lm")
+    cases = [Case(c, 16, 8, 2, 128, 64, 1200, 3, 300) for c in (lm, other)]
+    t = cases[0].d.torch
+    for c in cases:
+        c.append(0, 0, c.rows(1000)), c.append(1, 0, c.rows(31))
+    entries = [(0, 1000, 1), (1, 31, 1), (2, 0, 150)]
+    work = []
+    for c in cases:
+        proj = c.rows(152)
+        x, out = t.from_numpy(proj).to(c.d.dev), t.zeros(152, c.H * c.V, dtype=t.bfloat16, device=c.d.dev)
+        work.append((c, proj, x, out, c.batch(entries)))
+    t.cuda.synchronize()
+    for _ in range(10):
+        for c, _proj, x, out, b in work:
+            c.plan.run(b, x, c.kc, c.vc, out)
+    lm.sync(), other.sync()
+    for c, proj, x, out, b in work:
+        want, bound = c.want(entries, proj)
+        assert (np.abs(out.float().cpu().numpy() - want) <= bound).all()
+    other.close()
+
+
+def test_a_cache_of_more_than_four_gigabytes(lm):
+    """Slots whose keys and values lie behind 2^32 bytes: a prompt, few and single tokens in the last of them, beside the first."""
+    H, G, D, V, cap, slots = 16, 8, 128, 128, 60000, 140
+    c = Case(lm, 14, H, G, D, V, cap, slots, 256)
+    assert c.kc.numel() > 1 << 32
+    c.held = lambda: _first_rows(c, 400)
+    c.run_and_check([(139, 0, 150)])
+    c.run_and_check([(139, 150, 3), (0, 0, 2)])
+    c.run_and_check([(0, 2, 1), (139, 153, 1)])
+
+
+def _first_rows(c, rows):
+    """What the first rows of the first and the last slot hold; nothing of the others."""
+    out = []
+    for cache, values, width in ((c.kc, False, c.D), (c.vc, True, c.V)):
+        full = np.zeros((c.slots, c.G, rows, width))
+        for s in (0, c.slots - 1):
+            full[s] = c.plan.values(cache[s:s + 1], rows, values)[0].double().cpu().numpy()
+        out.append(full)
+    return out
+
+
 def test_recorded_steps(lm):
     """Two recordings over one plan's workspaces, replayed in turn with other positions and rows."""
     c = Case(lm, 13, 8, 2, 128, 128, 3000, 3, 64, sink=True)

@@ -405,6 +405,34 @@ def test_first_call_in_a_recording(lm):
     ctx.close()
 
 
+def test_weights_of_more_than_four_gigabytes(lm):
+    """The last rows lie behind 2^32 bytes."""
+    d = device(lm)
+    t = d.torch
+    n, k, last = (1 << 20) + 40, 8192, 72
+    gen = t.Generator(device=d.dev).manual_seed(3)
+    q = t.randint(0, 256, (n, k // 2), dtype=t.uint8, device=d.dev, generator=gen)
+    s = t.full((n, k // 128), 0.01, dtype=t.bfloat16, device=d.dev)
+    s[-last:] = (t.randn(last, k // 128, device=d.dev, generator=gen) * 0.02).bfloat16()
+    from peregrine_b200.layers import Linear4
+
+    lin = Linear4.from_quants(d, q, s)
+    assert lin.bytes() > 1 << 32
+    tail = q[-last:].cpu().numpy()
+    w = np.stack([tail & 15, tail >> 4], -1).reshape(last, k).astype(np.float64) - 8
+    w *= np.repeat(s[-last:].double().cpu().numpy(), 128, 1)
+    del q
+    for m in (1, 12, 40):
+        x = bf16(d, rng(m).standard_normal((m, k)))
+        y = t.zeros(m, n, device=d.dev)
+        t.cuda.synchronize()
+        lin.run(x, m, y)
+        lm.sync()
+        want, bound = sums(x.double().cpu().numpy(), w)
+        within(y[:, -last:].cpu().numpy(), want, bound)
+    lin.free()
+
+
 def test_two_contexts_at_once(lm):
     """The same weights read from two streams."""
     from peregrine_b200.runtime import GpuContext
