@@ -349,6 +349,42 @@ def test_experts(lm, m, E, I, top, width, ff, group):
     a.free(), b.free()
 
 
+def test_a_route_of_very_many_tiles(lm):
+    """More tiles to a pair of blocks than are looked up beforehand.  All tokens are the same, so an expert's rows are all the same, bit for bit."""
+    E, N, K, m = 2, 28800, 64, 16384
+    d = device(lm, m)
+    t, lib, h = d.torch, d.lib, lm.handle
+    g = rng(77)
+    q, s, w = quants(g, E, N, K, group=64)
+    lin = handle(d, q, s)
+    x = bf16(d, g.standard_normal((1, K))).expand(m, K).contiguous()
+    logits = t.zeros(m, E, device=d.dev)
+    logits[:, 0] = t.arange(m, device=d.dev) % 3 - 0.5        # one token in three goes to the second expert
+    route = C.c_void_p()
+    d.check(lib.pg_route_create(h, m, E, 0, 1, C.byref(route)))
+    rows = lib.pg_route_max_rows(route)
+    out = t.full((rows, N), 3.0, dtype=t.bfloat16, device=d.dev)
+    corr = t.zeros(E, device=d.dev)
+    t.cuda.synchronize()
+    d.check(lib.pg_route_run(h, route, d.code, logits.data_ptr(), E, m, corr.data_ptr(), 1, 1))
+    lin.run_routed(route, x, True, out)
+    lm.sync()
+    assert lm.device_status() == 0
+    second = int((t.arange(m) % 3 == 0).sum())
+    xs = x[:1].double().cpu().numpy()
+    for e, n in ((0, m - second), (1, second)):
+        want, bound = sums(xs, w[e])
+        bound = bound + 2.0 ** -8 * (np.abs(want) + bound)
+        near = (out[:, :64].double().cpu().numpy() - want[:, :64]) / bound[:, :64]
+        mine = np.nonzero((np.abs(near) <= 1).all(1))[0]
+        assert len(mine) >= n                                 # (rows without a token may hold anything)
+        one = out[int(mine[0])]
+        within(one.float().cpu().numpy()[None], want, bound)
+        assert int((out[t.from_numpy(mine).to(d.dev)] == one).all(1).sum()) >= n
+    d.check(lib.pg_route_free(h, route))
+    lin.free()
+
+
 # ---- graphs, contexts, refusals --------------------------------------------------------------------------------------
 def test_two_recordings_share_the_workspace(lm):
     """Products whose K goes over several CTAs, recorded twice, replayed in turn with other inputs, beside calls that are not recorded."""
