@@ -84,10 +84,11 @@ PG_API int32_t pg_route_create(pg_ctx *ctx, int64_t max_tokens, int64_t experts,
 PG_API int32_t pg_route_free(pg_ctx *ctx, pg_route *route);
 PG_API int64_t pg_route_max_rows(const pg_route *route); /* rows a routed output can have */
 /* logits [m, ld] of experts + identity columns; correction [experts + identity] is added to the scores for the choice
- * only; only the best `keep` of `groups` groups of neighbours can be chosen (groups <= 1: no limit). */
+ * only; only the best `keep` of `groups` groups of neighbours can be chosen (groups <= 1: no limit).  Scores that are not numbers are
+ * not chosen, so a token with one logit that is not a number, or is +infinity, chooses nothing: its pairs have weight 0 and no row. */
 PG_API int32_t pg_route_run(pg_ctx *ctx, pg_route *route, int32_t dtype, const float *d_logits, int64_t ld, int64_t m, const float *d_correction,
                             int32_t groups, int32_t keep);
-/* copies of the chosen ids [m, top] and weights [m, top] (device -> host, blocking) */
+/* copies of the chosen ids [m, top] and weights [m, top] (device -> host, blocking); a choice of nothing has the last output's id and weight 0 */
 PG_API int32_t pg_route_read(pg_ctx *ctx, const pg_route *route, int32_t *ids, float *weights);
 
 /* ---- rows of the residual stream ---- */

@@ -389,7 +389,7 @@ int32_t pgk_linear4_gemv(pg_ctx *ctx, const pg_linear4 *lin, const bf16 *a, int6
                          const PgRouted *routed, int64_t max_blocks)
 {
     const int64_t items = lin->tiles * (routed ? max_blocks : 1);
-    const int nt = m > 8 ? 2 : 1;   // (an expert has a row of a token at most)
+    const int nt = m > 8 ? 2 : 1;   // (the rows of an expert belong to different tokens, see pg_route.cu)
     const Parts p = parts_of(lin, items, ctx->sm_count, nt);
     PG_REQUIRE(p.KW <= v4_kw_max(nt) && p.sp <= 16, "linear4: K too long");
     if (p.sp > 1) {

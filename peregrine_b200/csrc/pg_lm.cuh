@@ -26,9 +26,9 @@ struct pg_route {
     int64_t max_tokens = 0, experts = 0, identity = 0, top = 0, max_rows = 0, m = 0;
     int block = PG_ROUTE_BLOCK;
     void *mem = nullptr;
-    int32_t *ids = nullptr;        // [m * top] expert of each pair (>= experts: identity)
+    int32_t *ids = nullptr;        // [m * top] expert of each pair (>= experts: identity; -1: no choice)
     float *weights = nullptr;      // [m * top]
-    int32_t *pair_row = nullptr;   // [m * top] row of the pair, -1 for identity
+    int32_t *pair_row = nullptr;   // [m * top] row of the pair, -1 for identity and for pairs without a choice
     int32_t *row_pair = nullptr;   // [max_rows] pair of the row, -1 for padding
     int32_t *count = nullptr;      // [experts] (zero between steps in the many-token form)
     int32_t *cursor = nullptr;     // [experts]

@@ -5,6 +5,9 @@
 //   more                 a warp per token counts per expert; one CTA lays out 128-row blocks; pairs take their rows.
 //                        (Which row of its expert a pair gets is left to the order of arrival: rows do not meet in any
 //                        sum, and a token adds its own pairs up in the order of its choices.)
+//
+// A choice that finds no score left that is a number chooses nothing: its pair has weight 0, the id -1 on the device (pg_route_read says the last
+// output) and no row.  So the rows of an expert belong to different tokens, which the 16-row blocks and the products on them rely on.
 #include <math.h>
 
 #include <new>
@@ -90,8 +93,8 @@ __device__ __forceinline__ void choose(const float *z, const float *__restrict__
         for (int i = 0; i < NV; i++)
             if (key[i] > best) best = key[i], idx = lane + 32 * i, w = e[i];
         warp_best(best, idx);
-        if (idx >= ch.n) {                                // not-a-number scores choose nothing: weight 0
-            if (lane == 0) ids[k] = ch.n - 1, weights[k] = 0.0f;
+        if (idx >= ch.n) {                                // not-a-number scores choose nothing
+            if (lane == 0) ids[k] = -1, weights[k] = 0.0f;
             continue;
         }
         if ((idx & 31) == lane) {
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(512)
     for (int p = threadIdx.x; p < pairs; p += 512) {
         const int id = sid[p];
         ids[p] = id;
-        rank[p] = id < experts ? atomicAdd(count + id, 1) : -1;
+        rank[p] = id >= 0 && id < experts ? atomicAdd(count + id, 1) : -1;
     }
     __syncthreads();
     // a block of 16 rows per expert in use, in the order of the experts
@@ -149,7 +152,7 @@ __global__ void __launch_bounds__(512)
     if (threadIdx.x == 0) *blocks = base;
     for (int p = threadIdx.x; p < pairs; p += 512) {
         const int r = rank[p];
-        const int row = r >= 0 && r < PG_ROUTE_SMALL ? count[sid[p]] * PG_ROUTE_SMALL + r : -1;
+        const int row = r >= 0 ? count[sid[p]] * PG_ROUTE_SMALL + r : -1;
         pair_row[p] = row;
         if (row >= 0) row_pair[row] = p;
     }
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(128)
     choose<NV>(logits + (int64_t)t * ld, correction, ch, sm + warp * ch.groups, ids + (int64_t)t * ch.top, weights + (int64_t)t * ch.top, lane);
     for (int k = lane; k < ch.top; k += 32) {
         const int id = __ldcg(ids + (int64_t)t * ch.top + k);
-        if (id < experts) atomicAdd(count + id, 1);
+        if (id >= 0 && id < experts) atomicAdd(count + id, 1);
     }
 }
 
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(256) route_place_kernel(int pairs, int experts
     if (p >= pairs) return;
     const int e = __ldcg(ids + p);
     int row = -1;
-    if (e < experts) {
+    if (e >= 0 && e < experts) {
         row = atomicAdd(cursor + e, 1);
         row_pair[row] = p;
     }
@@ -356,6 +359,8 @@ PG_API int32_t pg_route_read(pg_ctx *ctx, const pg_route *route, int32_t *ids, f
         PG_CUDA(cudaMemcpyAsync(weights, route->weights, bytes, cudaMemcpyDeviceToHost, ctx->stream));
     }
     PG_CUDA(cudaStreamSynchronize(ctx->stream));
+    for (int64_t p = 0; p < route->m * route->top; p++)
+        if (ids[p] < 0) ids[p] = (int32_t)(route->experts + route->identity) - 1;
     return PG_OK;
 }
 
