@@ -55,8 +55,8 @@ __device__ __forceinline__ void four_quants(const float (&w)[4], float scale, ui
     for (int e = 0; e < 4; e++) q[e] = four_quant(w[e], scale);
 }
 
-// ---- quants -> f16 pairs: bits 0-3 / 4-7 of both halves of a word, as q - 8 and 16 (q - 8), exact.  1024 + q and 1024 + 16 q are f16 numbers
-// whose low bits are the quant's: one logical operation, then the offset comes off.
+// ---- quants -> f16 pairs: bits 0-3 / 4-7 of both halves of a word, as q - 8, exact.  1024 + q and 64 + q are f16 numbers that have the quant in
+// their bits 0-3 and 4-7: one logical operation, then the offset comes off.  1024 + 16 q gives 16 (q - 8) with one constant less.
 __device__ __forceinline__ uint32_t four_lop(uint32_t w, uint32_t mask, uint32_t base)
 {
     uint32_t r;
@@ -69,10 +69,10 @@ __device__ __forceinline__ uint32_t four_sub_f16(uint32_t a, uint32_t b)
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-constexpr uint32_t FOUR_LO = 0x000f000fu, FOUR_HI = 0x00f000f0u, FOUR_F16 = 0x64006400u;
-constexpr uint32_t FOUR_OFF_LO = 0x64086408u, FOUR_OFF_HI = 0x64806480u;   // 1032 and 1152
-__device__ __forceinline__ uint32_t four_f16_lo(uint32_t w) { return four_sub_f16(four_lop(w, FOUR_LO, FOUR_F16), FOUR_OFF_LO); }
-__device__ __forceinline__ uint32_t four_f16_hi(uint32_t w) { return four_sub_f16(four_lop(w, FOUR_HI, FOUR_F16), FOUR_OFF_HI); }   // times 16
+constexpr uint32_t FOUR_LO = 0x000f000fu, FOUR_HI = 0x00f000f0u;
+__device__ __forceinline__ uint32_t four_f16_lo(uint32_t w) { return four_sub_f16(four_lop(w, FOUR_LO, 0x64006400u), 0x64086408u); }   // 1024, 1032
+__device__ __forceinline__ uint32_t four_f16_hi(uint32_t w) { return four_sub_f16(four_lop(w, FOUR_HI, 0x54005400u), 0x54805480u); }   // 64, 72
+__device__ __forceinline__ uint32_t four_f16_hi16(uint32_t w) { return four_sub_f16(four_lop(w, FOUR_HI, 0x64006400u), 0x64806480u); }   // 1024, 1152
 // the same as bf16, from bits 0-3: 128 + q, less 136
 __device__ __forceinline__ uint32_t four_bf16_lo(uint32_t w)
 {
@@ -102,8 +102,9 @@ __device__ __forceinline__ uint32_t four_pack_f16(float lo, float hi)
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-// Powers of two that bring numbers of magnitude up to `top` below 2^15 and back: f16 then holds every bf16 number down to 2^-29 of the
-// largest exactly, and smaller ones to 2^-39 of it.  (An infinity stays one, and finite numbers beside it stay finite.)
+// Powers of two that bring numbers of magnitude up to `top` below 2^15 and back: f16 then holds every bf16 number down to 2^-31 of the
+// largest exactly (eight bits, the last of them 2^-24 or more), and smaller ones to 2^-39 of it.  (An infinity stays one, and finite numbers beside it
+// stay finite.)
 __device__ __forceinline__ void four_range(float top, float &down, float &back)
 {
     const int e = max((int)(__float_as_uint(top) >> 23 & 255u), 20);

@@ -9,9 +9,9 @@
 // quants are f16 numbers that is an A operand of mma.sync m16n8k16, and a row's words are its columns in their order.  Scales: rows r and r + 8 side
 // by side; where a group is 128 long its two records both have them, so that a record is all that a block of 64 k needs.
 //
-// Scales are kept as f16 divided by a power of two per row, which brings the row's largest to [2^11, 2^12): scale * (q - 8) is then at most 8 + 3
-// significant bits, so an f16 number, exactly, as long as the row's scales are within 2^21 of each other (below, the smaller ones lose bits
-// that are under 2^-36 of the largest).
+// Scales are kept as f16 divided by a power of two per row, which brings the row's largest to [2^11, 2^12): a scale's 8 bits are then an f16 number,
+// exactly, as long as the row's scales are within 2^28 of each other (below, the smaller ones lose bits that are under 2^-36 of the largest), and so is
+// scale * (q - 8), a multiple of it with 11 bits at most.  All forms of the product take these weights, which are what pg_linear4_read says.
 #include <algorithm>
 #include <new>
 

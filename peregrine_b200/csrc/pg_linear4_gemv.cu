@@ -3,7 +3,7 @@
 //   * The weights are the M side of mma.sync m16n8k16 (16 rows x 16 k), activation rows its 8 columns; up to 16 rows of a take two column
 //     tiles on the same unpacked quants.  Quants become f16 integers (exact), sums of a group are scaled in f32.
 //   * The activations are bf16 and enter as f16: a warp divides each row of its part of K by a power of two of its own (four_range) and
-//     multiplies the sums back, so nothing is rounded that could be seen in an f32 sum.
+//     multiplies the sums back: exact down to 2^-27 of the part's largest, and smaller ones are off by 2^-36 of that at most.
 //   * One persistent CTA of 16 warps per SM.  `kw` warps share a tile of 16 weight rows, each with one part of K of at most 512 elements (256 with more than
 //     eight rows), whose activations it keeps in registers; a fill of its ring is one bulk copy, quants and scales.  The parts meet in shared memory
 //     in a fixed order; the warps of a tile take turns in adding.
@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
     if (!ROUTED) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     // activations of the warp's part of K: word 4 c + i of column r (and r + 8): the pairs of columns 32 c + 8 t + 2 i, every second one over 16 (the
-    // quants beside it come 16 times too large)
+    // quants beside it come 16 times too large: as q - 8 they take a constant more, which the registers do not have, 36.9 -> 38.6 us with 16 rows of
+    // 28672 x 4096; so every bf16 number down to 2^-27 of the part's largest is exact)
     uint32_t x[NT][KWM / 8];
     float back[NT][2];                                    // what the sums of columns 2 t and 2 t + 1 are multiplied by
     auto bring = [&](int blk) {
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(V4_THREADS, 1)
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
                                 const uint32_t w0 = u ? q[h] >> 8 : q[h], w1 = u ? q[2 + h] >> 8 : q[2 + h];
-                                const uint32_t a0 = four_f16_lo(w0), a1 = four_f16_lo(w1), a2 = four_f16_hi(w0), a3 = four_f16_hi(w1);
+                                const uint32_t a0 = four_f16_lo(w0), a1 = four_f16_lo(w1), a2 = four_f16_hi16(w0), a3 = four_f16_hi16(w1);
                                 const int i = 8 * b + 4 * h + 2 * u;
                                 if ((2 * b + h) % G32 == 0 && u == 0) {
                                     four_mma_f16_first(sum[0], a0, a1, a2, a3, x[0][i], x[0][i + 1]);

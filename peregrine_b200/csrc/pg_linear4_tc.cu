@@ -3,7 +3,7 @@
 //   * The weights are the M side: a pair of CTAs has 256 rows, each unpacks its 128 to f16 in TMEM, 128 k at a time (a thread per row, two or three
 //     teams of four warps that take the blocks in turn, two blocks of TMEM each); the activations are the N side, BN rows of f16 in shared memory by TMA, half in each CTA.
 //     scale * (q - 8) is an f16 number exactly (csrc/pg_linear4.cu), and linear4_rows_kernel writes the activations as f16 divided by a power of two
-//     per row, which holds bf16 numbers exactly down to 2^-29 of the row's largest: sums are those of the bf16 activations with the weights.
+//     per row, which holds bf16 numbers exactly down to 2^-31 of the row's largest: sums are those of the bf16 activations with the weights.
 //   * An accumulator sums up 512 k; eight warps add the accumulators up in f32 registers.  (The tensor cores cut sums off: 4096 k in one
 //     accumulator were 3.9e-6 off 64 bits, 512 at a time 6e-7.)  They write the outputs: lane = weight row, so a store is 32 columns of one row of y.
 //   * Where whole tiles would leave SMs idle, the tiles' blocks of 128 k are divided evenly over the pairs of CTAs; sums of a tile that several share
@@ -452,15 +452,15 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
                 for (int e = 0; e < 2; e++) {
                     unsigned short h;
                     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + s_off + e * s_step));
-                    const uint32_t sc = (uint32_t)h * 0x10001u, less = mul_f16x2(sc, 0x2c002c00u);   // times 1 / 16
+                    const uint32_t sc = (uint32_t)h * 0x10001u;
                     uint32_t v[16];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint32_t word = e ? q[i].y : q[i].x, word8 = word >> 8;
                         v[4 * i] = mul_f16x2(four_f16_lo(word), sc);
-                        v[4 * i + 1] = mul_f16x2(four_f16_hi(word), less);
+                        v[4 * i + 1] = mul_f16x2(four_f16_hi(word), sc);
                         v[4 * i + 2] = mul_f16x2(four_f16_lo(word8), sc);
-                        v[4 * i + 3] = mul_f16x2(four_f16_hi(word8), less);
+                        v[4 * i + 3] = mul_f16x2(four_f16_hi(word8), sc);
                     }
                     if (e == 0 && c == 0) {
                         if (!(ok = pg_mbar_wait_warp(free_at + turn * (8 * TEAMS), phase, abort_flag, status, limit_ns))) break;
