@@ -44,6 +44,7 @@ struct Cfg {
     static constexpr int R_UNPACK = 80, R_OUT = 128, R_REST = 64;
     static constexpr bool SHARES = COLS >= 64;
     static_assert(!SHARES || 4 * TEAMS * R_UNPACK + 8 * R_OUT + 4 * R_REST == (OUT + 8) * 96, "no more registers than there are");
+    static_assert(BN % 32 == 0 && BN >= 32 && BN <= 256, "a pair's products with the weights in TMEM take rows in steps of 32");
     static_assert(A_COL + 64 * SLOTS <= 512 && SMEM <= 227 * 1024, "TMEM, shared memory");
 };
 
@@ -540,7 +541,7 @@ __global__ void __launch_bounds__(Cfg<BN>::THREADS, 1)
 #pragma unroll
                             for (int j = 0; j < 16; j++) a[j] = 0.0f;
                             // (as many pairs' sums on their way at once as registers allow)
-                            constexpr int AHEAD = COLS == 64 ? 3 : COLS == 32 ? 2 : 4;
+                            constexpr int AHEAD = COLS == 64 ? 3 : 2;
                             for (int pair = lo; pair <= hi; pair += AHEAD) {
                                 float b[AHEAD][16];
 #pragma unroll
@@ -606,16 +607,16 @@ int32_t dispatch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float 
     if (rt.blocks) {
         // rows an expert has on average
         const int64_t rows = (pairs + lin->experts - 1) / lin->experts;
-        bn = rows <= 12 ? 16 : rows <= 24 ? 32 : rows <= 48 ? 64 : 128;
+        bn = rows <= 24 ? 32 : rows <= 48 ? 64 : 128;
     } else {
         // cycles, from measurements: of a block of 128 k (its unpacking, products and sums), and of a pair's stretch what it costs to put shared tiles
         // together.  (17 to 300 rows of five matrices from 4096 x 4096 to 28672 x 4096, BN 32, 64 and 128: at most 2 % from the best of the six.  Shared
         // stretches against whole tiles: 100 rows 4096 x 14336 30.6 and 51.9 us, 200 rows 4096 x 4096 25.6 and 20.4.)
         double best = 1e30;
         const int64_t sm_pairs = ctx->sm_count / CG;
-        for (int cand : {16, 32, 64, 128}) {
+        for (int cand : {32, 64, 128}) {
             const int64_t tiles = ((m + cand - 1) / cand) * ((lin->n + CG * BM - 1) / (CG * BM)), rounds = (tiles + sm_pairs - 1) / sm_pairs;
-            const double block = cand <= 32 ? 550.0 : cand == 64 ? 600.0 : 800.0, whole = (double)rounds * kblocks * block;
+            const double block = cand == 32 ? 550.0 : cand == 64 ? 600.0 : 800.0, whole = (double)rounds * kblocks * block;
             if (whole < best) best = whole, bn = cand, sh.blocks = 0;
             if (tiles > 1024) continue;
             const int64_t blocks = std::max<int64_t>(2, (tiles * kblocks + sm_pairs - 1) / sm_pairs);
@@ -629,8 +630,7 @@ int32_t dispatch(pg_ctx *ctx, const pg_linear4 *lin, const void *x, const float 
     }
     if (bn == 128) return launch<128, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
     if (bn == 64) return launch<64, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
-    if (bn == 32) return launch<32, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
-    return launch<16, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
+    return launch<32, ACT, TY>(ctx, lin, x, xback, m, limit, y, ldy, rt, sh);
 }
 
 }  // namespace
