@@ -432,7 +432,8 @@ __global__ void __launch_bounds__(WARPS * 32)
             b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, x));
             b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, x));
         }
-        const float n0 = fmaxf(m0, b0), n1 = fmaxf(m1, b1);
+        constexpr float P_UP = HALF ? ATTN_P_UP : 0.0f;
+        const float n0 = fmaxf(m0, b0 - P_UP), n1 = fmaxf(m1, b1 - P_UP);
         const float f0 = exp2f(m0 - n0), f1 = exp2f(m1 - n1);
         m0 = n0;
         m1 = n1;

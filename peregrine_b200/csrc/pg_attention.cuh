@@ -21,6 +21,9 @@ struct AttnShape {
     const int *v_bad;
 };
 constexpr int ATTN_TOPS = 32;
+// Probabilities in f16 are 2^7 times those of the row's maximum (2^15 at most where that may fall behind by 2^8): those down to 2^-32 of the largest then
+// count in the sums as they do in the denominator.  (From 1 on they ended at 2^-25: behind 131072 positions, 2^-8 of an output.)
+constexpr float ATTN_P_UP = 7.0f;
 
 #ifdef __CUDACC__
 // A chunked layer keeps whole chunks only, position p in row p mod cap: the rows of a chunk lie next to each other.

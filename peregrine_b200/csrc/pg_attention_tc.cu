@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
         const float sx = BIAS ? 1.0f : sl;              // (with a bias the scores are scaled before the maximum)
         const float bias = BIAS && s.slopes ? __ldg(s.slopes + g * s.rep + rc % s.rep) * LOG2E : 0.0f;
+        constexpr float P_UP = HALF ? ATTN_P_UP : 0.0f;
         float m = 0.0f, l0 = 0.0f, l1 = 0.0f;
         bool ok = true;
         for (int j = 0; j < tiles[t]; j++) {
@@ -260,13 +261,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sx;
             if (j == 0) {
                 // finite also where the row sees nothing of the first tile; f16 holds probabilities of the row's own maximum only
-                m = fmaxf(top, s.sink && !HALF ? 0.0f : -1e30f);
+                m = fmaxf(top - P_UP, s.sink && !HALF ? 0.0f : -1e30f);
             } else {
-                const bool behind = top > m + 8.0f;
+                const bool behind = top > m + (P_UP + 8.0f);
                 if (__any_sync(0xffffffffu, behind)) {
                     // (these scores were committed behind the previous keys' sums: O is at rest)
-                    const float f = behind ? pg_ex2(m - top) : 1.0f;
-                    if (behind) m = top;
+                    const float next = top - P_UP, f = behind ? pg_ex2(m - next) : 1.0f;
+                    if (behind) m = next;
                     l0 *= f;
                     l1 *= f;
 #pragma unroll 1
