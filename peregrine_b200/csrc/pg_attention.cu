@@ -901,7 +901,7 @@ PG_API int32_t pg_attention_run(pg_ctx *ctx, const pg_attention *p, const pg_bat
 #define PG_AT(DC, VC)                                                                                                        \
     do {                                                                                                                     \
         if (fused) return run_step<DC, VC, true>(ctx, s, batch, d_proj, ldp, q, kc, vc, p->d_part, p->d_tickets, out, ldo);  \
-        if (step) return run_step<DC, VC, false>(ctx, s, batch, d_proj, ldp, q, kc, vc, p->d_part, p->d_tickets, out, ldo);  \
+        return run_step<DC, VC, false>(ctx, s, batch, d_proj, ldp, q, kc, vc, p->d_part, p->d_tickets, out, ldo);            \
     } while (0)
     if (s.dp <= 64 && s.vp <= 64) PG_AT(4, 8);
     if (s.dp <= 128 && s.vp <= 128) PG_AT(8, 16);
