@@ -164,8 +164,8 @@ PG_API int32_t pg_attention_run(pg_ctx *ctx, const pg_attention *p, const pg_bat
  * columns, 256 bytes each, then for every pair of positions the bf16 scales of every 32 columns, both positions side by side.
  *   keys    position 8 n + r, column 16 s + 4 t + 2 i + h of 32: byte [r][t][s][2 h + n], low half for i = 0
  *   values  position 8 i + 2 t + h, column 16 s + 8 n + r of 32: byte [r][t][s][2 h + i], low half for n = 0
- * pg_attention: d_q, [max_rows][H][dp + 2] halves on a 16-byte boundary, is used where pg_attention4_prompt follows only; d_part: pg_attention4_part_floats(...); d_tickets: [pg_attention4_tickets(...)], zero before the
- * first call. */
+ * pg_attention: d_q, [max_rows][H][dp + 2] halves on a 16-byte boundary, is used where pg_attention4_prompt follows only; d_part:
+ * pg_attention4_part_floats(...) on a 16-byte boundary; d_tickets: [pg_attention4_tickets(...)], zero before the first call. */
 PG_API int64_t pg_cache4_bytes(int32_t width, int64_t positions);
 PG_API int64_t pg_attention4_part_floats(pg_ctx *ctx, const pg_attention *p);
 PG_API int64_t pg_attention4_tickets(pg_ctx *ctx);

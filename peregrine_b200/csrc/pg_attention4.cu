@@ -904,6 +904,7 @@ int32_t check(const pg_attention *p, const pg_batch *batch, const void *kc, cons
     PG_REQUIRE(p->chunk == 0 || p->positions <= p->cap || ((int64_t)(p->chunk + batch->max_len - 2) / p->chunk + 1) * p->chunk <= p->cap,
                "attention4: a step of %d tokens has more chunks of %d than the cache of %d rows", batch->max_len, p->chunk, p->cap);
     PG_REQUIRE(((uintptr_t)kc & 15) == 0 && ((uintptr_t)vc & 15) == 0, "attention4: caches start on 16-byte boundaries");
+    PG_REQUIRE(((uintptr_t)p->d_part & 15) == 0 && ((uintptr_t)out & 1) == 0, "attention4: workspace on no 16-byte boundary, or output not aligned");
     PG_REQUIRE(ldo >= (int64_t)p->heads * p->vdim, "attention4: rows too short");
     PG_REQUIRE(p->kv_heads <= 65535 && batch->rows >= 0 && batch->seqs >= 0 && batch->seqs <= 65535, "attention4: too many heads or sequences");
     return PG_OK;
@@ -942,6 +943,7 @@ PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_ba
     const AttnShape s = pgk_attention_shape(p);
     const Four f = four_of(s);
     PG_REQUIRE(d_proj && ldp >= (int64_t)(s.H + s.G) * s.D + (int64_t)s.G * s.V, "attention4: rows too short");
+    PG_REQUIRE(((uintptr_t)d_proj & 3) == 0 && (((uintptr_t)p->d_q & 15) == 0 || short_rows == batch->rows), "attention4: rows or queries not aligned");
     PG_REQUIRE(few >= 0 && few <= 4096 && short_rows >= 0 && short_rows <= batch->rows && short_len >= 0 && short_len <= few && (short_len == 0) == (short_rows == 0),
                "attention4: %lld rows of up to %lld tokens among sequences of up to %lld", (long long)short_rows, (long long)short_len, (long long)few);
     PG_REQUIRE(s.chunk == 0 || few <= 1, "attention4: a chunked layer takes one token of a sequence here");
@@ -1023,7 +1025,7 @@ PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg
 PG_API int32_t pg_cache4_read(pg_ctx *ctx, const void *d_cache, int32_t values, int32_t width, int64_t cap, int64_t parts, int64_t rows, float *d_out)
 {
     PG_ENTER(ctx);
-    PG_REQUIRE(d_cache && d_out && ((uintptr_t)d_cache & 15) == 0, "cache4_read: null pointer, or not on a 16-byte boundary");
+    PG_REQUIRE(d_cache && d_out && ((uintptr_t)d_cache & 15) == 0 && ((uintptr_t)d_out & 3) == 0, "cache4_read: null pointer, or not on a 16-byte boundary");
     PG_REQUIRE(width > 0 && width <= 256 && cap > 0 && parts > 0 && parts <= 65535 && rows > 0 && rows <= cap, "cache4_read: bad shape");
     const int w = (int)pg_up(width, 32), tile = (int)pg_cache4_tile_bytes(w);
     const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)parts);

@@ -118,6 +118,7 @@ int32_t create(pg_ctx *ctx, const void *src, const void *scales, int64_t n, int6
     PG_REQUIRE(out != nullptr, "linear4: out is null");
     *out = nullptr;
     PG_REQUIRE(src && n > 0 && k > 0 && experts > 0, "linear4: bad arguments");
+    PG_REQUIRE(((uintptr_t)(scales ? scales : src) & 1) == 0, "linear4: bf16 numbers not aligned");
     PG_REQUIRE(group == 32 || group == 64 || group == 128, "linear4: groups of %lld (32, 64 or 128 are there)", (long long)group);
     PG_REQUIRE(k % 64 == 0 && k % group == 0, "linear4: K must be a multiple of 64 and of the group (K = %lld, groups of %lld)", (long long)k, (long long)group);
     PG_REQUIRE(n <= (1 << 24) && k <= (1 << 16) && experts <= 65535 && experts * n < (1ll << 31) - 4096, "linear4: shape too large");
@@ -211,7 +212,7 @@ PG_API int64_t pg_linear4_bytes(const pg_linear4 *lin) { return lin ? lin->bytes
 PG_API int32_t pg_linear4_read(pg_ctx *ctx, const pg_linear4 *lin, float *d_w)
 {
     PG_ENTER(ctx);
-    PG_REQUIRE(lin && d_w && lin->device == ctx->device, "linear4_read: bad arguments");
+    PG_REQUIRE(lin && d_w && ((uintptr_t)d_w & 3) == 0 && lin->device == ctx->device, "linear4_read: bad arguments");
     const int64_t total = lin->experts * lin->n * lin->k;
     PG_REQUIRE(total < (1ll << 31) * 256, "linear4_read: too many weights for one call");
     return launch_whole(ctx, linear4_read_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, lin->w, lin->row, (int)lin->n, (int)lin->k, (int)lin->record,
