@@ -200,6 +200,7 @@ class Linear4:
         """The weights as the product takes them: f32 [experts, N, K]."""
         t = self.d.torch
         out = t.empty(self.experts, self.n, self.k, dtype=t.float32, device=self.d.dev)
+        t.cuda.current_stream(self.d.dev).synchronize()     # (the memory may be that of a tensor which torch's stream still works on)
         self.d.check(self.d.lib.pg_linear4_read(self.d.gpu.handle, self.handle, out.data_ptr()))
         self.d.gpu.sync()
         return out
@@ -327,6 +328,7 @@ class Attention4Plan:
         width = self.c.vdim if of_values else self.c.dim
         parts = cache.shape[0] * self.c.kv_heads
         out = t.empty(parts, rows, up(width, 32), dtype=t.float32, device=d.dev)
+        t.cuda.current_stream(d.dev).synchronize()           # (as in Linear4.values)
         d.check(d.lib.pg_cache4_read(d.gpu.handle, cache.data_ptr(), int(of_values), width, self.cap, parts, rows, out.data_ptr()))
         d.gpu.sync()
         return out.view(cache.shape[0], self.c.kv_heads, rows, -1)[..., :width]
