@@ -174,7 +174,8 @@ PG_API int64_t pg_attention4_tickets(pg_ctx *ctx);
 PG_API int32_t pg_attention4_run(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t few, int64_t short_rows, int64_t short_len, const float *d_proj,
                                  int64_t ldp, void *d_kcache, void *d_vcache, void *d_out, int32_t dtype, int64_t ldo);
 /* Sequence `seq` of the batch: len tokens in this step, positions with them, in slot `slot`.  Its cache is unfolded in d_work
- * (pg_attention4_unfold_bytes(...) on a 128-byte boundary) as f16 over a power of two of each head. */
+ * (pg_attention4_unfold_bytes(...) on a 128-byte boundary) as f16 over a power of two of each head.  A recorded call is for these numbers: replayed
+ * over a batch with others, its outputs mean nothing and the context's status says so. */
 PG_API int64_t pg_attention4_unfold_bytes(const pg_attention *p);
 PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg_batch *batch, int64_t seq, int64_t len, int64_t positions, int64_t slot,
                                     const void *d_kcache, const void *d_vcache, void *d_work, void *d_out, int32_t dtype, int64_t ldo);

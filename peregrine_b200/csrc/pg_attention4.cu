@@ -251,12 +251,19 @@ __global__ void __launch_bounds__(128) attn4_read_kernel(const unsigned char *__
 }
 
 // grid (ATTN_TOPS, G, keys and values): no value of a head's rows [0, rows) is larger than the largest of its tops.  (Scales that are not numbers
-// do not count: what lies beside them keeps its digits.)  Marks no row's values as bad.
+// do not count: what lies beside them keeps its digits.)  Marks no row's values as bad.  A batch that is not the one the host was told of (a recorded
+// call's may have changed) is reported.
 __global__ void __launch_bounds__(128) attn4_tops_kernel(const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc, const Four f, int rows, int bad,
-                                                         float *__restrict__ k_top, float *__restrict__ v_top, int *__restrict__ v_bad)
+                                                         float *__restrict__ k_top, float *__restrict__ v_top, int *__restrict__ v_bad, const pg_batch bt, int seq, int len,
+                                                         int positions, int slot, int32_t *status)
 {
     __shared__ float tops[4];
     pg_pdl_begin();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
+        const int row0 = __ldcg(bt.d_seq_row0 + seq);
+        if (__ldcg(bt.d_seq_row0 + seq + 1) - row0 != len || __ldcg(bt.d_pos + row0) + len != positions || __ldcg(bt.d_seq_slot + seq) != slot)
+            atomicExch(status, (int32_t)PG_ERR_INVALID);
+    }
     const bool values = blockIdx.z == 1;
     const int groups = values ? f.gv : f.gk, bytes = values ? f.vb : f.kb, part = blockIdx.x, words = groups * 8, tiles = (rows + 15) / 16;
     const unsigned char *head = values ? vc + blockIdx.y * f.vh : kc + blockIdx.y * f.kh;
@@ -1006,7 +1013,8 @@ PG_API int32_t pg_attention4_prompt(pg_ctx *ctx, const pg_attention *p, const pg
     const int bad = f.gv * (s.chunk ? s.cap / s.chunk : 1);
     s.q_up = (const float *)((const __half *)p->d_q + (int64_t)batch->rows * s.H * s.dp), s.k_top = k_top, s.v_top = v_top, s.v_bad = v_bad;
     const unsigned char *kc = (const unsigned char *)d_kcache + slot * s.G * f.kh, *vc = (const unsigned char *)d_vcache + slot * s.G * f.vh;
-    int32_t ru = launch_pdl(ctx, attn4_tops_kernel, dim3(ATTN_TOPS, (unsigned)s.G, 2), dim3(128), 0, kc, vc, f, rows, bad, k_top, v_top, v_bad);
+    int32_t ru = launch_pdl(ctx, attn4_tops_kernel, dim3(ATTN_TOPS, (unsigned)s.G, 2), dim3(128), 0, kc, vc, f, rows, bad, k_top, v_top, v_bad, *batch, (int)seq,
+                            (int)len, (int)positions, (int)slot, ctx->d_status);
     if (ru == PG_OK)
         ru = launch_pdl(ctx, attn4_unfold_kernel, dim3((unsigned)((padded + 15) / 16), (unsigned)s.G, 2), dim3(128), 0, s, f, kc, vc, rows, padded, k, v, v_bad);
     if (ru != PG_OK) return ru;

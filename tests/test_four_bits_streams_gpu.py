@@ -48,3 +48,38 @@ def test_caches(lm, values):
     got = c.plan.values(cache, 600, values)
     c.d.torch.cuda.synchronize()
     assert want.any() and c.d.torch.equal(got.cpu(), want)
+
+
+def words(entries, rows, seqs):
+    """A batch's array: tokens, positions and sequence of each row, first rows, slots."""
+    host = np.zeros(3 * rows + 2 * seqs + 1, np.int32)
+    at = 0
+    for i, (slot, pos, n) in enumerate(entries):
+        host[rows + at:rows + at + n], host[2 * rows + at:2 * rows + at + n] = np.arange(pos, pos + n), i
+        at += n
+        host[3 * rows + i + 1], host[3 * rows + seqs + 1 + i] = at, slot
+    return host
+
+
+def test_a_recorded_portion_is_for_its_positions(lm):
+    """Replayed over a batch with other positions, or another slot, a longer portion is reported; over its own it is as good as ever."""
+    from tests.test_attention4_digits_gpu import want
+
+    c = Case(lm, 17, 8, 2, 64, 96, 700, 2, 400)
+    t = c.d.torch
+    c.append(1, 0, c.rows(300)), c.append(0, 0, c.rows(300))
+    entries = [(1, 200, 150)]
+    b = c.batch(entries, fixed=True)
+    proj = c.rows(150)
+    x, out = t.from_numpy(proj).to(c.d.dev), t.zeros(150, c.H * c.V, dtype=t.bfloat16, device=c.d.dev)
+    t.cuda.synchronize()
+    with lm.record() as g:
+        c.plan.run(b, x, c.kc, c.vc, out)
+    for now, status in (([(1, 200, 150)], 0), ([(1, 250, 150)], -1), ([(0, 200, 150)], -1), ([(1, 200, 150)], 0)):
+        b.write(words(now, 150, 1))
+        g.launch()
+        lm.sync()
+        assert lm.device_status() == status
+    y, bound = want(c, entries, proj)
+    assert (np.abs(out.float().cpu().numpy().reshape(y.shape) - y) <= bound).all()
+    g.free()
