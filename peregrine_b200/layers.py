@@ -44,7 +44,7 @@ class Device:
         self.code = _lib.BF16 if dtype == "bfloat16" else _lib.F32
         self.act = torch.bfloat16 if dtype == "bfloat16" else torch.float32
         self.rows = int(step_rows)
-        self._buffers = {}
+        self._buffers, self._outgrown = {}, []
         self.buffer("batch", 1, BATCH_WORDS(self.rows), torch.int32)
 
     def f32(self, a):
@@ -63,11 +63,14 @@ class Device:
         return t.from_numpy(np.array(a, np.float32)).to(self.dev).to(t.bfloat16)
 
     def buffer(self, name: str, cols: int, rows: int = 0, dtype=None):
-        """[rows, cols] zeroed; the same (name, cols) is the same memory."""
+        """[rows, cols] zeroed; the same (name, cols) is the same memory, until more rows are asked for (a graph may have been recorded
+        with the smaller one, which is kept)."""
         rows, dtype = rows or self.rows, dtype or self.act
         key = (name, cols, dtype)
         t = self._buffers.get(key)
         if t is None or t.shape[0] < rows:
+            if t is not None:
+                self._outgrown.append(t)
             t = self._buffers[key] = self.torch.zeros(rows, cols, dtype=dtype, device=self.dev)
             # torch clears it on a stream of its own, and the context's stream may be the next to write to it
             self.torch.cuda.current_stream(self.dev).synchronize()

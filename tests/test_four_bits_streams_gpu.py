@@ -83,3 +83,32 @@ def test_a_recorded_portion_is_for_its_positions(lm):
     y, bound = want(c, entries, proj)
     assert (np.abs(out.float().cpu().numpy().reshape(y.shape) - y) <= bound).all()
     g.free()
+
+
+def test_a_later_plan_leaves_a_recorded_one_its_workspaces(lm):
+    """A wider plan on the same device takes larger workspaces; what a graph was recorded with stays its own."""
+    from peregrine_b200.layers import Attention4Plan
+
+    c = Case(lm, 18, 8, 2, 64, 64, 3000, 2, 200)
+    t = c.d.torch
+    c.append(0, 0, c.rows(2500)), c.append(1, 0, c.rows(300))
+    entries = [(0, 2500, 2), (1, 300, 150)]
+    b = c.batch(entries, fixed=True)
+    proj = c.rows(152)
+    x, out = t.from_numpy(proj).to(c.d.dev), t.zeros(152, c.H * c.V, dtype=t.bfloat16, device=c.d.dev)
+    t.cuda.synchronize()
+    with lm.record() as g:
+        c.plan.run(b, x, c.kc, c.vc, out)
+    sizes = [c.d.buffer("attn4.part", 1, 1, t.float32).numel(), c.d.buffer("attn4.work", 1, 1).numel() // 2]
+    Attention4Plan(c.d, 8, 2, 64, 256, 9000, 2, 2, scale=1.0)
+    others = [t.full((n,), 9.0, device=c.d.dev) for n in sizes for _ in range(8)]
+    t.cuda.synchronize()
+    g.launch()
+    lm.sync()
+    assert all((o == 9.0).all() for o in others)
+    graph = out.clone()
+    t.cuda.synchronize()
+    c.plan.run(b, x, c.kc, c.vc, out)
+    lm.sync()
+    assert t.equal(out, graph) and lm.device_status() == 0
+    g.free()
