@@ -131,7 +131,7 @@ struct Piece {
 constexpr int LIST = 192;               // pieces of a route that a pair looks up before it begins
 
 // A warp's sums of weight rows n0 + lane with rows m0 .. of a (`left` of them exist) -> outputs
-template <int COLS, int ACT, bool ALL, typename TY>
+template <int COLS, bool ALL, typename TY>
 __device__ __forceinline__ void put_rows(const float (&v)[COLS], float fac, const float (&xback)[COLS / 16], int left, bool in, TY *dst, int64_t ldy)
 {
 #pragma unroll
@@ -154,9 +154,9 @@ __device__ __forceinline__ void put(const float (&v)[COLS], float fac, const flo
     if constexpr (ACT == PG_ACT_NONE) {
         TY *dst = y + (int64_t)m0 * ldy + n0 + lane;
         if (left >= COLS)
-            put_rows<COLS, ACT, true>(v, fac, xback, left, in, dst, ldy);
+            put_rows<COLS, true>(v, fac, xback, left, in, dst, ldy);
         else
-            put_rows<COLS, ACT, false>(v, fac, xback, left, in, dst, ldy);
+            put_rows<COLS, false>(v, fac, xback, left, in, dst, ldy);
     } else {
         // lanes l and l ^ 8 have a gate and its up: the gate's lane takes the even rows, the other the odd ones
         const bool up = lane & 8;
