@@ -9,15 +9,17 @@
 // O^T = V^T P^T, so that a lane's probabilities are the B operand as they come.  A byte belongs to one position: appending is byte stores.
 //
 //   few tokens of a sequence    attn4_few_kernel: streams the cache once, a block of 16 (token, head of the group) rows per CTA, the context in slices.
-//                               Keys as f16 (exact: a quant as the low bits of an f16 number) times the query as f16 over a power of two, sums of 32
-//                               columns scaled in f32; values as bf16 integers (exact) times bf16(probability * scale).  One token per sequence
+//                               Keys as f16 (exact: a quant as the low bits of an f16 number) times the query as f16 over a power of two (11 bits down to
+//                               2^-24 of the row's largest), sums of 32 columns scaled in f32; values as bf16 integers (exact) times
+//                               bf16(probability * scale).  One token per sequence
 //                               (FUSED): the CTA with the newest position quantises and appends it.  The last CTA of a (sequence, rows) to finish
 //                               merges the slices.  What bounds it, 32 + 8 heads of 128: instructions, 300 to a tile of 16 positions and 128 + 128
 //                               columns, of which 64 take the quants apart (four bits at a time, the integer pipe at half rate); 4 contexts of 30000 to
 //                               60000 71 us, 3.1 TB/s of 6.5, 16 of 2048 to 4096 31 us.  One of 2000: 10 us, a launch and seven dependent trips to
 //                               memory (positions, tiles, slices' sums, tickets, the merge).
 //   longer portions             attn4_append_kernel, then per sequence attn4_unfold_kernel and the kernels that prompts over a bf16 cache run through, on
-//                               f16: keys and values over a power of two of their head, which is exact, queries over one of their own.
+//                               f16: keys and values over a power of two of their head, which is exact, queries over one of their own, probabilities
+//                               times 2^7 (ATTN_P_UP).  The sequences go one after the other, each with its context unfolded into the same workspace.
 #include <algorithm>
 #include <type_traits>
 
@@ -377,6 +379,7 @@ constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // mos
 
 // CTAs to an SM.  More than eight rows of heads wider than 64: one with 255 registers a lane, as two with 128 spill (32 + 8 heads of 128, 16 x 4 tokens at
 // 4096: 36.7 us instead of 64).  Up to eight rows keep two: one is slower in long contexts (4 at 60000: 85 instead of 75), faster in short ones (2000: 8.3, 9.3).
+// Heads wider than 128 with more than eight rows spill some 450 bytes even so.
 __host__ __device__ constexpr int a4_per_sm(int gk, int gv, bool hi) { return gk > 4 || gv > 4 || (hi && gk + gv > 4) ? 1 : 2; }
 
 // part [blocks of rows][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row

@@ -5,8 +5,9 @@
 //   * The activations are bf16 and enter as f16: a warp divides each row of its part of K by a power of two of its own (four_range) and
 //     multiplies the sums back: exact down to 2^-27 of the part's largest, and smaller ones are off by 2^-36 of that at most.
 //   * One persistent CTA of 16 warps per SM.  `kw` warps share a tile of 16 weight rows, each with one part of K of at most 512 elements (256 with more than
-//     eight rows), whose activations it keeps in registers; a fill of its ring is one bulk copy, quants and scales.  The parts meet in shared memory
-//     in a fixed order; the warps of a tile take turns in adding.
+//     eight rows), whose activations it holds as operands, 64 words of a lane's 128 registers (parts of 512 do not quite fit: 156 to 236 bytes of a lane
+//     are kept in local memory; parts of 256: up to 48); a fill of its ring is one bulk copy, quants and scales.  The parts meet in shared memory in a
+//     fixed order; the warps of a tile take turns in adding.
 //   * K beyond 16 such parts: sp CTAs take the same tiles, their sums go to slabs, the last one in (a ticket) adds in a fixed order.
 //   * ROUTED: rows come in blocks of 16 that share an expert.
 //
@@ -27,7 +28,7 @@ constexpr int V4_WARPS = 16, V4_THREADS = V4_WARPS * 32;
 constexpr int V4_SLOTS_MAX = 8;
 constexpr int V4_CELLS = 4;                               // tiles whose parts may be on their way at once
 __host__ __device__ constexpr int v4_ring(int nt) { return nt == 1 ? 2 * 4608 : 4 * 2304; }    // bytes of a warp's ring
-__host__ __device__ constexpr int v4_kw_max(int nt) { return nt == 1 ? 512 : 256; }   // (what the registers hold of the activations)
+__host__ __device__ constexpr int v4_kw_max(int nt) { return nt == 1 ? 512 : 256; }   // (64 words of the activations to a lane)
 
 // shared memory: ring | parts of a tile [V4_CELLS][16 warps][32 lanes][4 NT] | barriers
 // slabs (K over several CTAs): [sp][items][32 lanes][4 NT]

@@ -287,7 +287,12 @@ def halving_slopes(heads: int) -> np.ndarray:
 
 class Attention4Plan:
     """Attention over keys and values in 4 bits (csrc/pg_attention4.cu): shape, workspaces and the calls of a step.  Caches are uint8
-    [slots, kv_heads, key_bytes] and [.., value_bytes]; cap: rows of a slot, positions: most positions of a sequence (0: cap)."""
+    [slots, kv_heads, key_bytes] and [.., value_bytes]; cap: rows of a slot, positions: most positions of a sequence (0: cap); max_seqs: most
+    sequences of a step, for which no workspace here grows.
+
+    Longer portions unfold one sequence's context to f16: a workspace of the device's, which its plans share, of kv_heads * cap * (dim + vdim) * 2
+    bytes and a little (537 MB for 8 heads of 128 and 131072 positions), in no pool's count.  It is made with the plan, so that no step can lack it.
+    A recorded longer portion is for the positions and the slot that it was recorded with."""
 
     def __init__(self, d: Device, heads: int, kv_heads: int, dim: int, vdim: int, cap: int, slots: int, max_seqs: int, scale: float, sink: bool = False, slopes=None,
                  chunk: int = 0, positions: int = 0, eps: float = 0.0, q_norm=None, k_norm=None, temp=(0.0, 0.0)):
