@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
                     const float sum = pg_warp_sum(__half2float(v));
                     if (lane < 2) reinterpret_cast<float *>(&offset[c & 7][i])[c / 8 * 2 + lane] = sum * -0x1p-21f;   // (the keys' quants are 8 too large)
                 }
-            if (lane == 0) back[c] = up * sl;
+            if (lane == 0) back[c] = up * sl * 0x1p12f;   // (half of the 2^24 of the scores' smallest steps, so that neither factor leaves the range)
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
                         for (int n = 0; n < 2; n++)
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
-                                float v = sc[h][n][2 * u + j] * 0x1p24f;
+                                float v = sc[h][n][2 * u + j] * 0x1p12f;
                                 v = s.slopes ? fmaf(v, fac[u], fmaf(bias[u], (float)(16 * h + 8 * n + j), b0)) : v * fac[u];
                                 if (edge) {
                                     const int x = jp + 16 * h + 8 * n + 2 * t + j;

@@ -133,3 +133,14 @@ def test_many_small_probabilities_beside_a_large_one(lm, H, G, D, V, kw):
     proj[:, H * D:(H + G) * D] = 0.0
     proj[:, (H + G) * D:] = np.abs(proj[:, (H + G) * D:]) + 1.0
     check(c, [(0, 300, n)], proj)
+
+
+@pytest.mark.parametrize("n", [1, 4, 150])
+@pytest.mark.parametrize("keys", [1e35, 1e-35])
+def test_keys_and_queries_of_opposite_sizes(lm, n, keys):
+    """Scores up to a hundred from keys at one end of the range and queries at the other."""
+    H, G, D, V = 8, 2, 64, 64
+    c = Case(lm, n, H, G, D, V, 600, 2, 400)
+    resize = lambda x: np.concatenate([x[:, :H * D] * 12 / keys, x[:, H * D:(H + G) * D] * keys, x[:, (H + G) * D:]], 1).astype(np.float32)
+    c.append(0, 0, resize(c.rows(300)))
+    check(c, [(0, 300, n)], resize(c.rows(n)))
