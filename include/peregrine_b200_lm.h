@@ -72,7 +72,7 @@ PG_API int32_t pg_linear4_free(pg_ctx *ctx, pg_linear4 *lin);
 PG_API int64_t pg_linear4_bytes(const pg_linear4 *lin);
 /* the weights' values, f32 [experts][n][k] */
 PG_API int32_t pg_linear4_read(pg_ctx *ctx, const pg_linear4 *lin, float *d_w);
-/* as pg_linear_run_ld; sums are of the bf16 activations with the weights' values, in f32 */
+/* as pg_linear_run_ld; sums are of the bf16 activations with the weights' values, in f32 (weights below 2^96, so that no sum of a part leaves the range) */
 PG_API int32_t pg_linear4_run(pg_ctx *ctx, const pg_linear4 *lin, const void *d_a, int64_t lda, int32_t dtype, int64_t m, int32_t act, float limit, void *d_y,
                               int32_t y_dtype, int64_t ldy);
 /* as pg_linear_run_routed */
