@@ -379,7 +379,7 @@ constexpr int A4_WARPS = 8, A4_STAGES = 3, A4_SLICES = 64, A4_FILL = 2;   // mos
 
 // CTAs to an SM.  More than eight rows of heads wider than 64: one with 255 registers a lane, as two with 128 spill (32 + 8 heads of 128, 16 x 4 tokens at
 // 4096: 36.7 us instead of 64).  Up to eight rows keep two: one is slower in long contexts (4 at 60000: 85 instead of 75), faster in short ones (2000: 8.3, 9.3).
-// Heads wider than 128 with more than eight rows spill some 450 bytes even so.
+// Heads wider than 128 with more than eight rows spill some 490 bytes even so.
 __host__ __device__ constexpr int a4_per_sm(int gk, int gv, bool hi) { return gk > 4 || gv > 4 || (hi && gk + gv > 4) ? 1 : 2; }
 
 // part [blocks of rows][slices][16][vs + 4]: sums, then maximum (log 2 units) and denominator of each row
@@ -652,6 +652,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
                 }
                 // to units of log 2, bias, mask
                 float top[NT];
+                uint32_t hidden = 0;                      // bit (2 h + n) 2 NT + 2 u + j
 #pragma unroll
                 for (int u = 0; u < NT; u++) {
                     top[u] = -INFINITY;
@@ -666,7 +667,7 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
                                 v = s.slopes ? fmaf(v, fac[u], fmaf(bias[u], (float)(16 * h + 8 * n + j), b0)) : v * fac[u];
                                 if (edge) {
                                     const int x = jp + 16 * h + 8 * n + 2 * t + j;
-                                    if (x < x0 || x >= t1 || x > seen[u]) v = -INFINITY;
+                                    if (x < x0 || x >= t1 || x > seen[u]) v = -INFINITY, hidden |= 1u << ((2 * h + n) * 2 * NT + 2 * u + j);
                                 }
                                 sc[h][n][2 * u + j] = v;
                                 top[u] = fmaxf(top[u], v);
@@ -713,8 +714,11 @@ __global__ void __launch_bounds__(A4_WARPS * 32, a4_per_sm(GK, GV, HI))
 #pragma unroll
                             for (int u = 0; u < NT; u++) {
                                 float p0 = sc[h][n][2 * u] * pg_bf16_lo(scales[n][x]), p1 = sc[h][n][2 * u + 1] * pg_bf16_hi(scales[n][x]);
-                                // (what a row does not see may hold anything)
-                                if (edge) p0 = sc[h][n][2 * u] == 0.0f ? 0.0f : p0, p1 = sc[h][n][2 * u + 1] == 0.0f ? 0.0f : p1;
+                                // (what a row does not see may hold anything; what it sees is not a number whatever its weight, 0 too)
+                                if (edge) {
+                                    const int bit = (2 * h + n) * 2 * NT + 2 * u;
+                                    p0 = hidden >> bit & 1u ? 0.0f : p0, p1 = hidden >> (bit + 1) & 1u ? 0.0f : p1;
+                                }
                                 b[u][n] = pg_pack_bf16(p0, p1);
                             }
                         }

@@ -144,3 +144,22 @@ def test_keys_and_queries_of_opposite_sizes(lm, n, keys):
     resize = lambda x: np.concatenate([x[:, :H * D] * 12 / keys, x[:, H * D:(H + G) * D] * keys, x[:, (H + G) * D:]], 1).astype(np.float32)
     c.append(0, 0, resize(c.rows(300)))
     check(c, [(0, 300, n)], resize(c.rows(n)))
+
+
+@pytest.mark.parametrize("n", [1, 3, 150])
+@pytest.mark.parametrize("at", [5, 40, 299, 300])
+def test_a_value_that_is_not_finite_is_seen_however_small_its_weight(lm, n, at):
+    """A position whose score is 300 below the others', with values that are not numbers: rows that see it say so, the others do not."""
+    H, G, D, V = 4, 2, 64, 64
+    c = Case(lm, n + at, H, G, D, V, 600, 1, 400)
+    rows = c.rows(300 + n)
+    rows[:, :(H + G) * D] = 0.0
+    rows[:, :H * D:D] = 150.0 / c.scale
+    rows[:, H * D:(H + G) * D:D] = 1.0
+    rows[at, H * D:(H + G) * D:D] = -1.0
+    rows[at, (H + G) * D + 40] = np.nan                       # head 0's value, columns 32 .. 63
+    c.append(0, 0, rows[:300])
+    bad = np.isnan(c.step([(0, 300, n)], rows[300:]).reshape(n, H, V))
+    sees = 300 + np.arange(n) >= at
+    assert (bad[:, :2, 32:] == sees[:, None, None]).all()
+    assert not bad[:, :2, :32].any() and not bad[:, 2:].any()
