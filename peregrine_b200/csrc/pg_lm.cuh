@@ -97,13 +97,26 @@ __device__ __forceinline__ float pg_gelu_tanh(float z)
     const float c = 0.7978845608028654f;   // sqrt(2 / pi)
     return 0.5f * z * (1.0f + tanhf(c * (z + 0.044715f * z * z * z)));
 }
+// the smaller and the larger of two, not-a-number where one of them is
+__device__ __forceinline__ float pg_min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float pg_max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // one gated output of a product (pg_act)
 template <int ACT>
 __device__ __forceinline__ float pg_glu(float g, float u, float limit)
 {
     if (ACT == PG_ACT_GELU_TANH_GLU) return pg_gelu_tanh(g) * u;
-    g = fminf(g, limit);
-    u = fminf(fmaxf(u, -limit), limit);
+    g = pg_min_nan(g, limit);
+    u = pg_min_nan(pg_max_nan(u, -limit), limit);
     return g * pg_sigmoid(1.702f * g) * (u + 1.0f);
 }
 // 2^x, within two units in the last place (results below 2^-126 become 0)
